@@ -5,5 +5,5 @@ thin Python host mirror of that ABI plus seeded synthetic inputs. There is no CP
 the library or a CUDA device is missing.
 """
 from . import synth  # noqa: F401
-from .redcuda import (MoeLayer, RedcudaError, deltanet_step, lib, nib_dequant_rows, quant_dequant_rows, quant_matmul_tc, quant_matvec,  # noqa: F401
-                      router_select_softmax_topk, set_codebooks)
+from .redcuda import (DeltaDims, MoeLayer, PagedKv, RedcudaError, delta_rule, delta_rule_device, delta_step_device, deltanet_step, device_status, lib,  # noqa: F401
+                      nib_dequant_rows, quant_dequant_rows, quant_matmul_tc, quant_matvec, router_select_softmax_topk, set_codebooks, token_logprobs, token_logprobs_device)

@@ -56,6 +56,10 @@ static std::once_flag g_status_once;
 uint32_t *status_words() {
     std::call_once(g_status_once, [] {
         void *p = nullptr;
+        // the first call may be one that is being captured: the allocation is no work of the stream
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        struct Restore { cudaStreamCaptureMode *m; ~Restore() { cudaThreadExchangeStreamCaptureMode(m); } } restore{&mode};
+        cudaThreadExchangeStreamCaptureMode(&mode);
         if (cudaHostAlloc(&p, ST_WORDS * sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { cudaGetLastError(); return; }
         memset(p, 0, ST_WORDS * sizeof(uint32_t));
         g_status = (uint32_t *)p;      // unified addressing: the host pointer is valid on every device
@@ -66,11 +70,15 @@ int status_failed() {
     volatile uint32_t *st = g_status;
     if (!st) return 0;
     const uint32_t a = st[ST_ROUTER_NONFINITE], b = st[ST_TOKEN_RANGE], c = st[ST_EXPERT_RANGE], d = st[ST_TIMEOUT];
-    if (!(a | b | c | d)) return 0;
-    st[ST_ROUTER_NONFINITE] = 0; st[ST_TOKEN_RANGE] = 0; st[ST_EXPERT_RANGE] = 0; st[ST_TIMEOUT] = 0;
+    const uint32_t pg = st[ST_PAGE_RANGE], sl = st[ST_SLOT], sq = st[ST_SEQ_BOUNDS];
+    if (!(a | b | c | d | pg | sl | sq)) return 0;
+    for (uint32_t i = 0; i < ST_WORDS; ++i) st[i] = 0;
     if (a) set_error("invalid router softmax denominator (non-finite router logits)");
     else if (b) set_error("token id out of range on the device (non-finite logits in the argmax?)");
     else if (c) set_error("an expert id outside this shard reached an expert kernel");
+    else if (pg) set_error("a position beyond a sequence's page table, or a page id outside the cache");
+    else if (sl) set_error("a state slot outside the states, or one that two sequences of a call share");
+    else if (sq) set_error("sequence bounds that do not ascend within the rows of the call");
     else set_error("an expert kernel gave up waiting for a weight copy (bounded wait ran out); its outputs are incomplete");
     return 1;
 }
@@ -564,6 +572,8 @@ int redcuda_profile_report(char *buf, size_t cap) {
     }
     return n;
 }
+
+int redcuda_device_status(void) { return status_failed() ? 0 : 1; }
 
 int redcuda_device_count(void) {
     int n = 0;

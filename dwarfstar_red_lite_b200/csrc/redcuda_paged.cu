@@ -1,0 +1,506 @@
+// A paged K/V cache: rows of prompts written to its pages, and attention of one new token per sequence over them.
+//
+//   k_kv_append     a warp per token: its K and V rows, converted, to the page that the table names
+//   k_kv_attend     decode attention over the sequences' whole lengths (below)
+//   k_kv_attend_join  sums the parts of sequences that several blocks worked on
+#include "redcuda_paged.cuh"
+#include "redcuda_stage.cuh"
+#include "../../include/redcuda.h"
+
+#include <math.h>
+
+namespace rc {
+
+struct AppendArgs {
+    void *k, *v;
+    uint64_t page_stride, token_stride, head_stride;
+    const int32_t *table, *start, *cu;
+    const void *k_new, *v_new;
+    uint64_t row_stride;
+    uint32_t table_width, page_size, n_pages, n_seqs, n_tokens, n_kv, hd;
+    uint32_t *status;
+};
+
+// What bounds it is the copy: a row read once, written once. A lane moves VEC values (16 bytes of the cache's type) of K and of V at a time.
+template <class C, class R>
+__global__ void __launch_bounds__(128) k_kv_append(AppendArgs A) {
+    pdl_prologue();
+    constexpr int VEC = 16 / sizeof(C), PART = 16 / sizeof(R) < VEC ? 16 / sizeof(R) : VEC;
+    const uint32_t lane = threadIdx.x & 31u, t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (t >= A.n_tokens) return;
+    uint32_t b = t, at = 0u;
+    if (A.cu) {
+        b = find_seq(A.cu, A.n_seqs, t);
+        if (b >= A.n_seqs) return;               // behind the last sequence
+        const int32_t lo = A.cu[b], hi = A.cu[b + 1u];
+        if (lo < 0 || (int32_t)t < lo || (int32_t)t >= hi) { if (A.status && lane == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
+        at = t - (uint32_t)lo;
+    }
+    const int32_t s = A.start[b];
+    if (s < 0) return;
+    const uint64_t pos = (uint64_t)(uint32_t)s + at, pi = pos / A.page_size;
+    const int32_t page = pi < A.table_width ? A.table[(uint64_t)b * A.table_width + pi] : -1;
+    if (page < 0 || (uint32_t)page >= A.n_pages) { if (A.status && lane == 0u) A.status[ST_PAGE_RANGE] = 1u; return; }
+    const uint64_t dst = (uint64_t)page * A.page_stride + (pos - pi * A.page_size) * A.token_stride, src = (uint64_t)t * A.row_stride;
+    const uint32_t n = A.n_kv * A.hd;
+#pragma unroll 2
+    for (uint32_t i = lane * VEC; i < n; i += 32u * VEC) {
+        const uint32_t h = i / A.hd;
+        const uint64_t d = dst + (uint64_t)h * A.head_stride + (i - h * A.hd);
+        float x[VEC / PART][PART], y[VEC / PART][PART];
+#pragma unroll
+        for (int p = 0; p < VEC / PART; ++p) {
+            load_vals<PART>(reinterpret_cast<const R *>(A.k_new) + src + i + p * PART, x[p]);
+            load_vals<PART>(reinterpret_cast<const R *>(A.v_new) + src + i + p * PART, y[p]);
+        }
+        store_vals<VEC>(reinterpret_cast<C *>(A.k) + d, *reinterpret_cast<float (*)[VEC]>(&x[0][0]));
+        store_vals<VEC>(reinterpret_cast<C *>(A.v) + d, *reinterpret_cast<float (*)[VEC]>(&y[0][0]));
+    }
+}
+
+template <class C, class R> static int launch_append(const AppendArgs &A, cudaStream_t s) {
+    RC_LAUNCH((k_kv_append<C, R>), (A.n_tokens + 3u) / 4u, 128, 0, s, A);
+    RC_LAUNCHED();
+    return 1;
+}
+template <class C> static int launch_append_rows(const AppendArgs &A, uint32_t in_type, cudaStream_t s) {
+    return in_type == VT_F32 ? launch_append<C, float>(A, s) : in_type == VT_F16 ? launch_append<C, __half>(A, s) : launch_append<C, __nv_bfloat16>(A, s);
+}
+
+// ---- decode attention -------------------------------------------------------------------------------------------------------
+// With x_p = scale log2(e) q . k_p, a part of the positions is summed up as m = max x_p, l = sum 2^(x_p - m), O = sum 2^(x_p - m) v_p; parts are joined
+// by rescaling to the common m, and out = O / l.
+//
+// The work is cut by bytes: a tile is 16 KB of K and V of one K/V head, all tiles of all (sequence, K/V head, group of 8 query heads) are
+// counted through in that order, and every block takes an equal run of them, whatever the lengths are: they are read on the device, so that a
+// captured call follows them. A run that begins or ends inside a sequence's head leaves (m, l, O) in the workspace, at most two of them a
+// block, for k_kv_attend_join; what a block has whole it writes itself. A warp has a ring of tiles of its own that cp.async fills (four warps x three
+// stages x 16 KB in flight a block), so that the warps of a block meet only where a head ends.
+
+// the positions of sequence b that can be attended to
+__device__ __forceinline__ uint32_t kv_len(const AttendArgs &A, uint32_t b) {
+    const int32_t n = A.lens[b];
+    const uint64_t most = (uint64_t)A.table_width * A.page_size;
+    return n <= 0 ? 0u : (uint64_t)(uint32_t)n > most ? (uint32_t)most : (uint32_t)n;
+}
+
+// One tile of a warp's ring: its rows requested, rows beyond the end or without a page as zeros. Returns the rows that count, as bits.
+template <class T, int HD>
+__device__ __forceinline__ uint64_t kv_request(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t len, uint32_t tile, uint32_t dst) {
+    using L = KvTile<T, HD>;
+    const uint32_t lane = threadIdx.x & 31u;
+    int64_t off[L::TPL];
+    uint64_t valid = 0;
+#pragma unroll
+    for (int j = 0; j < L::TPL; ++j) {
+        const uint32_t r = j * 32u + lane, pos = tile * L::TP + r;
+        off[j] = -1;
+        if (r < L::TP && pos < len) {
+            const uint32_t pi = pos / A.page_size;
+            const int32_t page = A.table[(uint64_t)b * A.table_width + pi];
+            if (page >= 0 && (uint32_t)page < A.n_pages)
+                off[j] = (int64_t)((uint64_t)page * A.page_stride + (uint64_t)(pos - pi * A.page_size) * A.token_stride + (uint64_t)kvh * A.head_stride);
+            else if (A.status) A.status[ST_PAGE_RANGE] = 1u;
+        }
+        valid |= (uint64_t)__ballot_sync(0xffffffffu, off[j] >= 0) << (32 * j);
+    }
+    const T *kb = reinterpret_cast<const T *>(A.k), *vb = reinterpret_cast<const T *>(A.v);
+#pragma unroll
+    for (int i = 0; i < (int)(L::TP * L::CPR / 32u); ++i) {
+        const uint32_t n = i * 32u + lane, row = n / L::CPR, c = n % L::CPR;
+        const int64_t o = __shfl_sync(0xffffffffu, off[(i * 32 / (int)L::CPR) / 32], (int)(row & 31u));
+        const uint32_t sz = o >= 0 ? 16u : 0u, to = dst + row * L::ROW + L::swizzle(row, c) * 16u;
+        const uint64_t src = (uint64_t)(o >= 0 ? o : 0) + c * (16u / sizeof(T));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(kb + src), "r"(sz) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to + L::TP * L::ROW), "l"(vb + src), "r"(sz) : "memory");
+    }
+    return valid;
+}
+
+// a warp's share of a part: every KV_WARPS-th tile of [t0, t1), 8 query heads; (m, l, O) to shared memory. The sums on CUDA cores.
+template <class T, class QT, int HD>
+__device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t h0, uint32_t nh, uint32_t len, uint32_t t0, uint32_t t1,
+                                            uint8_t *ring, uint64_t *valid, float *p_sh, float *m_out, float *l_out, float *o_out) {
+    using L = KvTile<T, HD>;
+    constexpr int E = HD / 32;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+    // element i of a lane: a 16-byte piece (or less) of the row, two pieces for rows of 1 KB
+    auto elem = [&](int i) { return E * sizeof(T) > 16 ? (uint32_t)(i / 4) * 128u + lane * 4u + (uint32_t)(i % 4) : lane * E + (uint32_t)i; };
+    float2 q[8][E / 2], o[8][E / 2];
+    const QT *qp = reinterpret_cast<const QT *>(A.q) + (uint64_t)b * A.q_stride + (uint64_t)h0 * HD;
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+            q[h][i / 2] = make_float2(0.f, 0.f);
+            if (h < (int)nh) q[h][i / 2] = make_float2(to_f32(qp[h * HD + elem(i)]) * A.scale_log2, to_f32(qp[h * HD + elem(i + 1)]) * A.scale_log2);
+            o[h][i / 2] = make_float2(0.f, 0.f);
+        }
+    float m = -INFINITY, l = 0.f;                // of head lane / 4; l: this lane's share
+    uint32_t next = t0 + warp;
+#pragma unroll
+    for (int s = 0; s < KV_STAGES - 1; ++s) {
+        if (next < t1) { const uint64_t w = kv_request<T, HD>(A, b, kvh, len, next, ring_s + s * L::BYTES); if (lane == 0u) valid[s] = w; }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next += KV_WARPS;
+    }
+    uint32_t st = 0;
+    for (uint32_t t = t0 + warp; t < t1; t += KV_WARPS) {
+        const uint32_t fill = st == 0u ? KV_STAGES - 1 : st - 1u;
+        asm volatile("cp.async.wait_group %0;" :: "n"(KV_STAGES - 2) : "memory");
+        __syncwarp();
+        if (next < t1) { const uint64_t w = kv_request<T, HD>(A, b, kvh, len, next, ring_s + fill * L::BYTES); if (lane == 0u) valid[fill] = w; }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next += KV_WARPS;
+        const uint64_t live = valid[st];
+        const uint8_t *kt = ring + st * L::BYTES, *vt = kt + L::TP * L::ROW;
+        auto row = [&](const uint8_t *base, uint32_t r, float2 (&x)[E / 2]) {
+#pragma unroll
+            for (int i = 0; i < E; i += (E * sizeof(T) > 16 ? 4 : E)) {
+                constexpr int N = E * sizeof(T) > 16 ? 4 : E;
+                const uint32_t byte = elem(i) * sizeof(T);
+                float y[N];
+                load_vals<N>(reinterpret_cast<const T *>(base + r * L::ROW + L::swizzle(r, byte / 16u) * 16u + byte % 16u), y);
+#pragma unroll
+                for (int j = 0; j < N; j += 2) x[(i + j) / 2] = make_float2(y[j], y[j + 1]);
+            }
+        };
+#pragma unroll 1
+        for (uint32_t r = 0; r < L::TP; r += 4u) {
+            const uint32_t bits = (uint32_t)(live >> r) & 15u;
+            if (!bits) continue;
+            float s[32];                         // score of head i / 4, position r + i % 4: this lane's part
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float2 k[E / 2];
+                row(kt, r + j, k);
+#pragma unroll
+                for (int h = 0; h < 8; ++h) {
+                    float2 a = __fmul2_rn(q[h][0], k[0]);
+#pragma unroll
+                    for (int i = 1; i < E / 2; ++i) a = __ffma2_rn(q[h][i], k[i], a);
+                    s[h * 4 + j] = a.x + a.y;
+                }
+            }
+            // 32 sums over 32 lanes: each exchange halves the values that a lane carries; value i ends in lane i
+#pragma unroll
+            for (int w = 16; w; w >>= 1) {
+                const bool hi = lane & w;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (i < w) {
+                        const float keep = hi ? s[w + i] : s[i], send = hi ? s[i] : s[w + i];
+                        s[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+                    }
+            }
+            const float x = (bits >> (lane & 3u)) & 1u ? s[0] : -INFINITY;
+            float mx = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn, alpha = exp2f(m - base), p = exp2f(x - base);
+            const bool moved = __any_sync(0xffffffffu, mn > m);
+            m = mn;
+            l = l * alpha + p;
+            __syncwarp();
+            p_sh[lane] = p;
+            if ((lane & 3u) == 0u) p_sh[32u + lane / 4u] = alpha;
+            __syncwarp();
+            if (moved) {
+#pragma unroll
+                for (int h = 0; h < 8; ++h) {
+                    const float a = p_sh[32 + h];
+#pragma unroll
+                    for (int i = 0; i < E / 2; ++i) o[h][i] = __fmul2_rn(o[h][i], make_float2(a, a));
+                }
+            }
+            float2 v[4][E / 2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) row(vt, r + j, v[j]);
+#pragma unroll
+            for (int h = 0; h < 8; ++h) {
+                const float4 p4 = *reinterpret_cast<const float4 *>(p_sh + h * 4);
+#pragma unroll
+                for (int i = 0; i < E / 2; ++i) {
+                    o[h][i] = __ffma2_rn(make_float2(p4.x, p4.x), v[0][i], o[h][i]);
+                    o[h][i] = __ffma2_rn(make_float2(p4.y, p4.y), v[1][i], o[h][i]);
+                    o[h][i] = __ffma2_rn(make_float2(p4.z, p4.z), v[2][i], o[h][i]);
+                    o[h][i] = __ffma2_rn(make_float2(p4.w, p4.w), v[3][i], o[h][i]);
+                }
+            }
+        }
+        __syncwarp();
+        st = st + 1u == KV_STAGES ? 0u : st + 1u;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if ((lane & 3u) == 0u) { m_out[lane / 4u] = m; l_out[lane / 4u] = l; }
+    __syncthreads();                             // the rings are read no more
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+#pragma unroll
+        for (int i = 0; i < E; i += 2) { o_out[h * HD + elem(i)] = o[h][i / 2].x; o_out[h * HD + elem(i + 1)] = o[h][i / 2].y; }
+}
+
+// the new row of sequence b, K/V head kvh, to its page (the whole block)
+template <class T, class QT, int HD>
+__device__ __forceinline__ void kv_write_new(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t pos) {
+    const uint32_t pi = pos / A.page_size;
+    const int32_t page = A.table[(uint64_t)b * A.table_width + pi];
+    if (page < 0 || (uint32_t)page >= A.n_pages) return;       // reported where the row is read
+    const uint64_t d = (uint64_t)page * A.page_stride + (uint64_t)(pos - pi * A.page_size) * A.token_stride + (uint64_t)kvh * A.head_stride;
+    const uint64_t s = (uint64_t)b * A.new_stride + (uint64_t)kvh * HD;
+    for (uint32_t i = threadIdx.x; i < 2u * HD; i += blockDim.x) {
+        const uint32_t e = i % HD;
+        const QT *from = reinterpret_cast<const QT *>(i < HD ? A.k_new : A.v_new);
+        reinterpret_cast<T *>(i < HD ? A.k : A.v)[d + e] = from_f32<T>(to_f32(from[s + e]));
+    }
+}
+
+template <class T, class QT, int HD>
+__global__ void __launch_bounds__(KV_WARPS * 32, 1) k_kv_attend(AttendArgs A) {
+    pdl_prologue();
+    using L = KvTile<T, HD>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint64_t s_sum[KV_WARPS], s_base, s_valid[KV_WARPS][KV_STAGES];
+    __shared__ uint32_t s_b;
+    __shared__ __align__(16) float s_p[KV_WARPS][40], s_m[KV_WARPS][8], s_l[KV_WARPS][8];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, HG = A.n_kv * A.gsplit;
+    QT *const out = reinterpret_cast<QT *>(A.out);
+
+    // how many tiles there are, and the sequence in which this block's run begins
+    const uint32_t per = (A.n_seqs + KV_WARPS * 32u - 1u) / (KV_WARPS * 32u), b_lo = min(A.n_seqs, tid * per), b_hi = min(A.n_seqs, b_lo + per);
+    uint64_t mine = 0;
+    for (uint32_t b = b_lo; b < b_hi; ++b) mine += (kv_len(A, b) + L::TP - 1u) / L::TP;
+    uint64_t incl = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) { const uint64_t x = __shfl_up_sync(0xffffffffu, incl, w); if (lane >= (uint32_t)w) incl += x; }
+    if (lane == 31u) s_sum[warp] = incl;
+    __syncthreads();
+    uint64_t total = 0;
+    for (uint32_t w = 0; w < KV_WARPS; ++w) { if (w < warp) incl += s_sum[w]; total += s_sum[w]; }
+    total *= HG;
+    const uint64_t q = max((total + gridDim.x - 1u) / gridDim.x, (uint64_t)KV_MIN_TILES), u0 = q * blockIdx.x, u1 = min(total, u0 + q);
+    uint64_t base = (incl - mine) * HG;
+    if (u0 < u1 && base <= u0 && u0 < incl * HG) {
+        uint32_t b = b_lo;
+        for (;; ++b) { const uint64_t n = (uint64_t)((kv_len(A, b) + L::TP - 1u) / L::TP) * HG; if (u0 < base + n) break; base += n; }
+        s_b = b; s_base = base;
+    }
+    for (uint32_t b = blockIdx.x; b < A.n_seqs; b += gridDim.x) {
+        if (A.status && tid == 0u && A.lens[b] > 0 && (uint32_t)A.lens[b] != kv_len(A, b)) A.status[ST_PAGE_RANGE] = 1u;
+        if (kv_len(A, b) == 0u) {                // nothing to attend to
+            for (uint32_t i = tid; i < A.n_q * HD; i += KV_WARPS * 32u) out[(uint64_t)b * A.n_q * HD + i] = from_f32<QT>(0.f);
+            if (A.lse) for (uint32_t i = tid; i < A.n_q; i += KV_WARPS * 32u) A.lse[(uint64_t)b * A.n_q + i] = -INFINITY;
+        }
+    }
+    __syncthreads();
+    uint32_t parts_b = 0, parts_h = 0, parts_n = 0;            // the head that begins here and ends in a later block
+    if (u0 < u1) {
+        uint32_t b = s_b;
+        base = s_base;
+        uint64_t u = u0;
+        while (u < u1) {
+            const uint32_t len = kv_len(A, b), nt = (len + L::TP - 1u) / L::TP;
+            if (u >= base + (uint64_t)nt * HG) { base += (uint64_t)nt * HG; ++b; continue; }
+            const uint32_t hg = (uint32_t)((u - base) / nt), t0 = (uint32_t)((u - base) - (uint64_t)hg * nt), t1 = (uint32_t)min((uint64_t)nt, t0 + (u1 - u));
+            const uint32_t kvh = hg / A.gsplit, g0 = (hg % A.gsplit) * 8u, h0 = kvh * A.G + g0, nh = min(8u, A.G - g0);
+            if (A.k_new && t1 == nt && len == (uint32_t)A.lens[b]) kv_write_new<T, QT, HD>(A, b, kvh, len - 1u);
+            __syncthreads();                     // the new row is written; what the last head left in shared memory has been read
+            float *o_sh = reinterpret_cast<float *>(sm);
+            attend_part_f32<T, QT, HD>(A, b, kvh, h0, nh, len, t0, t1, sm + warp * KV_STAGES * L::BYTES, s_valid[warp], s_p[warp], s_m[warp], s_l[warp], o_sh + warp * 8u * HD);
+            __syncthreads();
+            // the warps' parts together
+            const bool whole = t0 == 0u && t1 == nt;
+            const uint32_t slot = blockIdx.x * 2u + (t0 == 0u ? 1u : 0u);
+            for (uint32_t i = tid; i < 8u * HD; i += KV_WARPS * 32u) {
+                const uint32_t h = i / HD;
+                float M = s_m[0][h], sum = 0.f, w[KV_WARPS], lt = 0.f;
+#pragma unroll
+                for (uint32_t j = 1; j < KV_WARPS; ++j) M = fmaxf(M, s_m[j][h]);
+                const float z = M == -INFINITY ? 0.f : M;
+#pragma unroll
+                for (uint32_t j = 0; j < KV_WARPS; ++j) { w[j] = exp2f(s_m[j][h] - z); sum += w[j] * o_sh[j * 8u * HD + i]; lt += w[j] * s_l[j][h]; }
+                if (whole) {
+                    if (h < nh) {
+                        out[((uint64_t)b * A.n_q + h0) * HD + i] = from_f32<QT>(lt == 0.f ? 0.f : sum / lt);
+                        if (A.lse && i % HD == 0u) A.lse[(uint64_t)b * A.n_q + h0 + h] = lt == 0.f ? -INFINITY : M * 0.693147180559945309f + logf(lt);
+                    }
+                } else {
+                    A.part[(uint64_t)slot * 8u * HD + i] = sum;
+                    if (i % HD == 0u) { A.part_ml[slot * 16u + h] = M; A.part_ml[slot * 16u + 8u + h] = lt; }
+                }
+            }
+            if (t0 == 0u && t1 < nt) { parts_b = b; parts_h = hg; parts_n = (uint32_t)((base + (uint64_t)(hg + 1u) * nt - 1u) / q) - blockIdx.x; }
+            u += t1 - t0;
+        }
+    }
+    if (tid == 0u) { A.meta[blockIdx.x * 4u] = parts_b; A.meta[blockIdx.x * 4u + 1u] = parts_h; A.meta[blockIdx.x * 4u + 2u] = parts_n; }
+}
+
+// grid (blocks of k_kv_attend, 8 heads): the head that begins in block x, if it ends in a later one
+template <class QT, int HD>
+__global__ void __launch_bounds__(128) k_kv_attend_join(AttendArgs A) {
+    pdl_prologue();
+    extern __shared__ float s_w[];               // a weight for every part
+    __shared__ float s_red[4], s_l;
+    const uint32_t c = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, n = A.meta[c * 4u + 2u];
+    if (n == 0u) return;
+    const uint32_t b = A.meta[c * 4u], hg = A.meta[c * 4u + 1u], g0 = (hg % A.gsplit) * 8u, head = (hg / A.gsplit) * A.G + g0 + h;
+    if (g0 + h >= A.G) return;
+    auto slot = [&](uint32_t p) { return p == 0u ? c * 2u + 1u : (c + p) * 2u; };
+    float M = -INFINITY;
+    for (uint32_t p = tid; p <= n; p += 128u) M = fmaxf(M, A.part_ml[slot(p) * 16u + h]);
+    for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+    if ((tid & 31u) == 0u) s_red[tid >> 5] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float z = M == -INFINITY ? 0.f : M;
+    for (uint32_t p = tid; p <= n; p += 128u) s_w[p] = exp2f(A.part_ml[slot(p) * 16u + h] - z);
+    __syncthreads();
+    if (tid < 32u) {
+        float l = 0.f;
+        for (uint32_t p = tid; p <= n; p += 32u) l += s_w[p] * A.part_ml[slot(p) * 16u + 8u + h];
+        for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+        if (tid == 0u) { s_l = l; if (A.lse) A.lse[(uint64_t)b * A.n_q + head] = l == 0.f ? -INFINITY : M * 0.693147180559945309f + logf(l); }
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < HD; i += 128u) {
+        float sum = 0.f;
+#pragma unroll 8
+        for (uint32_t p = 0; p <= n; ++p) sum += s_w[p] * A.part[((uint64_t)slot(p) * 8u + h) * HD + i];
+        reinterpret_cast<QT *>(A.out)[((uint64_t)b * A.n_q + head) * HD + i] = from_f32<QT>(s_l == 0.f ? 0.f : sum / s_l);
+    }
+}
+
+template <class T, class QT, int HD> static int launch_attend(const AttendArgs &A, uint32_t blocks, cudaStream_t s) {
+    constexpr size_t smem = (size_t)KV_WARPS * KV_STAGES * KvTile<T, HD>::BYTES;
+    static std::atomic<uint64_t> set{0};          // devices on which the limit has been raised
+    int dev = 0;
+    RC_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1u)) {
+        RC_CUDA(cudaFuncSetAttribute(k_kv_attend<T, QT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    prof_begin("kv_attend", s);
+    RC_LAUNCH((k_kv_attend<T, QT, HD>), blocks, KV_WARPS * 32, smem, s, A);
+    RC_LAUNCHED();
+    prof_end(s);
+    prof_begin("kv_attend_join", s);
+    RC_LAUNCH((k_kv_attend_join<QT, HD>), dim3(blocks, 8), 128, (blocks + 1u) * sizeof(float), s, A);
+    RC_LAUNCHED();
+    prof_end(s);
+    return 1;
+}
+template <class T, class QT> static int launch_attend_hd(const AttendArgs &A, uint32_t hd, uint32_t blocks, cudaStream_t s) {
+    return hd == 256u ? launch_attend<T, QT, 256>(A, blocks, s) : hd == 128u ? launch_attend<T, QT, 128>(A, blocks, s) : launch_attend<T, QT, 64>(A, blocks, s);
+}
+
+// the cache's strides in elements (0: dense), or a message
+static int kv_check(const redcuda_paged_kv *kv, const char *who, uint64_t (&st)[3]) {
+    RC_REQUIRE(kv && kv->k && kv->v, "%s: null cache", who);
+    const uint32_t size = val_size(kv->type);
+    RC_REQUIRE(size, "%s: cache type %u is none of F32, F16, BF16", who, kv->type);
+    RC_REQUIRE(kv->head_dim == 64u || kv->head_dim == 128u || kv->head_dim == 256u, "%s: heads of %u values (64, 128 or 256 are served)", who, kv->head_dim);
+    RC_REQUIRE(kv->n_kv && kv->n_kv <= 65535u && kv->page_size && kv->page_size <= 0x7fffffffu && kv->n_pages && kv->n_pages <= 0x7fffffffu, "%s: empty or too large cache", who);
+    const bool dense = !kv->page_stride && !kv->token_stride && !kv->head_stride;
+    st[2] = dense ? kv->head_dim : kv->head_stride;
+    st[1] = dense ? (uint64_t)kv->n_kv * kv->head_dim : kv->token_stride;
+    st[0] = dense ? st[1] * kv->page_size : kv->page_stride;
+    for (int i = 0; i < 3; ++i)
+        RC_REQUIRE(st[i] >= kv->head_dim && st[i] * size % 16u == 0u && st[i] < (1ull << 46), "%s: cache stride %llu (a multiple of 16 bytes, at least a head)", who, (unsigned long long)st[i]);
+    RC_REQUIRE((uint64_t)kv->n_pages * st[0] < (1ull << 46), "%s: cache too large", who);
+    RC_REQUIRE(aligned16(kv->k) && aligned16(kv->v), "%s: cache pointers are not 16-byte aligned", who);
+    return 1;
+}
+
+static uint64_t attend_workspace(uint32_t blocks, uint32_t hd) { return (uint64_t)blocks * (2u * (8u * hd + 16u) * 4u + 16u); }
+
+}  // namespace rc
+
+using namespace rc;
+
+extern "C" {
+
+int redcuda_kv_append_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *start_dev,
+                             uint32_t n_tokens, const int32_t *cu_seqlens_dev, uint32_t in_type, const void *k_dev, const void *v_dev, uint64_t row_stride,
+                             void *stream) {
+    uint64_t st[3];
+    if (!kv_check(kv, "kv append", st)) return 0;
+    RC_REQUIRE(table_dev && start_dev && k_dev && v_dev && n_seqs && table_width, "kv append: null or empty argument");
+    RC_REQUIRE(val_size(in_type), "kv append: rows of type %u (F32, F16 or BF16 are served)", in_type);
+    RC_REQUIRE(n_seqs < 0x7fffffffu && n_tokens < 0x7fffffffu && table_width < 0x7fffffffu, "kv append: too many rows");
+    RC_REQUIRE(cu_seqlens_dev || n_tokens == n_seqs, "kv append: %u rows for %u sequences without bounds", n_tokens, n_seqs);
+    const uint64_t row = (uint64_t)kv->n_kv * kv->head_dim;
+    if (!row_stride) row_stride = row;
+    RC_REQUIRE(row_stride >= row && row_stride * val_size(in_type) % 16u == 0u && row_stride < (1ull << 32), "kv append: row stride %llu", (unsigned long long)row_stride);
+    RC_REQUIRE(aligned16(k_dev) && aligned16(v_dev), "kv append: rows are not 16-byte aligned");
+    if (!require_device()) return 0;
+    if (!n_tokens) return 1;
+    AppendArgs A{kv->k, kv->v, st[0], st[1], st[2], table_dev, start_dev, cu_seqlens_dev, k_dev, v_dev, row_stride, table_width, kv->page_size, kv->n_pages, n_seqs, n_tokens, kv->n_kv,
+                 kv->head_dim, status_words()};
+    cudaStream_t s = (cudaStream_t)stream;
+    prof_begin("kv_append", s);
+    const int ok = kv->type == VT_F32 ? launch_append_rows<float>(A, in_type, s) : kv->type == VT_F16 ? launch_append_rows<__half>(A, in_type, s) : launch_append_rows<__nv_bfloat16>(A, in_type, s);
+    prof_end(s);
+    return ok;
+}
+
+uint64_t redcuda_kv_attend_workspace(const redcuda_paged_kv *kv, uint32_t n_q) {
+    uint64_t st[3];
+    if (!kv_check(kv, "kv attend", st)) return 0;
+    RC_REQUIRE(n_q && n_q % kv->n_kv == 0u, "kv attend: %u query heads over %u K/V heads", n_q, kv->n_kv);
+    if (!require_device()) return 0;
+    const uint32_t sms = sm_count();
+    RC_REQUIRE(sms, "kv attend: the device's size is not known");
+    return attend_workspace(sms, kv->head_dim);
+}
+
+int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *lens_dev,
+                             uint32_t n_q, uint32_t q_type, const void *q_dev, uint64_t q_stride, const void *k_new_dev, const void *v_new_dev,
+                             uint64_t new_stride, float scale, void *out_dev, float *lse_dev, void *workspace_dev, uint64_t workspace_bytes, void *stream) {
+    uint64_t st[3];
+    if (!kv_check(kv, "kv attend", st)) return 0;
+    RC_REQUIRE(table_dev && lens_dev && q_dev && out_dev && n_seqs && table_width, "kv attend: null or empty argument");
+    RC_REQUIRE((k_new_dev != nullptr) == (v_new_dev != nullptr), "kv attend: a new key without a value, or a value without a key");
+    RC_REQUIRE(n_q && n_q <= 65535u && n_q % kv->n_kv == 0u, "kv attend: %u query heads over %u K/V heads", n_q, kv->n_kv);
+    RC_REQUIRE(n_seqs < 0x7fffffffu && table_width < 0x7fffffffu, "kv attend: too many sequences or pages");
+    RC_REQUIRE((uint64_t)table_width * kv->page_size < (1ull << 32), "kv attend: a page table of more than 2^32 positions");
+    RC_REQUIRE(q_type == kv->type || (q_type == VT_F32 && kv->type == VT_F16), "kv attend: queries of type %u over a cache of type %u (F32 over F32 or F16, or the cache's own type)", q_type, kv->type);
+    const uint32_t qs = val_size(q_type), hd = kv->head_dim;
+    const uint64_t qrow = (uint64_t)n_q * hd, nrow = (uint64_t)kv->n_kv * hd;
+    if (!q_stride) q_stride = qrow;
+    if (!new_stride) new_stride = nrow;
+    RC_REQUIRE(q_stride >= qrow && q_stride * qs % 16u == 0u && q_stride < (1ull << 32) && new_stride >= nrow && new_stride * qs % 16u == 0u && new_stride < (1ull << 32),
+               "kv attend: row strides %llu and %llu (multiples of 16 bytes, at least a row)", (unsigned long long)q_stride, (unsigned long long)new_stride);
+    RC_REQUIRE(aligned16(q_dev) && aligned16(k_new_dev) && aligned16(v_new_dev) && aligned16(out_dev) && aligned16(workspace_dev), "kv attend: a pointer is not 16-byte aligned");
+    const uint64_t out_bytes = (uint64_t)n_seqs * qrow * qs;
+    RC_REQUIRE(!overlap(out_dev, out_bytes, q_dev, span_bytes(n_seqs, q_stride, qrow, qs)) && !overlap(out_dev, out_bytes, k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) &&
+               !overlap(out_dev, out_bytes, v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)), "kv attend: the output lies inside the inputs");
+    RC_REQUIRE(!(scale != scale), "kv attend: scale is not a number");
+    if (!require_device()) return 0;
+    const uint32_t sms = sm_count();
+    RC_REQUIRE(sms, "kv attend: the device's size is not known");
+    RC_REQUIRE(workspace_dev && workspace_bytes >= attend_workspace(sms, hd), "kv attend: a workspace of %llu bytes is needed", (unsigned long long)attend_workspace(sms, hd));
+    AttendArgs A{};
+    A.k = kv->k; A.v = kv->v; A.page_stride = st[0]; A.token_stride = st[1]; A.head_stride = st[2];
+    A.table = table_dev; A.table_width = table_width; A.page_size = kv->page_size; A.n_pages = kv->n_pages;
+    A.lens = lens_dev; A.n_seqs = n_seqs; A.n_kv = kv->n_kv; A.n_q = n_q; A.G = n_q / kv->n_kv; A.gsplit = (A.G + 7u) / 8u;
+    A.q = q_dev; A.q_stride = q_stride; A.k_new = k_new_dev; A.v_new = v_new_dev; A.new_stride = new_stride;
+    A.scale_log2 = (float)((scale == 0.f ? 1.0 / sqrt((double)hd) : (double)scale) * 1.4426950408889634074);
+    A.out = out_dev; A.lse = lse_dev; A.status = status_words();
+    // no more blocks than there can be runs of tiles
+    const uint64_t tile = 8192u / (hd * val_size(kv->type)), tiles = ((uint64_t)table_width * kv->page_size + tile - 1u) / tile;
+    auto few = [](uint64_t n) { return n < 8192u ? n : 8192u; };      // more than that of one thing is blocks enough
+    const uint64_t runs = (few(tiles) * few(n_seqs) * few(A.n_kv * A.gsplit) + KV_MIN_TILES - 1u) / KV_MIN_TILES;
+    const uint32_t blocks = runs < sms ? (uint32_t)runs : sms;
+    A.part = (float *)workspace_dev;
+    A.part_ml = A.part + (size_t)blocks * 2u * 8u * hd;
+    A.meta = (uint32_t *)(A.part_ml + (size_t)blocks * 2u * 16u);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (kv->type == VT_F32) return launch_attend_hd<float, float>(A, hd, blocks, s);
+    if (kv->type == VT_BF16) return launch_attend_hd<__nv_bfloat16, __nv_bfloat16>(A, hd, blocks, s);
+    return q_type == VT_F32 ? launch_attend_hd<__half, float>(A, hd, blocks, s) : launch_attend_hd<__half, __half>(A, hd, blocks, s);
+}
+
+}  // extern "C"

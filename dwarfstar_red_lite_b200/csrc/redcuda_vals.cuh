@@ -1,0 +1,73 @@
+// The value types of the batch operators' rows (F32, F16, BF16 by ggml id): loads as floats, stores rounded to nearest even, and what their
+// entry points check on the host.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "redcuda_common.cuh"
+
+namespace rc {
+
+constexpr uint32_t VT_F32 = 0u, VT_F16 = 1u, VT_BF16 = 30u;       // ggml ids
+inline uint32_t val_size(uint32_t t) { return t == VT_F32 ? 4u : t == VT_F16 || t == VT_BF16 ? 2u : 0u; }
+
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+inline bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+    return a && b && na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+// bytes of `rows` rows of n elements that lie `stride` elements apart
+inline uint64_t span_bytes(uint64_t rows, uint64_t stride, uint64_t n, uint32_t size) { return rows ? ((rows - 1u) * stride + n) * size : 0u; }
+// streaming multiprocessors of the current device (0: unknown)
+inline uint32_t sm_count() {
+    static std::atomic<uint32_t> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0u;
+    uint32_t c = known[dev].load(std::memory_order_relaxed);
+    if (!c && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(c = (uint32_t)n, std::memory_order_relaxed);
+    return c;
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// N neighbouring values, aligned to N values
+template <class T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+template <int N, class T> __device__ __forceinline__ void load_vals(const T *p, float (&x)[N]) {
+    static_assert(N * sizeof(T) <= 16, "one load");
+    const Pack<T, N> a = *reinterpret_cast<const Pack<T, N> *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f32(a.v[i]);
+}
+template <int N, class T> __device__ __forceinline__ void store_vals(T *p, const float (&x)[N]) {
+    static_assert(N * sizeof(T) <= 16, "one store");
+    Pack<T, N> a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.v[i] = from_f32<T>(x[i]);
+    *reinterpret_cast<Pack<T, N> *>(p) = a;
+}
+
+// The sequence that row t belongs to: the last b with cu[b] <= t, found by a whole warp, 32 entries a step; n_seqs or more: behind the last one,
+// ~0u: ahead of the first. Only ascending bounds are searched right; others give some b, which the caller holds against cu[b] and cu[b + 1].
+__device__ __forceinline__ uint32_t find_seq(const int32_t *cu, uint32_t n_seqs, uint32_t t) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t lo = 0u, n = n_seqs + 1u;           // entries lo .. lo + n - 1 are open
+    bool first = true;
+    while (n > 1u || first) {
+        const uint32_t step = (n + 31u) / 32u, i = lane * step;
+        const bool le = i < n && cu[lo + i] <= (int32_t)t;
+        const uint32_t m = __ballot_sync(0xffffffffu, le);
+        if (first && !(m & 1u)) return ~0u;
+        first = false;
+        const uint32_t at = (m ? 31u - (uint32_t)__clz((int)m) : 0u) * step;
+        n = min(step, n - at); lo += at;
+    }
+    return lo;
+}
+#endif
+
+}  // namespace rc

@@ -20,6 +20,8 @@ EXPORTS = [
     "redcuda_moe_create", "redcuda_moe_destroy", "redcuda_moe_resident_bytes", "redcuda_moe_forward",
     "redcuda_moe_forward_device", "redcuda_moe_route_device", "redcuda_moe_experts_device", "redcuda_moe_shared_device",
     "redcuda_moe_combine_device", "redcuda_moe_partial_device",
+    "redcuda_device_status", "redcuda_kv_append_device", "redcuda_kv_attend_workspace", "redcuda_kv_attend_device", "redcuda_delta_step_device",
+    "redcuda_delta_rule_workspace", "redcuda_delta_rule_device", "redcuda_delta_rule", "redcuda_token_logprobs_device", "redcuda_token_logprobs",
     "redcuda_launch_count", "redcuda_profile_enable", "redcuda_profile_report",
     "redcuda_ep_unique_id", "redcuda_ep_ipc_handle", "redcuda_ep_attach_peers", "redcuda_ep_detach_peers", "redcuda_ep_create", "redcuda_ep_destroy", "redcuda_ep_layer_forward", "redcuda_ep_layer_forward_n", "redcuda_ep_last_ids_device", "redcuda_ep_step", "redcuda_engine_shard", "redcuda_engine_attach_ep",
     # engine ABI (include/rl_engine.h)
@@ -45,6 +47,20 @@ class MoeDesc(C.Structure):
                                           "expert_begin", "expert_count", "max_tokens", "weights_on_device"]] + \
                [("router", C.c_void_p), ("gate_exps", C.c_void_p), ("up_exps", C.c_void_p), ("down_exps", C.c_void_p),
                 ("sh_gate_inp", C.c_void_p), ("sh_gate", C.c_void_p), ("sh_up", C.c_void_p), ("sh_down", C.c_void_p), ("expert_stride", C.c_uint32)]
+
+
+class PagedKvDesc(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ["type", "n_kv", "head_dim", "page_size", "n_pages"]] + \
+               [(n, C.c_uint64) for n in ["page_stride", "token_stride", "head_stride"]] + [("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class DeltaDims(C.Structure):
+    """Shapes of the gated delta rule: DeltaDims(type, n_group, dt_rank, d_state[, q_stride, k_stride, v_stride, scale])."""
+    _fields_ = [(n, C.c_uint32) for n in ["type", "n_group", "dt_rank", "d_state"]] + [(n, C.c_uint64) for n in ["q_stride", "k_stride", "v_stride"]] + [("scale", C.c_float)]
+
+    def workspace(self, n_tokens: int, n_seqs: int) -> int:
+        """Bytes of device workspace that delta_rule_device needs for so many tokens and sequences (0: none)."""
+        return int(lib().redcuda_delta_rule_workspace(C.byref(self), n_tokens, n_seqs))
 
 
 _lib = None
@@ -95,6 +111,18 @@ def lib():
     L.redcuda_engine_shard.argtypes = [C.c_int, C.c_int]
     L.redcuda_engine_attach_ep.argtypes = [C.c_void_p, C.c_void_p]
     L.redcuda_ep_step.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    P, U, U64, F = C.c_void_p, C.c_uint32, C.c_uint64, C.c_float
+    L.redcuda_kv_append_device.argtypes = [P, P, U, U, P, U, P, U, P, P, U64, P]
+    L.redcuda_kv_attend_workspace.restype = U64
+    L.redcuda_kv_attend_workspace.argtypes = [P, U]
+    L.redcuda_kv_attend_device.argtypes = [P, P, U, U, P, U, U, P, U64, P, P, U64, F, P, P, P, U64, P]
+    L.redcuda_delta_step_device.argtypes = [P, U, P, U, P, P, P, P, P, P, P, P]
+    L.redcuda_delta_rule_workspace.restype = U64
+    L.redcuda_delta_rule_workspace.argtypes = [P, U, U]
+    L.redcuda_delta_rule_device.argtypes = [P, U, U, P, P, U, P, P, P, P, P, P, P, P, U64, P]
+    L.redcuda_delta_rule.argtypes = [P, U, U, P, P, U, P, P, P, P, P, P, P]
+    L.redcuda_token_logprobs_device.argtypes = [U, U, U, U64, P, P, U, P, P, P, P, P]
+    L.redcuda_token_logprobs.argtypes = [U, U, U, U64, P, P, U, P, P, P, P]
     L.redcuda_profile_enable.argtypes = [C.c_int]
     L.redcuda_profile_report.argtypes = [C.c_char_p, C.c_size_t]
     L.redcuda_set_device.argtypes = [C.c_int]
@@ -254,6 +282,94 @@ def deltanet_step(p: dict, qkv: np.ndarray, z: np.ndarray, ba: np.ndarray, conv_
     _check(lib().redcuda_deltanet_step(C.byref(P), B, qkv.ctypes.data, z.ctypes.data, ba.ctypes.data, conv_state.ctypes.data,
                                        rec_state.ctypes.data, out.ctypes.data))
     return out
+
+
+def device_status():
+    """Raises when a kernel has reported something that it left out (see redcuda.h) since the last failure; the caller has waited for the stream."""
+    _check(lib().redcuda_device_status())
+
+
+class PagedKv:
+    """A paged K/V cache in the caller's device memory (redcuda_paged_kv): the layout and where it lies; it owns nothing."""
+
+    def __init__(self, ggml_type: int, n_kv: int, head_dim: int, page_size: int, n_pages: int, k_ptr: int, v_ptr: int, page_stride: int = 0, token_stride: int = 0,
+                 head_stride: int = 0):
+        self.desc = PagedKvDesc(ggml_type, n_kv, head_dim, page_size, n_pages, page_stride, token_stride, head_stride, k_ptr, v_ptr)
+        self._ref = C.byref(self.desc)
+
+    def attend_workspace(self, n_q: int) -> int:
+        """Bytes of device workspace that attend_device needs for n_q query heads, whatever the batch."""
+        n = lib().redcuda_kv_attend_workspace(self._ref, n_q)
+        if not n:
+            _check(0)
+        return int(n)
+
+    def append_device(self, table_ptr: int, table_width: int, n_seqs: int, start_ptr: int, n_tokens: int, cu_seqlens_ptr: int, in_type: int, k_ptr: int, v_ptr: int, stream: int,
+                      row_stride: int = 0):
+        """K/V rows of n_tokens tokens to the pages; cu_seqlens_ptr 0: one row per sequence."""
+        _check(lib().redcuda_kv_append_device(self._ref, table_ptr, table_width, n_seqs, start_ptr, n_tokens, cu_seqlens_ptr or None, in_type, k_ptr, v_ptr, row_stride, stream or None))
+
+    def attend_device(self, table_ptr: int, table_width: int, n_seqs: int, lens_ptr: int, n_q: int, q_type: int, q_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int,
+                      stream: int, scale: float = 0.0, k_new_ptr: int = 0, v_new_ptr: int = 0, lse_ptr: int = 0, q_stride: int = 0, new_stride: int = 0):
+        """One query row per sequence over its pages; with k_new_ptr / v_new_ptr the sequences' new rows are written first."""
+        _check(lib().redcuda_kv_attend_device(self._ref, table_ptr, table_width, n_seqs, lens_ptr, n_q, q_type, q_ptr, q_stride, k_new_ptr or None, v_new_ptr or None, new_stride, scale,
+                                              out_ptr, lse_ptr or None, workspace_ptr, workspace_bytes, stream or None))
+
+
+def delta_step_device(dims: DeltaDims, n_seqs: int, slots_ptr: int, n_slots: int, q_ptr: int, k_ptr: int, v_ptr: int, gate_ptr: int, beta_ptr: int, state_ptr: int, out_ptr: int, stream: int):
+    """One token of each sequence through the gated delta rule; the states in slots are updated in place (slots_ptr 0: sequence b has slot b)."""
+    _check(lib().redcuda_delta_step_device(C.byref(dims), n_seqs, slots_ptr or None, n_slots, q_ptr, k_ptr, v_ptr, gate_ptr, beta_ptr, state_ptr, out_ptr, stream or None))
+
+
+def delta_rule_device(dims: DeltaDims, n_tokens: int, n_seqs: int, cu_seqlens_ptr: int, slots_ptr: int, n_slots: int, q_ptr: int, k_ptr: int, v_ptr: int, gate_ptr: int, beta_ptr: int,
+                      state_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int, stream: int):
+    """Prompts laid end to end through the gated delta rule."""
+    _check(lib().redcuda_delta_rule_device(C.byref(dims), n_tokens, n_seqs, cu_seqlens_ptr, slots_ptr or None, n_slots, q_ptr, k_ptr, v_ptr, gate_ptr, beta_ptr, state_ptr, out_ptr,
+                                           workspace_ptr or None, workspace_bytes, stream or None))
+
+
+def delta_rule(q: np.ndarray, k: np.ndarray, v: np.ndarray, gate: np.ndarray, beta: np.ndarray, state: np.ndarray, cu_seqlens=None, slots=None, scale: float = 0.0) -> np.ndarray:
+    """Gated delta rule of host rows: q, k [T, n_group, d_state], v [T, dt_rank, d_state] (float32 or float16), gate, beta [T, dt_rank]; state [n_slots, dt_rank,
+    d_state, d_state] is updated in place. cu_seqlens None: one sequence."""
+    dtype = np.float16 if v.dtype == np.float16 else np.float32
+    q, k, v = (np.ascontiguousarray(a, dtype) for a in (q, k, v))
+    gate, beta = (np.ascontiguousarray(a, np.float32) for a in (gate, beta))
+    T, H, S = v.shape
+    if q.shape != k.shape or q.shape[0] != T or q.shape[2] != S or gate.shape != (T, H) or beta.shape != (T, H):
+        raise ValueError("delta_rule: the rows' shapes do not go together")
+    if state.dtype != np.float32 or not state.flags.c_contiguous or state.shape[1:] != (H, S, S):
+        raise ValueError("states must be C-contiguous float32 arrays [n_slots, dt_rank, d_state, d_state] (they are updated in place)")
+    cu = np.ascontiguousarray([0, T] if cu_seqlens is None else cu_seqlens, np.int32)
+    sl = None if slots is None else np.ascontiguousarray(slots, np.int32)
+    if sl is not None and sl.size != cu.size - 1:
+        raise ValueError("delta_rule: a slot for every sequence")
+    out = np.zeros((T, H, S), dtype)
+    dims = DeltaDims(1 if dtype == np.float16 else 0, q.shape[1], H, S, 0, 0, 0, scale)
+    _check(lib().redcuda_delta_rule(C.byref(dims), T, cu.size - 1, cu.ctypes.data, None if sl is None else sl.ctypes.data, state.shape[0], q.ctypes.data, k.ctypes.data, v.ctypes.data,
+                                    gate.ctypes.data, beta.ctypes.data, state.ctypes.data, out.ctypes.data))
+    return out
+
+
+def token_logprobs_device(ggml_type: int, rows: int, vocab: int, row_stride: int, logits_ptr: int, tokens_ptr: int, top_n: int, logprob_ptr: int, entropy_ptr: int, top_ids_ptr: int,
+                          top_logprobs_ptr: int, stream: int):
+    """Log probability of the given tokens, entropy and the top_n alternatives of rows of logits; any output may be 0."""
+    _check(lib().redcuda_token_logprobs_device(ggml_type, rows, vocab, row_stride, logits_ptr, tokens_ptr or None, top_n, logprob_ptr or None, entropy_ptr or None, top_ids_ptr or None,
+                                               top_logprobs_ptr or None, stream or None))
+
+
+def token_logprobs(logits: np.ndarray, tokens=None, top_n: int = 0):
+    """(logprob [rows] or None, entropy [rows], top_ids [rows, top_n], top_logprobs [rows, top_n]) of host logits [rows, vocab] (float32 or float16)."""
+    x = np.ascontiguousarray(logits, np.float16 if logits.dtype == np.float16 else np.float32)
+    x = x.reshape(-1, x.shape[-1])
+    rows, vocab = x.shape
+    tok = None if tokens is None else np.ascontiguousarray(tokens, np.int32).reshape(-1)
+    if tok is not None and tok.size != rows:
+        raise ValueError("token_logprobs: a token for every row")
+    lp, ent = (None if tok is None else np.empty(rows, np.float32)), np.empty(rows, np.float32)
+    ids, top = np.empty((rows, top_n), np.int32), np.empty((rows, top_n), np.float32)
+    _check(lib().redcuda_token_logprobs(1 if x.dtype == np.float16 else 0, rows, vocab, 0, x.ctypes.data, None if tok is None else tok.ctypes.data, top_n,
+                                        None if lp is None else lp.ctypes.data, ent.ctypes.data, ids.ctypes.data if top_n else None, top.ctypes.data if top_n else None))
+    return lp, ent, ids, top
 
 
 class MoeLayer:

@@ -248,6 +248,95 @@ int redcuda_moe_combine_device(redcuda_moe *m, uint32_t ntok, const float *pair_
 int redcuda_profile_enable(int on);
 int redcuda_profile_report(char *buf, size_t cap);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Operators of a batched server: many sequences at once, each with its own K/V pages and DeltaNet states. No counterpart in
+ * the reference, which serves one sequence (attention_branch and deltanet_branch, native/redlite_native_engine_cpu.c:120-325).
+ * "Device" entry points as everywhere: device pointers of the current device, asynchronous on `stream`, nothing is allocated,
+ * and a call may be captured in a CUDA graph. Types are ggml ids: 0 F32, 1 F16, 30 BF16. What a kernel must not act on (a page id
+ * outside the cache, a state slot that two sequences share) it leaves out and reports: redcuda_device_status, or the next
+ * host call, fails with a message.
+ * Pointers and row strides are multiples of 16 bytes (logits, whole numbers and 32-bit side arrays: of their own size). Sizes that are
+ * refused are refused before anything is launched.
+ * ---------------------------------------------------------------------------------------------------------- */
+
+/* 1 when no kernel has reported anything since the last failure that was read, else 0 with a message (and the reports are
+ * cleared). The caller waits for the stream first. */
+int redcuda_device_status(void);
+
+/* A paged K/V cache in the caller's device memory: n_pages pages of page_size positions, each position n_kv rows of head_dim values
+ * (64, 128 or 256) of `type`. Element (page, position, head, i) of K is k[page * page_stride + position * token_stride + head *
+ * head_stride + i]; strides all 0: dense in that order. Which pages hold a sequence is said by a page table
+ * [n_seqs][table_width] of int32 on the device: position p of sequence b lies in page table[b][p / page_size]. */
+typedef struct {
+    uint32_t type, n_kv, head_dim, page_size, n_pages;
+    uint64_t page_stride, token_stride, head_stride;       /* in elements */
+    void *k, *v;
+} redcuda_paged_kv;
+
+/* Writes the K/V rows [n_kv][head_dim] (in_type; converted, rounded to nearest even) of n_tokens tokens to the cache. Rows cu_seqlens[b] up to
+ * cu_seqlens[b + 1] - 1 are positions start[b], start[b] + 1, ... of sequence b; cu_seqlens NULL: one row per sequence, row b being position
+ * start[b] of sequence b. A sequence with a negative start is left out, as are rows from cu_seqlens[n_seqs] on. row_stride: elements between
+ * the rows of two tokens, 0 = n_kv * head_dim. */
+int redcuda_kv_append_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *start_dev,
+                             uint32_t n_tokens, const int32_t *cu_seqlens_dev, uint32_t in_type, const void *k_dev, const void *v_dev, uint64_t row_stride,
+                             void *stream);
+
+/* Attention of ONE query row per sequence over the positions 0 .. lens[b] - 1 of its pages: for query head h, which reads K/V head h / (n_q / n_kv),
+ *     x_p = scale * q . k_p,   out = sum_p exp(x_p) v_p / sum_p exp(x_p),   lse = log sum_p exp(x_p)
+ * q and out [n_seqs][n_q][head_dim] of q_type (q_stride elements between the query rows of two sequences, 0 = n_q * head_dim; out is dense and lies
+ * outside the inputs), lse_dev [n_seqs][n_q] F32 or NULL. scale 0: 1 / sqrt(head_dim). With k_new_dev / v_new_dev (both or neither; q_type, new_stride as
+ * row_stride above) the sequences' new rows are first written to position lens[b] - 1, so that a decode step is one call. A sequence of no positions
+ * (lens[b] <= 0) has nothing written to the cache, out = 0 and lse = -infinity. Positions whose page is not in the cache are left out.
+ * Types: q_type F32 with a cache of F32 or F16, or q_type equal to the cache's type. With an F16 or BF16 cache an infinity in a row that is
+ * attended to gives NaN. workspace_dev: redcuda_kv_attend_workspace bytes (for n_q heads on the current device, any batch; 0 = invalid
+ * arguments), 16-byte aligned; calls that overlap on the GPU need one each. */
+uint64_t redcuda_kv_attend_workspace(const redcuda_paged_kv *kv, uint32_t n_q);
+int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *lens_dev,
+                             uint32_t n_q, uint32_t q_type, const void *q_dev, uint64_t q_stride, const void *k_new_dev, const void *v_new_dev,
+                             uint64_t new_stride, float scale, void *out_dev, float *lse_dev, void *workspace_dev, uint64_t workspace_bytes, void *stream);
+
+/* The gated delta rule by itself (the recurrence inside redcuda_deltanet_step, native/redlite_native_engine_cpu.c:198-216), for each value head h of a
+ * sequence, with key head h / (dt_rank / n_group) and S [d_state][d_state] (rows: values, columns: keys):
+ *     S <- exp(gate) S;   d = beta (v - S k);   S <- S + d k^T;   out = scale * S q
+ * q, k [tokens][n_group][d_state], v, out [tokens][dt_rank][d_state] of `type`, gate (the logarithm of the decay) and beta [tokens][dt_rank]
+ * F32, state [n_slots][dt_rank][d_state][d_state] F32, updated in place. d_state 32, 64, 128 or 256. Strides in elements between two tokens, 0: dense; out is dense
+ * and lies outside the inputs. scale 0: 1 / sqrt(d_state). */
+typedef struct {
+    uint32_t type, n_group, dt_rank, d_state;
+    uint64_t q_stride, k_stride, v_stride;
+    float scale;
+} redcuda_delta_dims;
+
+/* One token of each of n_seqs sequences. slots_dev[b]: the state of sequence b (NULL: b); -1: the sequence is left out, its row of out
+ * as it was. A slot outside 0 .. n_slots - 1, or one that an earlier sequence of the call has, is reported and its sequence left out. */
+int redcuda_delta_step_device(const redcuda_delta_dims *d, uint32_t n_seqs, const int32_t *slots_dev, uint32_t n_slots, const void *q_dev, const void *k_dev,
+                              const void *v_dev, const float *gate_dev, const float *beta_dev, float *state_dev, void *out_dev, void *stream);
+
+/* Prompts laid end to end: tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of the n_tokens rows are sequence b's, in order (n_seqs + 1 ascending numbers on
+ * the device; a sequence may be empty; rows from cu_seqlens[n_seqs] on are left as they were). Slots as above. workspace_dev:
+ * redcuda_delta_rule_workspace bytes, 16-byte aligned (0: none is needed); calls that overlap on the GPU need one each. */
+uint64_t redcuda_delta_rule_workspace(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs);
+int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs, const int32_t *cu_seqlens_dev, const int32_t *slots_dev,
+                              uint32_t n_slots, const void *q_dev, const void *k_dev, const void *v_dev, const float *gate_dev, const float *beta_dev,
+                              float *state_dev, void *out_dev, void *workspace_dev, uint64_t workspace_bytes, void *stream);
+/* The same with host pointers, synchronous; state is read and written back. */
+int redcuda_delta_rule(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs, const int32_t *cu_seqlens, const int32_t *slots, uint32_t n_slots,
+                       const void *q, const void *k, const void *v, const float *gate, const float *beta, float *state, void *out);
+
+/* What an answer carries beside its tokens, from rows of logits [rows][vocab] of `type` (row_stride elements apart, 0 = vocab): with lse = log sum_i exp(x_i)
+ *     logprob = x[token] - lse,   entropy = lse - sum_i p_i x_i  (p = softmax),
+ *     the top_n largest values in descending order, the lower id first among equal ones: their ids and x - lse.
+ * tokens [rows] int32 (NULL: no logprob is written; -1: none in this row, its logprob is NaN; any other id outside the vocabulary is reported and NaN).
+ * Every output may be NULL (top_ids and top_logprobs together, with top_n 0). top_n <= min(vocab, REDCUDA_MAX_ALTERNATIVES). Logits of -infinity
+ * are masked: probability 0; a row of nothing else has logprob -infinity and entropy 0. A row with a NaN or +infinity has NaN everywhere
+ * and ids of -1. */
+#define REDCUDA_MAX_ALTERNATIVES 32u
+int redcuda_token_logprobs_device(uint32_t type, uint32_t rows, uint32_t vocab, uint64_t row_stride, const void *logits_dev, const int32_t *tokens_dev, uint32_t top_n,
+                                  float *logprob_dev, float *entropy_dev, int32_t *top_ids_dev, float *top_logprobs_dev, void *stream);
+/* The same with host pointers, synchronous. */
+int redcuda_token_logprobs(uint32_t type, uint32_t rows, uint32_t vocab, uint64_t row_stride, const void *logits, const int32_t *tokens, uint32_t top_n,
+                           float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs);
+
 /* number of kernel launches the library has issued on this thread's device since load (for bench accounting) */
 uint64_t redcuda_launch_count(void);
 

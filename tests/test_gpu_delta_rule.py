@@ -1,0 +1,273 @@
+"""The gated delta rule of a batch of sequences, a token each and whole prompts, against the recurrence in 64 bits.
+
+Tolerance: with keys of length one and 0 <= beta <= 1 a token's map of a state row m is no expansion, so the errors of the tokens add up, each at most some 2^-22 (|m| + |v|)
+(sums of 16 rounded steps, products of numbers held to 2^-22); they are of either sign, hence a root of their number, four deviations of which are
+8 sqrt(T + 16) 2^-22 (max |m| + max |v|), plus half a step of the output's type."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import dwarfstar_red_lite_b200 as rc
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": (0, torch.float32), "f16": (1, torch.float16), "bf16": (30, torch.bfloat16)}
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _inputs(g, T, groups, rank, S, dt, n_slots, gate="mixed", keys="random"):
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    unit = lambda x: (x / x.norm(dim=-1, keepdim=True)).to(dt)  # noqa: E731
+    x = dict(q=unit(rnd(T, groups, S)), k=unit(rnd(T, groups, S)), v=rnd(T, rank, S).to(dt), beta=torch.sigmoid(rnd(T, rank)), state=rnd(n_slots, rank, S, S) * 0.1)
+    if keys == "same":                                    # every key the same: what a token corrects is what the one before it wrote
+        x["k"] = x["k"][:1].expand(T, groups, S).contiguous()
+        x["beta"] = torch.ones_like(x["beta"])
+    if keys == "near":
+        x["k"] = unit(x["k"][:1].float() + 0.05 * rnd(T, groups, S))
+    x["gate"] = {"mixed": -torch.exp(rnd(T, rank) * 1.5 - 2.0), "none": torch.zeros(T, rank, device="cuda"), "strong": -torch.rand(T, rank, generator=g, device="cuda") * 60,
+                 "cut": torch.where(torch.rand(T, rank, generator=g, device="cuda") < 0.1, -math.inf, -0.01)}[gate]
+    return x
+
+
+def _reference(x, cu, slots, scale):
+    """Rows of out and the states, in 64 bits; a token's map is applied to all heads at once."""
+    out, state = torch.zeros(x["v"].shape, dtype=torch.float64, device="cuda"), x["state"].double()
+    width = x["v"].shape[1] // x["q"].shape[1]
+    most = 0.0
+    for b, s in enumerate(slots):
+        if s < 0:
+            continue
+        m = state[s]
+        for t in range(cu[b], cu[b + 1]):
+            k, q = (x[n][t].double().repeat_interleave(width, 0) for n in ("k", "q"))
+            m = m * torch.exp(x["gate"][t].double())[:, None, None]
+            d = (x["v"][t].double() - torch.einsum("hij,hj->hi", m, k)) * x["beta"][t].double()[:, None]
+            m = m + d[:, :, None] * k[:, None]
+            out[t] = torch.einsum("hij,hj->hi", m, q) * scale
+        most = max(most, float(m.norm(dim=-1).max()))
+        state[s] = m
+    return out, state, max(most, float(x["state"].double().norm(dim=-1).max()))
+
+
+def _close(x, cu, slots, got, state, scale):
+    out, want, most = _reference(x, cu, slots, scale)
+    T = max(b - a for a, b in zip(cu, cu[1:])) if len(cu) > 1 else 1
+    unit = 8 * math.sqrt(T + 16) * 2.0 ** -22 * (most + float(x["v"].double().abs().max()))
+    rows = torch.zeros(got.shape[0], dtype=torch.bool, device="cuda")
+    for b, s in enumerate(slots):
+        if s >= 0:
+            rows[cu[b]:cu[b + 1]] = True
+    tol = unit * abs(scale) + torch.finfo(got.dtype).eps / 2 * out.abs()
+    far = ((got.double() - out).abs() / tol)[rows]
+    assert far.numel() == 0 or float(far.max()) <= 1, float(far.max())
+    assert bool((got[~rows] == 7.0).all())                # rows of no sequence
+    far = ((state.double() - want).abs() / unit)
+    assert float(far.max()) <= 1, float(far.max())
+    used = [s for s in slots if s >= 0]
+    rest = [s for s in range(state.shape[0]) if s not in used]
+    assert torch.equal(state[rest], x["state"][rest])
+
+
+def _rule(x, cu, slots, dims, n_slots, stream=None):
+    state, out = x["state"].clone(), torch.full_like(x["v"], 7.0)
+    cu_d, sl = torch.tensor(cu, dtype=torch.int32, device="cuda"), torch.tensor(slots, dtype=torch.int32, device="cuda")
+    T = x["v"].shape[0]
+    work = torch.full((dims.workspace(T, len(slots)),), 0xff, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    rc.delta_rule_device(dims, T, len(slots), cu_d.data_ptr(), sl.data_ptr(), n_slots, *[x[n].data_ptr() for n in ("q", "k", "v", "gate", "beta")], state.data_ptr(), out.data_ptr(),
+                         work.data_ptr(), work.numel(), (stream or torch.cuda.current_stream()).cuda_stream)
+    torch.cuda.synchronize()
+    return out, state
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("groups, rank, S", [(16, 32, 128), (2, 6, 64), (1, 1, 32), (3, 3, 128), (2, 8, 256)])
+def test_prompts(dtype, groups, rank, S):
+    lens = [1, 0, 63, 64, 65, 2, 130, 17, 200]
+    cu = np.cumsum([0] + lens).tolist()
+    g = _gen(groups * S)
+    x = _inputs(g, cu[-1] + 5, groups, rank, S, TYPES[dtype][1], len(lens) + 3)       # five rows behind the last sequence
+    slots = [7, 0, 3, 11, 1, -1, 4, 9, 2]
+    dims = rc.DeltaDims(TYPES[dtype][0], groups, rank, S)
+    out, state = _rule(x, cu, slots, dims, len(lens) + 3)
+    _close(x, cu, slots, out, state, 1 / math.sqrt(S))
+    rc.device_status()
+
+
+@pytest.mark.parametrize("S", [64, 128])
+@pytest.mark.parametrize("gate", ["none", "strong", "cut"])
+@pytest.mark.parametrize("keys", ["random", "same", "near"])
+def test_gates_and_keys(S, gate, keys):
+    cu = [0, 700]
+    x = _inputs(_gen(S), 700, 2, 4, S, torch.float32, 1, gate, keys)
+    dims = rc.DeltaDims(0, 2, 4, S)
+    _close(x, cu, [0], *_rule(x, cu, [0], dims, 1), 1 / math.sqrt(S))
+
+
+@pytest.mark.parametrize("T", [3000, 5001])
+def test_long_prompts(T):
+    cu = [0, T - 1000, T]
+    x = _inputs(_gen(T), T, 1, 2, 128, torch.float32, 2)
+    _close(x, cu, [1, 0], *_rule(x, cu, [1, 0], rc.DeltaDims(0, 1, 2, 128), 2), 1 / math.sqrt(128))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_strides_and_scale(dtype):
+    """q, k and v as parts of one row, as a projection leaves them."""
+    T, groups, rank, S = 150, 2, 4, 128
+    dt = TYPES[dtype][1]
+    x = _inputs(_gen(1), T, groups, rank, S, dt, 1)
+    row = torch.cat([x["q"].flatten(1), x["k"].flatten(1), x["v"].flatten(1)], 1)
+    n = row.shape[1]
+    y = dict(x, q=row, k=row[:, groups * S:], v=row[:, 2 * groups * S:])
+    dims = rc.DeltaDims(TYPES[dtype][0], groups, rank, S, n, n, n, 0.25)
+    state, out = x["state"].clone(), torch.full_like(x["v"], 7.0)
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    work = torch.empty(dims.workspace(T, 1), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    rc.delta_rule_device(dims, T, 1, cu.data_ptr(), 0, 1, *[y[k].data_ptr() for k in ("q", "k", "v", "gate", "beta")], state.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel(),
+                         torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    _close(x, [0, T], [0], out, state, 0.25)
+
+
+def test_large_and_small_states():
+    """States, values and keys far from 1: what is held in fewer bits has to be scaled by what is there."""
+    for size in (1e-6, 1e5):
+        x = _inputs(_gen(2), 300, 1, 2, 128, torch.float32, 1)
+        x["v"], x["state"] = x["v"] * size, x["state"] * size
+        _close(x, [0, 300], [0], *_rule(x, [0, 300], [0], rc.DeltaDims(0, 1, 2, 128), 1), 1 / math.sqrt(128))
+    x = _inputs(_gen(3), 300, 1, 2, 128, torch.float32, 1)
+    x["k"], x["beta"], x["q"] = x["k"] * 50.0, x["beta"] / 2500.0, x["q"] * 1e-4
+    x["state"] = x["state"] / 50.0
+    y = dict(x, k=x["k"] / 50.0, beta=x["beta"] * 2500.0, state=x["state"] * 50.0, q=x["q"] * 1e4)       # the same with keys of length one: S k is the same
+    out, state = _rule(x, [0, 300], [0], rc.DeltaDims(0, 1, 2, 128), 1)
+    _close(y, [0, 300], [0], out * 50.0 * 1e4, state * 50.0, 1 / math.sqrt(128))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("groups, rank, S", [(16, 32, 128), (2, 6, 64), (1, 3, 32), (2, 4, 256)])
+@pytest.mark.parametrize("B", [1, 2, 33])
+def test_steps(dtype, groups, rank, S, B):
+    x = _inputs(_gen(B), B, groups, rank, S, TYPES[dtype][1], B + 2, "cut")
+    slots = torch.randperm(B + 2)[:B].tolist()
+    if B > 2:
+        slots[3] = -1                                     # a padded row of the batch
+    state, out, sl = x["state"].clone(), torch.full_like(x["v"], 7.0), torch.tensor(slots, dtype=torch.int32, device="cuda")
+    dims = rc.DeltaDims(TYPES[dtype][0], groups, rank, S)
+    torch.cuda.synchronize()
+    rc.delta_step_device(dims, B, sl.data_ptr(), B + 2, *[x[n].data_ptr() for n in ("q", "k", "v", "gate", "beta")], state.data_ptr(), out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    _close(x, list(range(B + 1)), slots, out, state, 1 / math.sqrt(S))
+    rc.device_status()
+
+
+@pytest.mark.parametrize("form", ["rule", "step"])
+def test_slots_that_cannot_be(form):
+    """A slot beyond the states, one below -1, one that an earlier sequence has: reported, the sequences left out, the others served."""
+    x = _inputs(_gen(4), 5, 1, 2, 64, torch.float32, 3)
+    slots, cu = [1, 3, 1, -2, 0], list(range(6))
+    dims = rc.DeltaDims(0, 1, 2, 64)
+    if form == "rule":
+        out, state = _rule(x, cu, slots, dims, 3)
+    else:
+        state, out, sl = x["state"].clone(), torch.full_like(x["v"], 7.0), torch.tensor(slots, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        rc.delta_step_device(dims, 5, sl.data_ptr(), 3, *[x[n].data_ptr() for n in ("q", "k", "v", "gate", "beta")], state.data_ptr(), out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+    with pytest.raises(rc.RedcudaError, match="slot"):
+        rc.device_status()
+    _close(x, cu, [1, -1, -1, -1, 0], out, state, 1 / 8)
+
+
+@pytest.mark.parametrize("cu, fine", [([0, 300, 200, 350], [True, False, True]), ([0, 100, 999, 350], [True, False, False]), ([-5, 100, 200, 350], [False, True, True]),
+                                      ([0, 100, 100, 400], [True, True, False])])
+def test_bounds_that_cannot_be(cu, fine):
+    """Bounds that fall, leave the rows or begin below them: reported, those sequences left out."""
+    x = _inputs(_gen(5), 350, 1, 2, 128, torch.float32, 3)
+    dims = rc.DeltaDims(0, 1, 2, 128)
+    out, state = _rule(x, cu, [0, 1, 2], dims, 3)
+    with pytest.raises(rc.RedcudaError, match="bounds"):
+        rc.device_status()
+    for b in range(3):
+        if not fine[b]:
+            assert torch.equal(state[b], x["state"][b])
+        else:
+            y = {n: (a[cu[b]:cu[b + 1]] if n != "state" else a[b:b + 1]) for n, a in x.items()}
+            if b and cu[b] < max(cu[:b + 1]):             # rows that two sequences claim may hold either's output
+                _, want, most = _reference(y, [0, cu[b + 1] - cu[b]], [0], 1.0)
+                assert float((state[b] - want[0]).abs().max()) < 1e-4 * most
+            else:
+                want, st, _ = _reference(y, [0, cu[b + 1] - cu[b]], [0], 1 / math.sqrt(128))
+                assert float((state[b] - st[0]).abs().max()) < 1e-4
+
+
+def test_a_nan_stays_in_its_sequence():
+    x = _inputs(_gen(6), 400, 1, 2, 128, torch.float32, 3)
+    cu = [0, 130, 260, 400]
+    clean, _ = _rule(x, cu, [0, 1, 2], rc.DeltaDims(0, 1, 2, 128), 3)
+    x["v"][200, 1, 5] = math.nan
+    out, state = _rule(x, cu, [0, 1, 2], rc.DeltaDims(0, 1, 2, 128), 3)
+    assert torch.equal(out[:130], clean[:130]) and torch.equal(out[260:], clean[260:])
+    assert torch.equal(out[130:200], clean[130:200]) and bool(out[200:260, 1, 5].isnan().all()) and bool(state[1, 1, 5].isnan().all())
+    assert bool(state[0].isfinite().all()) and bool(state[2].isfinite().all())
+
+
+def test_capture_and_repeats():
+    x = _inputs(_gen(7), 500, 2, 4, 128, torch.bfloat16, 4)
+    dims, s = rc.DeltaDims(30, 2, 4, 128), torch.cuda.Stream()
+    state, out = x["state"].clone(), torch.zeros_like(x["v"])
+    cu, slots = torch.tensor([0, 0, 0, 0], dtype=torch.int32, device="cuda"), torch.tensor([2, 0, 3], dtype=torch.int32, device="cuda")
+    work = torch.empty(dims.workspace(500, 3), dtype=torch.uint8, device="cuda")
+    call = lambda: rc.delta_rule_device(dims, 500, 3, cu.data_ptr(), slots.data_ptr(), 4, *[x[n].data_ptr() for n in ("q", "k", "v", "gate", "beta")], state.data_ptr(), out.data_ptr(),  # noqa: E731
+                                        work.data_ptr(), work.numel(), s.cuda_stream)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            call()
+        for bounds in ([0, 500, 500, 500], [0, 100, 290, 500], [0, 1, 2, 3]):
+            cu.copy_(torch.tensor(bounds, dtype=torch.int32))
+            state.copy_(x["state"])
+            out.fill_(7.0)
+            graph.replay()
+            s.synchronize()
+            got = out.clone(), state.clone()
+            _close(x, bounds, [2, 0, 3], *got, 1 / math.sqrt(128))
+            state.copy_(x["state"])
+            call()
+            s.synchronize()
+            assert torch.equal(out, got[0]) and torch.equal(state, got[1])
+    del graph
+
+
+def test_prompt_is_its_tokens():
+    """A prompt at once, in two pieces, and a token at a time leave the same states and outputs, within the rounding."""
+    x = _inputs(_gen(8), 333, 2, 4, 128, torch.float32, 1)
+    dims = rc.DeltaDims(0, 2, 4, 128)
+    whole, state = _rule(x, [0, 333], [0], dims, 1)
+    parts, st = [], x["state"]
+    for a, b in ((0, 190), (190, 191), (191, 333)):
+        y = {n: t[a:b].contiguous() for n, t in x.items() if n != "state"}
+        o, st = _rule(dict(y, state=st), [0, b - a], [0], dims, 1)
+        parts.append(o)
+    assert float((torch.cat(parts) - whole).abs().max()) <= 2e-5 and float((st - state).abs().max()) <= 2e-5
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_host_form(dtype):
+    x = _inputs(_gen(9), 90, 2, 4, 64, torch.float16 if dtype == np.float16 else torch.float32, 3)
+    h = {n: t.cpu().numpy() for n, t in x.items()}
+    state = h["state"].copy()
+    out = rc.delta_rule(h["q"], h["k"], h["v"], h["gate"], h["beta"], state, [0, 30, 90], [2, 0])
+    assert out.dtype == dtype
+    _close(x, [0, 30, 90], [2, 0], torch.from_numpy(out).cuda(), torch.from_numpy(state).cuda(), 1 / 8)
+    with pytest.raises(rc.RedcudaError, match="slot"):
+        rc.delta_rule(h["q"], h["k"], h["v"], h["gate"], h["beta"], state, [0, 30, 90], [2, 2])
