@@ -14,7 +14,8 @@ namespace rc {
 
 namespace cg = cooperative_groups;
 
-constexpr int LP_WARPS = 8, LP_CLUSTER = 8, LP_TOP = (int)REDCUDA_MAX_ALTERNATIVES;
+constexpr int LP_WARPS = 8, LP_CLUSTER = 8, LP_UNROLL = 4;
+static_assert(REDCUDA_MAX_ALTERNATIVES <= 32u && LP_WARPS == 8, "a list is one key a lane; eight floors are read at once");
 
 struct LogprobArgs {
     const void *x;
@@ -47,125 +48,194 @@ __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b) {
     return r;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }      // 2 units
+
+__device__ __forceinline__ float4 lp_floor(const float *s) {                 // other warps write it meanwhile
+    float4 r;
+    asm volatile("ld.volatile.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"((uint32_t)__cvta_generic_to_shared(s)));
+    return r;
+}
+
+// 32 keys, one a lane, in two networks: any order to descending, and the 32 largest of two descending lists.
+__device__ __forceinline__ uint64_t lp_exchange(uint64_t key, int w, bool larger) {
+    const uint64_t other = __shfl_xor_sync(0xffffffffu, key, w);
+    return (key > other) == larger ? key : other;
+}
+__device__ __forceinline__ uint64_t lp_sort(uint64_t key) {
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (uint32_t run = 2; run <= 32; run <<= 1)
+#pragma unroll
+        for (uint32_t w = run >> 1; w; w >>= 1) key = lp_exchange(key, (int)w, ((lane & w) == 0u) == ((lane & run) == 0u || run == 32u));
+    return key;
+}
+__device__ __forceinline__ uint64_t lp_merge(uint64_t a, uint64_t b) {       // both descending
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - (int)lane);
+    uint64_t key = a > r ? a : r;
+#pragma unroll
+    for (uint32_t w = 16; w; w >>= 1) key = lp_exchange(key, (int)w, (lane & w) == 0u);
+    return key;
+}
+
+// What bounds it is the row's bytes, if a value takes no more than the eight instructions it has here (of which one is an exponential, a
+// sixteenth of the fp32 rate). The alternatives therefore cost one comparison a lane and round of LP_UNROLL pieces: a warp keeps its 32 largest keys, one a
+// lane, and looks at single values only where the largest of a lane's round reaches what is known to be among the row's n largest. That is the n-th of the warp's own,
+// or the least of the warps' ceil(n / LP_WARPS)-th largest, which every warp publishes (n values are at least that large; a stale one is a lower bound too).
 template <class T>
-__global__ void __launch_bounds__(LP_WARPS * 32) k_token_logprobs(LogprobArgs A) {
+__global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs A) {
     pdl_prologue();
-    constexpr int VEC = 16 / sizeof(T);
+    constexpr int VEC = 16 / sizeof(T), U = LP_UNROLL, NV = U * VEC;
+    constexpr float LOG2E = 1.44269504088896340736f;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank(), row = blockIdx.x / parts;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, n = A.top_n;
-    __shared__ uint64_t s_keys[LP_WARPS * LP_TOP], s_best[LP_CLUSTER * LP_TOP];
-    __shared__ LpSums s_sums[LP_WARPS > LP_CLUSTER ? LP_WARPS : LP_CLUSTER];
+    __shared__ uint64_t s_keys[LP_WARPS][32], s_best[LP_CLUSTER][32];
+    __shared__ LpSums s_sums[LP_WARPS], s_parts[LP_CLUSTER];
+    __shared__ __align__(16) float s_floor[LP_WARPS];
     const T *x = reinterpret_cast<const T *>(A.x) + (uint64_t)row * A.row_stride;
     // the row as up to VEC - 1 single values, whole 16-byte pieces, up to VEC - 1 single values
     const uint32_t head = min(A.vocab, (uint32_t)((16u - ((uintptr_t)x & 15u)) & 15u) / (uint32_t)sizeof(T)), pieces = (A.vocab - head) / VEC;
     const uint32_t per = (pieces + parts - 1u) / parts, p0 = min(pieces, part * per), p1 = min(pieces, p0 + per);
+    if (lane == 0u) s_floor[warp] = -INFINITY;
+    __syncthreads();
 
-    LpSums S{-INFINITY, 0.f, 0.f};
-    bool odd = false;                            // a NaN or +infinity
-    uint64_t best = 0ull;                        // lane i: the i-th largest of what the warp has seen
-    uint64_t least = 0ull;                       // the n-th
-    auto sum = [&](float v) {
-        odd |= !(v < INFINITY);
-        if (v > S.m) {                           // never so for a NaN
-            const float d = S.m - v, e = expf(d);
-            S.u = e > 0.f ? e * (S.u + S.s * d) : 0.f;
-            S.s *= e; S.m = v;
-        }
-        if (v > -INFINITY) {
-            const float d = v - S.m, e = expf(d);
-            S.s += e;
-            S.u += e > 0.f ? e * d : 0.f;
-        }
-    };
-    auto insert = [&](uint64_t key) {            // the same key in every lane
-        const bool above = best >= key;
-        const uint64_t up = __shfl_up_sync(0xffffffffu, best, 1);
-        const bool above_up = lane == 0u || up >= key;
-        best = above ? best : above_up ? key : up;
+    float m = -INFINITY;                         // a lane's sums are kept in two halves each
+    float2 s2 = make_float2(0.f, 0.f), u2 = make_float2(0.f, 0.f);
+    uint64_t best = 0ull, least = 0ull;          // lane i: the i-th largest key; the n-th
+    float bar = n ? -INFINITY : INFINITY;        // values below it are not among the row's n largest
+    const uint32_t share = (n + LP_WARPS - 1u) / LP_WARPS;
+    auto listed = [&]() {                        // the list has changed
         least = __shfl_sync(0xffffffffu, best, (int)n - 1);
+        const uint64_t mine = __shfl_sync(0xffffffffu, best, (int)share - 1);
+        if (lane == 0u) reinterpret_cast<volatile float *>(s_floor)[warp] = mine ? lp_value(mine) : -INFINITY;
     };
-    auto offer = [&](bool have, float v, uint32_t i) {        // by the whole warp
-        if (n == 0u) return;
-        const uint64_t key = have && v == v ? lp_key(v, i) : 0ull;
-        for (uint32_t todo = __ballot_sync(0xffffffffu, key > least); todo; todo &= todo - 1u) {
-            const uint64_t k = __shfl_sync(0xffffffffu, key, (int)__ffs((int)todo) - 1);
-            if (k > least) insert(k);
+    auto offer = [&](uint64_t key) {             // a key of each lane, 0: none
+        uint32_t todo = __ballot_sync(0xffffffffu, key > least);
+        if (!todo) return;
+        if (__popc(todo) > 4) {
+            best = lp_merge(best, lp_sort(key));
+        } else {
+            for (; todo; todo &= todo - 1u) {
+                const uint64_t k = __shfl_sync(0xffffffffu, key, (int)__ffs((int)todo) - 1), up = __shfl_up_sync(0xffffffffu, best, 1);
+                best = best >= k ? best : lane == 0u || up >= k ? k : up;
+            }
         }
+        listed();
     };
-    for (uint32_t p = p0 + warp * 32u; p < p1; p += LP_WARPS * 32u) {
-        const bool have = p + lane < p1;
-        float v[VEC] = {};
-        if (have) load_vals<VEC>(x + head + (uint64_t)(p + lane) * VEC, v);
+    auto rescale = [&](float to) {
+        const float f = to > m ? exp2_fast(max_nan(m - to, -150.f) * LOG2E) : 1.f, d = m == -INFINITY ? 0.f : m - to;
+        u2 = make_float2(f > 0.f ? f * (u2.x + s2.x * d) : 0.f, f > 0.f ? f * (u2.y + s2.y * d) : 0.f);
+        s2.x *= f; s2.y *= f;
+        m = to;
+    };
+    for (uint32_t p = p0 + warp * (32u * U); p < p1; p += LP_WARPS * 32u * U) {
+        float v[NV];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            if (have) sum(v[i]);
-            offer(have, v[i], head + (p + lane) * VEC + i);
+        for (int u = 0; u < U; ++u) {
+            if (p + u * 32u + lane < p1) load_vals<VEC>(x + head + (uint64_t)(p + u * 32u + lane) * VEC, *reinterpret_cast<float (*)[VEC]>(&v[u * VEC]));
+            else
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u * VEC + i] = -INFINITY;
+        }
+        float most = v[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) most = fmaxf(most, v[i]);
+        if (__any_sync(0xffffffffu, most > m)) rescale(fmaxf(m, most));
+        const float base = m == -INFINITY ? 0.f : m;
+        const float2 nb = make_float2(-base, -base), l2 = make_float2(LOG2E, LOG2E);
+#pragma unroll
+        for (int i = 0; i < NV; i += 2) {
+            float2 d = __fadd2_rn(make_float2(v[i], v[i + 1]), nb);
+            d = make_float2(max_nan(d.x, -150.f), max_nan(d.y, -150.f));       // of a probability that is 0, e d = 0; of a NaN, a NaN
+            float2 e = __fmul2_rn(d, l2);
+            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+            s2 = __fadd2_rn(s2, e);
+            u2 = __ffma2_rn(e, d, u2);
+        }
+        const float4 f0 = lp_floor(&s_floor[0]), f1 = lp_floor(&s_floor[4]);
+        if (n) bar = fmaxf(fmaxf(bar, fminf(fminf(fminf(f0.x, f0.y), fminf(f0.z, f0.w)), fminf(fminf(f1.x, f1.y), fminf(f1.z, f1.w)))), least ? lp_value(least) : -INFINITY);
+        if (__any_sync(0xffffffffu, most >= bar)) {
+            // a lane's largest first, which lifts the bar for its others
+            uint32_t todo = 0u, top = ~0u;
+#pragma unroll
+            for (int i = NV - 1; i >= 0; --i) if (v[i] == most && p + (i / VEC) * 32u + lane < p1) top = (uint32_t)i;
+            auto index = [&](uint32_t i) { return head + (p + (i / VEC) * 32u + lane) * VEC + i % VEC; };
+            offer(top != ~0u && most >= bar ? lp_key(most, index(top)) : 0ull);
+            const float now = fmaxf(bar, least ? lp_value(least) : -INFINITY);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) if (v[i] >= now && (uint32_t)i != top && p + (i / VEC) * 32u + lane < p1) todo |= 1u << i;
+            while (__any_sync(0xffffffffu, todo)) {
+                uint64_t key = 0ull;
+                if (todo) { const uint32_t i = (uint32_t)__ffs((int)todo) - 1u; key = lp_key(to_f32(x[index(i)]), index(i)); }
+                offer(key);
+                todo &= todo - 1u;
+            }
         }
     }
     if (part == 0u && warp == 0u) {              // the single values at both ends
         const uint32_t tail = head + pieces * VEC, ends = head + A.vocab - tail;
         const uint32_t i = lane < head ? lane : tail + lane - head;
         const bool have = lane < ends;
-        const float v = have ? to_f32(x[i]) : 0.f;
-        if (have) sum(v);
-        offer(have, v, i);
+        const float v = have ? to_f32(x[i]) : -INFINITY;
+        if (v > m) rescale(v);
+        const float d = max_nan(v - (m == -INFINITY ? 0.f : m), -150.f), e = exp2_fast(d * LOG2E);
+        s2.x += e;
+        u2.x += e * d;
+        if (n) offer(have && v == v ? lp_key(v, i) : 0ull);
     }
+    LpSums S{m, s2.x + s2.y, u2.x + u2.y};
 #pragma unroll
     for (int w = 16; w; w >>= 1) {
-        LpSums o{__shfl_xor_sync(0xffffffffu, S.m, w), __shfl_xor_sync(0xffffffffu, S.s, w), __shfl_xor_sync(0xffffffffu, S.u, w)};
+        const LpSums o{__shfl_xor_sync(0xffffffffu, S.m, w), __shfl_xor_sync(0xffffffffu, S.s, w), __shfl_xor_sync(0xffffffffu, S.u, w)};
         S = lp_join(S, o);
     }
-    if (__any_sync(0xffffffffu, odd)) S.s = NAN;
     if (lane == 0u) s_sums[warp] = S;
-    if (lane < n) s_keys[warp * n + lane] = best;
-    __syncthreads();
-    // the n largest of the lists in s: every key finds its place by counting those above it (0: no value, no place)
-    auto select = [&](const uint64_t *s, uint32_t count, uint64_t *to) {
-        for (uint32_t i = tid; i < count; i += LP_WARPS * 32u) {
-            const uint64_t key = s[i];
-            uint32_t above = 0u;
-            for (uint32_t j = 0; j < count; ++j) above += s[j] > key;
-            if (key && above < n) to[above] = key;
+    s_keys[warp][lane] = best;
+    cluster.sync();                              // and the other blocks have begun: their shared memory may be written
+    if (warp == 0u) {
+        S = lane < LP_WARPS ? s_sums[lane] : LpSums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int w = LP_WARPS / 2; w; w >>= 1) {
+            const LpSums o{__shfl_xor_sync(0xffffffffu, S.m, w), __shfl_xor_sync(0xffffffffu, S.s, w), __shfl_xor_sync(0xffffffffu, S.u, w)};
+            S = lp_join(S, o);
         }
-    };
-    LpSums B = s_sums[0];
-    for (int w = 1; w < LP_WARPS; ++w) B = lp_join(B, s_sums[w]);
-    __syncthreads();
-    cluster.sync();                              // the other blocks have begun: their shared memory may be written
-    {
-        uint64_t *to = cluster.map_shared_rank(s_best, 0) + part * n;
-        for (uint32_t i = tid; i < n; i += LP_WARPS * 32u) to[i] = 0ull;
-        __syncthreads();
-        select(s_keys, LP_WARPS * n, to);
-        if (tid == 0u) cluster.map_shared_rank(s_sums, 0)[part] = B;
+        if (n) {
+#pragma unroll
+            for (int w = 1; w < LP_WARPS; ++w) best = lp_merge(best, s_keys[w][lane]);
+            if (parts > 1u) cluster.map_shared_rank(s_best[part], 0)[lane] = best;
+        }
+        if (parts > 1u && lane == 0u) *cluster.map_shared_rank(&s_parts[part], 0) = S;
     }
-    cluster.sync();
-    if (part != 0u) return;
-    for (uint32_t i = tid; i < n; i += LP_WARPS * 32u) s_keys[i] = 0ull;
-    __syncthreads();
-    select(s_best, parts * n, s_keys);
-    B = s_sums[0];
-    for (uint32_t w = 1; w < parts; ++w) B = lp_join(B, s_sums[w]);
-    __syncthreads();
-    const float ls = logf(B.s);                              // nothing left: m = -infinity, s = 0
-    const bool nan = !(B.s == B.s), none = !nan && B.m == -INFINITY;
-    if (tid == 0u) {
+    if (parts > 1u) cluster.sync();
+    if (part != 0u || warp != 0u) return;
+    if (parts > 1u) {
+        S = lane < parts ? s_parts[lane] : LpSums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int w = LP_CLUSTER / 2; w; w >>= 1) {
+            const LpSums o{__shfl_xor_sync(0xffffffffu, S.m, w), __shfl_xor_sync(0xffffffffu, S.s, w), __shfl_xor_sync(0xffffffffu, S.u, w)};
+            S = lp_join(S, o);
+        }
+        if (n) for (uint32_t w = 1; w < parts; ++w) best = lp_merge(best, s_best[w][lane]);
+    }
+    S.m = __shfl_sync(0xffffffffu, S.m, 0); S.s = __shfl_sync(0xffffffffu, S.s, 0); S.u = __shfl_sync(0xffffffffu, S.u, 0);
+    const float ls = logf(S.s);                  // nothing left: m = -infinity, s = 0
+    const bool nan = !(S.s == S.s), none = !nan && S.m == -INFINITY;
+    if (lane == 0u) {
         if (A.logprob) {
             const int32_t t = A.tokens[row];
             float lp = NAN;
-            if (t >= 0 && (uint32_t)t < A.vocab) lp = nan ? NAN : none ? -INFINITY : (to_f32(x[t]) - B.m) - ls;
+            if (t >= 0 && (uint32_t)t < A.vocab) lp = nan ? NAN : none ? -INFINITY : (to_f32(x[t]) - S.m) - ls;
             else if (t != -1 && A.status) A.status[ST_TOKEN_RANGE] = 1u;
             A.logprob[row] = lp;
         }
-        if (A.entropy) A.entropy[row] = nan ? NAN : none ? 0.f : fmaxf(ls - B.u / B.s, 0.f);
+        if (A.entropy) A.entropy[row] = nan ? NAN : none ? 0.f : fmaxf(ls - S.u / S.s, 0.f);
     }
-    if (A.top_ids)
-        for (uint32_t i = tid; i < n; i += LP_WARPS * 32u) {
-            const uint64_t key = s_keys[i];
-            A.top_ids[(uint64_t)row * n + i] = nan ? -1 : (int32_t)~(uint32_t)key;
-            A.top_lp[(uint64_t)row * n + i] = nan ? NAN : none ? -INFINITY : (lp_value(key) - B.m) - ls;
-        }
+    if (lane < n) {
+        A.top_ids[(uint64_t)row * n + lane] = nan ? -1 : (int32_t)~(uint32_t)best;
+        A.top_lp[(uint64_t)row * n + lane] = nan ? NAN : none ? -INFINITY : (lp_value(best) - S.m) - ls;
+    }
 }
 
 template <class T> static int launch_logprobs(const LogprobArgs &A, uint32_t rows, cudaStream_t s) {

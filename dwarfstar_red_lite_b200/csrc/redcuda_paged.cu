@@ -8,6 +8,7 @@
 #include "../../include/redcuda.h"
 
 #include <math.h>
+#include <type_traits>
 
 namespace rc {
 
@@ -73,9 +74,10 @@ template <class C> static int launch_append_rows(const AppendArgs &A, uint32_t i
 //
 // The work is cut by bytes: a tile is 16 KB of K and V of one K/V head, all tiles of all (sequence, K/V head, group of 8 query heads) are
 // counted through in that order, and every block takes an equal run of them, whatever the lengths are: they are read on the device, so that a
-// captured call follows them. A run that begins or ends inside a sequence's head leaves (m, l, O) in the workspace, at most two of them a
-// block, for k_kv_attend_join; what a block has whole it writes itself. A warp has a ring of tiles of its own that cp.async fills (four warps x three
-// stages x 16 KB in flight a block), so that the warps of a block meet only where a head ends.
+// captured call follows them. A head costs as much as some tiles more (KV_HEAD_COST). A run that begins or ends inside a sequence's head leaves (m, l, O) in the workspace, at most two of them a
+// block, for k_kv_attend_join; what a block has whole it writes itself. A warp has a ring of tiles of its own, so that the warps of a block meet only where a head ends.
+
+__device__ __forceinline__ float kv_lse(float m, float l) { return l == 0.f ? -INFINITY : m * 0.693147180559945309f + logf(l); }
 
 // the positions of sequence b that can be attended to
 __device__ __forceinline__ uint32_t kv_len(const AttendArgs &A, uint32_t b) {
@@ -83,6 +85,10 @@ __device__ __forceinline__ uint32_t kv_len(const AttendArgs &A, uint32_t b) {
     const uint64_t most = (uint64_t)A.table_width * A.page_size;
     return n <= 0 ? 0u : (uint64_t)(uint32_t)n > most ? (uint32_t)most : (uint32_t)n;
 }
+
+// What a head counts in the deal: its tiles, and as many more as its begin and end take (KV_HEAD_COST). Those come first: a run that ends among them leaves
+// the whole head to the next block.
+template <uint32_t TP> __device__ __forceinline__ uint32_t kv_cost(uint32_t len) { return len ? (len + TP - 1u) / TP + KV_HEAD_COST : 0u; }
 
 // One tile of a warp's ring: its rows requested, rows beyond the end or without a page as zeros. Returns the rows that count, as bits.
 template <class T, int HD>
@@ -117,7 +123,7 @@ __device__ __forceinline__ uint64_t kv_request(const AttendArgs &A, uint32_t b, 
     return valid;
 }
 
-// a warp's share of a part: every KV_WARPS-th tile of [t0, t1), 8 query heads; (m, l, O) to shared memory. The sums on CUDA cores.
+// A warp's share of a part: every KV_WARPS-th tile of [t0, t1), 8 query heads; (m, l, O) to shared memory. For a cache of floats the sums on CUDA cores.
 template <class T, class QT, int HD>
 __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t h0, uint32_t nh, uint32_t len, uint32_t t0, uint32_t t1,
                                             uint8_t *ring, uint64_t *valid, float *p_sh, float *m_out, float *l_out, float *o_out) {
@@ -139,7 +145,7 @@ __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b,
         }
     float m = -INFINITY, l = 0.f;                // of head lane / 4; l: this lane's share
     uint32_t next = t0 + warp;
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < KV_STAGES - 1; ++s) {
         if (next < t1) { const uint64_t w = kv_request<T, HD>(A, b, kvh, len, next, ring_s + s * L::BYTES); if (lane == 0u) valid[s] = w; }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -242,6 +248,184 @@ __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b,
         for (int i = 0; i < E; i += 2) { o_out[h * HD + elem(i)] = o[h][i / 2].x; o_out[h * HD + elem(i + 1)] = o[h][i / 2].y; }
 }
 
+// The same share on the tensor cores, for a cache of 16-bit values. m16n8k16 has 16 rows where a group has 8 heads: rows 0-7 carry the upper digit of the
+// heads' queries (or weights), rows 8-15 the lower, so that two digits cost what one would, and the two halves of an accumulator (both in the same
+// lane) are added at the end. A query of floats over F16 is q 2^e = hi + lo with 2^e such that the head's largest is below 2^15 (22 bits); a query of the
+// cache's own type is its upper digit. A weight is 2^(x - m) = hi + lo likewise, 22 bits in F16 (with m chosen KV_P_BIAS lower, so that small weights keep
+// their lower digit), 16 in BF16, where the output is rounded to 8. m is moved only when the maximum has grown by more than KV_SLACK, as
+// that rescales the accumulators; the weights stay below 2^(KV_P_BIAS + KV_SLACK).
+constexpr float KV_P_BIAS = 6.f, KV_SLACK = 8.f;
+
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+template <class T> __device__ __forceinline__ float2 unpack2(uint32_t x);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x)); }
+template <class T> __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <class T, class QT, int HD>
+__device__ __forceinline__ void attend_part_mma(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t h0, uint32_t nh, uint32_t len, uint32_t t0, uint32_t t1,
+                                            uint8_t *ring, uint64_t *valid, float *m_out, float *l_out, float *o_out) {
+    using L = KvTile<T, HD>;
+    constexpr bool TWO = !std::is_same<T, QT>::value;
+    constexpr float BIAS = std::is_same<T, __half>::value ? KV_P_BIAS : 0.f;
+    constexpr int KS = HD / 16, NT = L::TP / 8, DT = HD / 8;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c2 = (lane & 3u) * 2u;
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+    uint32_t next = t0 + warp;
+#pragma unroll 1
+    for (int s = 0; s < KV_STAGES - 1; ++s) {
+        if (next < t1) { const uint64_t w = kv_request<T, HD>(A, b, kvh, len, next, ring_s + s * L::BYTES); if (lane == 0u) valid[s] = w; }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next += KV_WARPS;
+    }
+    uint32_t st = 0;
+    // the query of head g: elements 16 s + c2, + 1, + 8, + 9 of it
+    uint32_t qh[KS][2], ql[TWO ? KS : 1][2];
+    float sc = A.scale_log2;
+    {
+        const QT *qp = reinterpret_cast<const QT *>(A.q) + (uint64_t)b * A.q_stride + (uint64_t)(h0 + g) * HD;
+        const bool have = g < nh;
+        if constexpr (TWO) {
+            float most = 0.f;
+            if (have)
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float2 x = *reinterpret_cast<const float2 *>(qp + 16 * s + c2 + 8 * u);
+                        most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
+                    }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            int e = 0;
+            if (most > 0.f && most < INFINITY) e = min(141 - (int)(__float_as_uint(most) >> 23), 126);       // 127 + 14: the largest in [2^14, 2^15)
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+            sc *= 1.f / up;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float2 x = make_float2(0.f, 0.f);
+                    if (have) x = *reinterpret_cast<const float2 *>(qp + 16 * s + c2 + 8 * u);
+                    x.x *= up; x.y *= up;
+                    qh[s][u] = pack2<T>(x.x, x.y);
+                    const float2 h = unpack2<T>(qh[s][u]);
+                    ql[s][u] = pack2<T>(x.x - h.x, x.y - h.y);
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) qh[s][u] = have ? *reinterpret_cast<const uint32_t *>(qp + 16 * s + c2 + 8 * u) : 0u;
+        }
+    }
+    float o[DT][4], m = -INFINITY, l = 0.f;      // m, l: of head g; l this lane's share
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] = 0.f;
+    // what a lane addresses of four 8 x 8 pieces: K rows lane % 8 and pieces lane / 8; V rows (lane / 8 % 2) * 8 + lane % 8 and pieces lane / 16
+    const uint32_t kr = lane & 7u, kc = lane >> 3, vr = (lane >> 3 & 1u) * 8u + (lane & 7u), vc = lane >> 4;
+    for (uint32_t t = t0 + warp; t < t1; t += KV_WARPS) {
+        const uint32_t fill = st == 0u ? KV_STAGES - 1 : st - 1u;
+        asm volatile("cp.async.wait_group %0;" :: "n"(KV_STAGES - 2) : "memory");
+        __syncwarp();
+        if (next < t1) { const uint64_t w = kv_request<T, HD>(A, b, kvh, len, next, ring_s + fill * L::BYTES); if (lane == 0u) valid[fill] = w; }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next += KV_WARPS;
+        const uint64_t live = valid[st];
+        const uint32_t kt = ring_s + st * L::BYTES, vt = kt + L::TP * L::ROW;
+        float x[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {        // two runs of eight positions, each in two sums
+            float c[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s += 2) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t row = (uint32_t)(n + i) * 8u + kr;
+                    uint32_t k[4];
+                    ldsm4(k, kt + row * L::ROW + L::swizzle(row, (uint32_t)s * 2u + kc) * 16u);
+                    mma16816<T>(c[2 * i], qh[s][0], TWO ? ql[TWO ? s : 0][0] : 0u, qh[s][1], TWO ? ql[TWO ? s : 0][1] : 0u, k[0], k[1]);
+                    mma16816<T>(c[2 * i + 1], qh[s + 1][0], TWO ? ql[TWO ? s + 1 : 0][0] : 0u, qh[s + 1][1], TWO ? ql[TWO ? s + 1 : 0][1] : 0u, k[2], k[3]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float v = TWO ? (c[2 * i][j] + c[2 * i + 1][j]) + (c[2 * i][j + 2] + c[2 * i + 1][j + 2]) : c[2 * i][j] + c[2 * i + 1][j];
+                    const uint32_t pos = (uint32_t)(n + i) * 8u + c2 + (uint32_t)j;
+                    x[n + i][j] = (live >> pos) & 1u ? v * sc : -INFINITY;
+                }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(x[n][0], x[n][1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const bool move = mx > m + KV_SLACK;     // from -infinity too
+        if (__any_sync(0xffffffffu, move)) {
+            const float to = move ? mx : m, alpha = move ? exp2f(m - to) : 1.f;
+            m = to;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m - BIAS;
+        uint32_t pa[NT / 2][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float p0 = exp2f(x[n][0] - base), p1 = exp2f(x[n][1] - base);
+            l += p0 + p1;
+            const uint32_t hi = pack2<T>(p0, p1);
+            const float2 h = unpack2<T>(hi);
+            pa[n / 2][(n & 1) * 2] = hi;
+            pa[n / 2][(n & 1) * 2 + 1] = pack2<T>(p0 - h.x, p1 - h.y);
+        }
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j)
+#pragma unroll
+            for (int d = 0; d < DT; d += 2) {
+                const uint32_t row = (uint32_t)j * 16u + vr;
+                uint32_t v[4];
+                ldsm4_t(v, vt + row * L::ROW + L::swizzle(row, (uint32_t)d + vc) * 16u);
+                mma16816<T>(o[d], pa[j][0], pa[j][1], pa[j][2], pa[j][3], v[0], v[1]);
+                mma16816<T>(o[d + 1], pa[j][0], pa[j][1], pa[j][2], pa[j][3], v[2], v[3]);
+            }
+        __syncwarp();
+        st = st + 1u == KV_STAGES ? 0u : st + 1u;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if ((lane & 3u) == 0u) { m_out[g] = m - BIAS; l_out[g] = l; }
+    __syncthreads();                             // the rings are read no more
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<float2 *>(o_out + g * HD + d * 8u + c2) = make_float2(o[d][0] + o[d][2], o[d][1] + o[d][3]);
+}
+
 // the new row of sequence b, K/V head kvh, to its page (the whole block)
 template <class T, class QT, int HD>
 __device__ __forceinline__ void kv_write_new(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t pos) {
@@ -264,14 +448,14 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) k_kv_attend(AttendArgs A) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ uint64_t s_sum[KV_WARPS], s_base, s_valid[KV_WARPS][KV_STAGES];
     __shared__ uint32_t s_b;
-    __shared__ __align__(16) float s_p[KV_WARPS][40], s_m[KV_WARPS][8], s_l[KV_WARPS][8];
+    __shared__ __align__(16) float s_p[sizeof(T) == 4 ? KV_WARPS : 1][40], s_m[KV_WARPS][8], s_l[KV_WARPS][8], s_scale[8];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, HG = A.n_kv * A.gsplit;
     QT *const out = reinterpret_cast<QT *>(A.out);
 
     // how many tiles there are, and the sequence in which this block's run begins
     const uint32_t per = (A.n_seqs + KV_WARPS * 32u - 1u) / (KV_WARPS * 32u), b_lo = min(A.n_seqs, tid * per), b_hi = min(A.n_seqs, b_lo + per);
     uint64_t mine = 0;
-    for (uint32_t b = b_lo; b < b_hi; ++b) mine += (kv_len(A, b) + L::TP - 1u) / L::TP;
+    for (uint32_t b = b_lo; b < b_hi; ++b) mine += kv_cost<L::TP>(kv_len(A, b));
     uint64_t incl = mine;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) { const uint64_t x = __shfl_up_sync(0xffffffffu, incl, w); if (lane >= (uint32_t)w) incl += x; }
@@ -284,7 +468,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) k_kv_attend(AttendArgs A) {
     uint64_t base = (incl - mine) * HG;
     if (u0 < u1 && base <= u0 && u0 < incl * HG) {
         uint32_t b = b_lo;
-        for (;; ++b) { const uint64_t n = (uint64_t)((kv_len(A, b) + L::TP - 1u) / L::TP) * HG; if (u0 < base + n) break; base += n; }
+        for (;; ++b) { const uint64_t n = (uint64_t)kv_cost<L::TP>(kv_len(A, b)) * HG; if (u0 < base + n) break; base += n; }
         s_b = b; s_base = base;
     }
     for (uint32_t b = blockIdx.x; b < A.n_seqs; b += gridDim.x) {
@@ -301,76 +485,119 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) k_kv_attend(AttendArgs A) {
         base = s_base;
         uint64_t u = u0;
         while (u < u1) {
-            const uint32_t len = kv_len(A, b), nt = (len + L::TP - 1u) / L::TP;
-            if (u >= base + (uint64_t)nt * HG) { base += (uint64_t)nt * HG; ++b; continue; }
-            const uint32_t hg = (uint32_t)((u - base) / nt), t0 = (uint32_t)((u - base) - (uint64_t)hg * nt), t1 = (uint32_t)min((uint64_t)nt, t0 + (u1 - u));
+            const uint32_t len = kv_len(A, b), nt = (len + L::TP - 1u) / L::TP, cost = kv_cost<L::TP>(len);
+            if (u >= base + (uint64_t)cost * HG) { base += (uint64_t)cost * HG; ++b; continue; }
+            const uint32_t hg = (uint32_t)((u - base) / cost);
+            const uint64_t end = base + (uint64_t)(hg + 1u) * cost;             // of this head; its tiles are the last nt units before it
+            const uint32_t t0 = end - u >= nt ? 0u : nt - (uint32_t)(end - u), t1 = end <= u1 ? nt : end - u1 >= nt ? 0u : nt - (uint32_t)(end - u1);
+            u = min(end, u1);
+            if (t0 == t1) continue;              // the run ends inside the head's surcharge
             const uint32_t kvh = hg / A.gsplit, g0 = (hg % A.gsplit) * 8u, h0 = kvh * A.G + g0, nh = min(8u, A.G - g0);
             if (A.k_new && t1 == nt && len == (uint32_t)A.lens[b]) kv_write_new<T, QT, HD>(A, b, kvh, len - 1u);
             __syncthreads();                     // the new row is written; what the last head left in shared memory has been read
             float *o_sh = reinterpret_cast<float *>(sm);
-            attend_part_f32<T, QT, HD>(A, b, kvh, h0, nh, len, t0, t1, sm + warp * KV_STAGES * L::BYTES, s_valid[warp], s_p[warp], s_m[warp], s_l[warp], o_sh + warp * 8u * HD);
+            uint8_t *ring = sm + warp * KV_STAGES * L::BYTES;
+            float *o_warp = o_sh + warp * 8u * HD;
+            if constexpr (sizeof(T) == 4)
+                attend_part_f32<T, QT, HD>(A, b, kvh, h0, nh, len, t0, t1, ring, s_valid[warp], s_p[sizeof(T) == 4 ? warp : 0], s_m[warp], s_l[warp], o_warp);
+            else
+                attend_part_mma<T, QT, HD>(A, b, kvh, h0, nh, len, t0, t1, ring, s_valid[warp], s_m[warp], s_l[warp], o_warp);
             __syncthreads();
             // the warps' parts together
             const bool whole = t0 == 0u && t1 == nt;
             const uint32_t slot = blockIdx.x * 2u + (t0 == 0u ? 1u : 0u);
-            for (uint32_t i = tid; i < 8u * HD; i += KV_WARPS * 32u) {
-                const uint32_t h = i / HD;
-                float M = s_m[0][h], sum = 0.f, w[KV_WARPS], lt = 0.f;
+            if (tid < 8u) {
+                float M = s_m[0][tid], lt = 0.f;
 #pragma unroll
-                for (uint32_t j = 1; j < KV_WARPS; ++j) M = fmaxf(M, s_m[j][h]);
+                for (uint32_t j = 1; j < KV_WARPS; ++j) M = fmaxf(M, s_m[j][tid]);
                 const float z = M == -INFINITY ? 0.f : M;
 #pragma unroll
-                for (uint32_t j = 0; j < KV_WARPS; ++j) { w[j] = exp2f(s_m[j][h] - z); sum += w[j] * o_sh[j * 8u * HD + i]; lt += w[j] * s_l[j][h]; }
-                if (whole) {
-                    if (h < nh) {
-                        out[((uint64_t)b * A.n_q + h0) * HD + i] = from_f32<QT>(lt == 0.f ? 0.f : sum / lt);
-                        if (A.lse && i % HD == 0u) A.lse[(uint64_t)b * A.n_q + h0 + h] = lt == 0.f ? -INFINITY : M * 0.693147180559945309f + logf(lt);
-                    }
-                } else {
-                    A.part[(uint64_t)slot * 8u * HD + i] = sum;
-                    if (i % HD == 0u) { A.part_ml[slot * 16u + h] = M; A.part_ml[slot * 16u + 8u + h] = lt; }
-                }
+                for (uint32_t j = 0; j < KV_WARPS; ++j) { const float w = exp2f(s_m[j][tid] - z); lt += w * s_l[j][tid]; s_m[j][tid] = w; }
+                s_scale[tid] = whole ? lt == 0.f ? 0.f : 1.f / lt : 1.f;
+                if (!whole) { A.part_ml[slot * 16u + tid] = M; A.part_ml[slot * 16u + 8u + tid] = lt; }
+                else if (tid < nh && A.lse) A.lse[(uint64_t)b * A.n_q + h0 + tid] = kv_lse(M, lt);
             }
-            if (t0 == 0u && t1 < nt) { parts_b = b; parts_h = hg; parts_n = (uint32_t)((base + (uint64_t)(hg + 1u) * nt - 1u) / q) - blockIdx.x; }
-            u += t1 - t0;
+            __syncthreads();
+            for (uint32_t i = tid * 4u; i < 8u * HD; i += KV_WARPS * 128u) {
+                const uint32_t h = i / HD;
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t j = 0; j < KV_WARPS; ++j) {
+                    const float4 y = *reinterpret_cast<const float4 *>(o_sh + j * 8u * HD + i);
+                    const float w = s_m[j][h];
+                    x[0] += w * y.x; x[1] += w * y.y; x[2] += w * y.z; x[3] += w * y.w;
+                }
+                const float f = s_scale[h];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = x[e] * f;
+                if (!whole) store_vals<4>(A.part + (uint64_t)slot * 8u * HD + i, x);
+                else if (h < nh) store_vals<4>(out + ((uint64_t)b * A.n_q + h0) * HD + i, x);
+            }
+            if (t0 == 0u && t1 < nt) { parts_b = b; parts_h = hg; parts_n = (uint32_t)((end - 1u) / q) - blockIdx.x; }
         }
     }
     if (tid == 0u) { A.meta[blockIdx.x * 4u] = parts_b; A.meta[blockIdx.x * 4u + 1u] = parts_h; A.meta[blockIdx.x * 4u + 2u] = parts_n; }
 }
 
-// grid (blocks of k_kv_attend, 8 heads): the head that begins in block x, if it ends in a later one
+// Grid (blocks of k_kv_attend, 8 heads): the head that begins in block x, if it ends in a later one. HD / 4 threads have four values each, 1024 / HD such rows of
+// threads every so many-th part; what bounds it is the chain of dependent reads, so the first parts are requested with the weights.
 template <class QT, int HD>
-__global__ void __launch_bounds__(128) k_kv_attend_join(AttendArgs A) {
+__global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
     pdl_prologue();
+    constexpr uint32_t COLS = HD / 4, ROWS = 256u / COLS, AHEAD = 4u;
     extern __shared__ float s_w[];               // a weight for every part
-    __shared__ float s_red[4], s_l;
-    const uint32_t c = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, n = A.meta[c * 4u + 2u];
+    __shared__ float s_max[8], s_sum[8];
+    __shared__ __align__(16) float s_o[ROWS][HD];
+    const uint32_t c = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, col = tid % COLS, row = tid / COLS;
+    const uint4 meta = *reinterpret_cast<const uint4 *>(A.meta + c * 4u);
+    const uint32_t n = meta.z;
     if (n == 0u) return;
-    const uint32_t b = A.meta[c * 4u], hg = A.meta[c * 4u + 1u], g0 = (hg % A.gsplit) * 8u, head = (hg / A.gsplit) * A.G + g0 + h;
+    const uint32_t b = meta.x, hg = meta.y, g0 = (hg % A.gsplit) * 8u, head = (hg / A.gsplit) * A.G + g0 + h;
     if (g0 + h >= A.G) return;
     auto slot = [&](uint32_t p) { return p == 0u ? c * 2u + 1u : (c + p) * 2u; };
-    float M = -INFINITY;
-    for (uint32_t p = tid; p <= n; p += 128u) M = fmaxf(M, A.part_ml[slot(p) * 16u + h]);
+    auto part = [&](uint32_t p) { return *reinterpret_cast<const float4 *>(A.part + ((uint64_t)slot(p) * 8u + h) * HD + col * 4u); };
+    float4 x[AHEAD];
+#pragma unroll
+    for (uint32_t i = 0; i < AHEAD; ++i) x[i] = row + i * ROWS <= n ? part(row + i * ROWS) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, l = 0.f;
+    for (uint32_t p = tid; p <= n; p += 256u) {  // once, unless a device has more than 256 multiprocessors
+        const float m = A.part_ml[slot(p) * 16u + h], lp = A.part_ml[slot(p) * 16u + 8u + h], to = fmaxf(M, m), z = to == -INFINITY ? 0.f : to;
+        l = l * exp2f(M - z) + lp * exp2f(m - z);
+        M = to;
+        s_w[p] = m;
+    }
+    const float M0 = M;
     for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
-    if ((tid & 31u) == 0u) s_red[tid >> 5] = M;
+    if ((tid & 31u) == 0u) s_max[tid >> 5] = M;
     __syncthreads();
-    M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    M = s_max[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) M = fmaxf(M, s_max[i]);
     const float z = M == -INFINITY ? 0.f : M;
-    for (uint32_t p = tid; p <= n; p += 128u) s_w[p] = exp2f(A.part_ml[slot(p) * 16u + h] - z);
+    l *= exp2f(M0 - z);
+    for (uint32_t p = tid; p <= n; p += 256u) s_w[p] = exp2f(s_w[p] - z);
+    for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+    if ((tid & 31u) == 0u) s_sum[tid >> 5] = l;
     __syncthreads();
-    if (tid < 32u) {
-        float l = 0.f;
-        for (uint32_t p = tid; p <= n; p += 32u) l += s_w[p] * A.part_ml[slot(p) * 16u + 8u + h];
-        for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-        if (tid == 0u) { s_l = l; if (A.lse) A.lse[(uint64_t)b * A.n_q + head] = l == 0.f ? -INFINITY : M * 0.693147180559945309f + logf(l); }
-    }
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l += s_sum[i];
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, float4 y) { o.x += w * y.x; o.y += w * y.y; o.z += w * y.z; o.w += w * y.w; };
+#pragma unroll
+    for (uint32_t i = 0; i < AHEAD; ++i)
+        if (row + i * ROWS <= n) add(s_w[row + i * ROWS], x[i]);
+#pragma unroll 4
+    for (uint32_t p = row + AHEAD * ROWS; p <= n; p += ROWS) add(s_w[p], part(p));
+    *reinterpret_cast<float4 *>(&s_o[row][col * 4u]) = o;
     __syncthreads();
-    for (uint32_t i = tid; i < HD; i += 128u) {
+    for (uint32_t i = tid; i < HD; i += 256u) {
         float sum = 0.f;
-#pragma unroll 8
-        for (uint32_t p = 0; p <= n; ++p) sum += s_w[p] * A.part[((uint64_t)slot(p) * 8u + h) * HD + i];
-        reinterpret_cast<QT *>(A.out)[((uint64_t)b * A.n_q + head) * HD + i] = from_f32<QT>(s_l == 0.f ? 0.f : sum / s_l);
+#pragma unroll
+        for (uint32_t r = 0; r < ROWS; ++r) sum += s_o[r][i];
+        reinterpret_cast<QT *>(A.out)[((uint64_t)b * A.n_q + head) * HD + i] = from_f32<QT>(l == 0.f ? 0.f : sum / l);
     }
+    if (tid == 0u && A.lse) A.lse[(uint64_t)b * A.n_q + head] = kv_lse(M, l);
 }
 
 template <class T, class QT, int HD> static int launch_attend(const AttendArgs &A, uint32_t blocks, cudaStream_t s) {
@@ -387,7 +614,7 @@ template <class T, class QT, int HD> static int launch_attend(const AttendArgs &
     RC_LAUNCHED();
     prof_end(s);
     prof_begin("kv_attend_join", s);
-    RC_LAUNCH((k_kv_attend_join<QT, HD>), dim3(blocks, 8), 128, (blocks + 1u) * sizeof(float), s, A);
+    RC_LAUNCH((k_kv_attend_join<QT, HD>), dim3(blocks, 8), 256, (blocks + 1u) * sizeof(float), s, A);
     RC_LAUNCHED();
     prof_end(s);
     return 1;
@@ -494,9 +721,9 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     auto few = [](uint64_t n) { return n < 8192u ? n : 8192u; };      // more than that of one thing is blocks enough
     const uint64_t runs = (few(tiles) * few(n_seqs) * few(A.n_kv * A.gsplit) + KV_MIN_TILES - 1u) / KV_MIN_TILES;
     const uint32_t blocks = runs < sms ? (uint32_t)runs : sms;
-    A.part = (float *)workspace_dev;
+    A.meta = (uint32_t *)workspace_dev;
+    A.part = (float *)(A.meta + (size_t)blocks * 4u);
     A.part_ml = A.part + (size_t)blocks * 2u * 8u * hd;
-    A.meta = (uint32_t *)(A.part_ml + (size_t)blocks * 2u * 16u);
     cudaStream_t s = (cudaStream_t)stream;
     if (kv->type == VT_F32) return launch_attend_hd<float, float>(A, hd, blocks, s);
     if (kv->type == VT_BF16) return launch_attend_hd<__nv_bfloat16, __nv_bfloat16>(A, hd, blocks, s);

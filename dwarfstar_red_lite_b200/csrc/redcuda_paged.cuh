@@ -4,7 +4,8 @@
 
 namespace rc {
 
-constexpr int KV_WARPS = 4, KV_STAGES = 3;
+constexpr int KV_WARPS = 6, KV_STAGES = 2;
+constexpr uint32_t KV_HEAD_COST = 12u;           // what a head's begin and end take, in tiles
 constexpr uint32_t KV_MIN_TILES = 4u;            // tiles that a block takes at least
 
 struct AttendArgs {
