@@ -11,18 +11,6 @@
 
 namespace rc {
 
-// The state slot of sequence b, or -1: none, out of range, or one that an earlier sequence has (two sequences would write it at once).
-// For the whole block (it meets a barrier).
-__device__ __forceinline__ int32_t delta_slot(const int32_t *slots, uint32_t n_slots, uint32_t b, uint32_t *status) {
-    if (!slots) return b < n_slots ? (int32_t)b : -1;
-    const int32_t s = slots[b];
-    bool bad = s < -1 || (s >= 0 && (uint32_t)s >= n_slots);
-    if (s >= 0) for (uint32_t i = threadIdx.x; i < b; i += blockDim.x) bad |= slots[i] == s;
-    bad = __syncthreads_or(bad);
-    if (bad && threadIdx.x == 0u && status) status[ST_SLOT] = 1u;
-    return bad ? -1 : s;
-}
-
 // Lanes of a row: S / E of them with E columns each, in pieces of four columns that lie 4 S / E apart, so that a quarter warp reads 128 bytes in a row.
 template <int S> struct DeltaLanes {
     static constexpr int E = S == 256 ? 8 : 4, LPR = S / E, RPW = 32 / LPR;      // a warp reads RPW rows at once
@@ -144,6 +132,9 @@ template <bool STEP> static int launch_scan_t(const DeltaArgs &A, uint32_t type,
     return type == VT_F32 ? launch_scan_s<float, STEP>(A, S, n_seqs, s) : type == VT_F16 ? launch_scan_s<__half, STEP>(A, S, n_seqs, s) : launch_scan_s<__nv_bfloat16, STEP>(A, S, n_seqs, s);
 }
 
+// In chunks on the tensor cores, or a token at a time
+static bool delta_in_chunks(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs) { return d->d_state == 128u && n_tokens >= 16u * (uint64_t)n_seqs; }
+
 // What a call's arguments have to be; fills the strides. rows: tokens of q, k, v and out
 static int delta_check(const redcuda_delta_dims *d, const char *who, uint32_t rows, uint32_t n_seqs, uint32_t n_slots, DeltaArgs &A) {
     RC_REQUIRE(d, "%s: null dimensions", who);
@@ -200,8 +191,9 @@ int redcuda_delta_step_device(const redcuda_delta_dims *d, uint32_t n_seqs, cons
 }
 
 uint64_t redcuda_delta_rule_workspace(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs) {
-    (void)d; (void)n_tokens; (void)n_seqs;
-    return 0;
+    DeltaArgs A{};
+    if (!delta_check(d, "delta rule", n_tokens, n_seqs, 1u, A)) return 0;
+    return delta_in_chunks(d, n_tokens, n_seqs) ? delta_chunk_workspace(d->type, d->n_group, d->dt_rank, n_tokens, n_seqs) : 0u;
 }
 
 int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs, const int32_t *cu_seqlens_dev, const int32_t *slots_dev,
@@ -220,7 +212,7 @@ int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, ui
     A.status = status_words();
     cudaStream_t s = (cudaStream_t)stream;
     prof_begin("delta_rule", s);
-    const int ok = launch_scan_t<false>(A, d->type, d->d_state, n_seqs, s);
+    const int ok = delta_in_chunks(d, n_tokens, n_seqs) ? launch_delta_chunks(A, d->type, n_seqs, (uint8_t *)workspace_dev, s) : launch_scan_t<false>(A, d->type, d->d_state, n_seqs, s);
     prof_end(s);
     return ok;
 }

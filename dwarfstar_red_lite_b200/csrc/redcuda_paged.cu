@@ -602,13 +602,8 @@ __global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
 
 template <class T, class QT, int HD> static int launch_attend(const AttendArgs &A, uint32_t blocks, cudaStream_t s) {
     constexpr size_t smem = (size_t)KV_WARPS * KV_STAGES * KvTile<T, HD>::BYTES;
-    static std::atomic<uint64_t> set{0};          // devices on which the limit has been raised
-    int dev = 0;
-    RC_CUDA(cudaGetDevice(&dev));
-    if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1u)) {
-        RC_CUDA(cudaFuncSetAttribute(k_kv_attend<T, QT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
+    static std::atomic<uint64_t> set{0};
+    if (!raise_smem_limit(reinterpret_cast<const void *>(k_kv_attend<T, QT, HD>), smem, set)) return 0;
     prof_begin("kv_attend", s);
     RC_LAUNCH((k_kv_attend<T, QT, HD>), blocks, KV_WARPS * 32, smem, s, A);
     RC_LAUNCHED();

@@ -26,6 +26,16 @@ inline uint32_t sm_count() {
     return c;
 }
 
+// raises a kernel's limit of dynamic shared memory once per device; set: a bit for each device on which that has been done
+inline int raise_smem_limit(const void *kernel, size_t bytes, std::atomic<uint64_t> &set) {
+    int dev = 0;
+    RC_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && (set.load(std::memory_order_relaxed) >> dev & 1u)) return 1;
+    RC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return 1;
+}
+
 #ifdef __CUDACC__
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
