@@ -9,28 +9,33 @@
 // where it is given in 16 bits, and products of lower digits with one another are left out (2^-22 of a product).
 // Values that are not finite must not reach a product with a zero of the triangle: they are taken out, and from their token on what depends on them is NaN.
 #include "redcuda_delta.cuh"
+#include "redcuda_tc_gemm.cuh"
 
 #include <math.h>
+#include <type_traits>
 
 namespace rc {
 
 constexpr int DC_T = 64, DC_S = 128;             // tokens of a chunk; the state
-constexpr uint32_t DC_TILE = DC_T * DC_S * 2u;   // a digit of the chunk's keys or queries: [token][128] with the 16-byte pieces of a row turned by its number
-constexpr uint32_t DC_SQ = DC_T * DC_T * 2u;     // a digit of T or P: [t][s], likewise
+// Operand tiles as the MMAs read them (K-major, no swizzle): [k / 8][row][8 values], 16 bytes a row and piece.
+constexpr uint32_t DC_KQ = 2u * DC_T * DC_S * 2u;        // a digit of the chunk's keys (rows 0 .. 63) and queries (64 .. 127), k: the state's columns
+constexpr uint32_t DC_KT = DC_T * DC_S * 2u;             // a digit of the keys transposed: rows: the state's columns, k: tokens
+constexpr uint32_t DC_SQ = DC_T * DC_T * 2u;             // a digit of T or P, rows t, k: s
 struct DcMeta {                                  // of a chunk and value head
     float dec[DC_T], kdec[DC_T];                 // exp(G_t), exp(G_last - G_t)
     float last, f_k, f_q, f_t, f_p;              // exp(G_last); what a digit's unit is worth in K, Q, T, P
-    uint32_t nan_from, bad_q[2], pad[120];       // tokens from which on everything is NaN; tokens whose query is not finite
+    float most_dec;                              // the largest exp(G_t)
+    uint32_t nan_from, bad_q[2], pad[119];       // tokens from which on everything is NaN; tokens whose query is not finite
 };
 static_assert(sizeof(DcMeta) == 1024, "copied in whole");
 constexpr uint32_t DC_REC = 4u * DC_SQ + (uint32_t)sizeof(DcMeta);       // T hi, T lo, P hi, P lo, meta
-__host__ __device__ constexpr uint32_t dc_keys(int dig) { return 2u * (uint32_t)dig * DC_TILE; }      // K hi (, K lo), Q hi (, Q lo)
+__host__ __device__ constexpr uint32_t dc_keys(int dig) { return (uint32_t)dig * (DC_KQ + DC_KT); }      // KQ hi (, lo), KT hi (, lo)
 
 // Chunks are numbered so that a sequence finds its own without the lengths of the others: chunk c of sequence b is number cu[b] / 64 + b + c.
 static uint64_t dc_slots(uint32_t n_tokens, uint32_t n_seqs) { return (uint64_t)n_tokens / DC_T + n_seqs; }
 
-__device__ __forceinline__ uint32_t dc_tile_at(uint32_t t, uint32_t piece) { return t * 256u + (piece ^ (t & 7u)) * 16u; }
-__device__ __forceinline__ uint32_t dc_sq_at(uint32_t t, uint32_t piece) { return t * 128u + (piece ^ (t & 7u)) * 16u; }
+__device__ __forceinline__ uint32_t dc_kq_at(uint32_t row, uint32_t piece) { return piece * 2048u + row * 16u; }       // of KQ, and of KT
+__device__ __forceinline__ uint32_t dc_sq_at(uint32_t row, uint32_t piece) { return piece * 1024u + row * 16u; }
 __device__ __forceinline__ uint32_t dc_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 2^e that brings `most` into [2^14, 2^15) (fp16 holds 2^15.99), and its reciprocal
 __device__ __forceinline__ void dc_scale(float most, float &up, float &unit) {
@@ -42,8 +47,8 @@ __device__ __forceinline__ void dc_scale(float most, float &up, float &unit) {
 __device__ __forceinline__ uint32_t dc_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
 __device__ __forceinline__ void dc_digits(float a, float b, uint32_t &hi, uint32_t &lo) {
     hi = dc_pack(a, b);
-    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    lo = dc_pack(a - h.x, b - h.y);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi)), l = __fadd2_rn(make_float2(a, b), make_float2(-h.x, -h.y));
+    lo = dc_pack(l.x, l.y);
 }
 __device__ __forceinline__ void dc_ldsm(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -98,27 +103,42 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
     if (chunk < 0 || chunk * DC_T >= hi - lo) return;
     const uint32_t t0 = (uint32_t)lo + (uint32_t)chunk * DC_T, n = min((uint32_t)DC_T, (uint32_t)hi - t0);
 
-    // rows 8 warp .. 8 warp + 7 of K and Q, four values a lane
-    float kx[8][4], qx[8][4], mk = 0.f, mq = 0.f;
+    // rows 8 warp .. 8 warp + 7 of K and Q: a lane has row lane % 8 and the 8-value pieces lane / 8 + 4 i
+    const uint32_t t = warp * 8u + (lane & 7u);
+    float kx[4][8], qx[4][8], mk = 0.f, mq = 0.f;
     if (tid < 4u) s_bad[tid >> 1][tid & 1u] = 0u;
     __syncthreads();
+    bool fk = true, fq = true;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-        const uint32_t t = warp * 8u + r;
-        float mr = 0.f, mr2 = 0.f;
-        bool fk = true, fq = true;
-        if (t < n) {
-            load_vals<4>(reinterpret_cast<const T *>(A.k) + (uint64_t)(t0 + t) * A.k_stride + (uint64_t)kh * DC_S + lane * 4u, kx[r]);
-            load_vals<4>(reinterpret_cast<const T *>(A.q) + (uint64_t)(t0 + t) * A.q_stride + (uint64_t)kh * DC_S + lane * 4u, qx[r]);
+    for (int i = 0; i < 4; ++i) {
+        constexpr int N = 16 / sizeof(T) < 8 ? 4 : 8;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { fk &= fabsf(kx[r][i]) < INFINITY; fq &= fabsf(qx[r][i]) < INFINITY; mr = fmaxf(mr, fabsf(kx[r][i])); mr2 = fmaxf(mr2, fabsf(qx[r][i])); }
+        for (int e = 0; e < 8; e += N) {
+            const uint32_t col = kh * DC_S + (lane >> 3) * 8u + i * 32u + e;
+            if (t < n) {
+                load_vals<N>(reinterpret_cast<const T *>(A.k) + (uint64_t)(t0 + t) * A.k_stride + col, *reinterpret_cast<float (*)[N]>(&kx[i][e]));
+                load_vals<N>(reinterpret_cast<const T *>(A.q) + (uint64_t)(t0 + t) * A.q_stride + col, *reinterpret_cast<float (*)[N]>(&qx[i][e]));
+            } else
+#pragma unroll
+                for (int j = 0; j < N; ++j) kx[i][e + j] = qx[i][e + j] = 0.f;
         }
-        const bool ak = __all_sync(0xffffffffu, fk), aq = __all_sync(0xffffffffu, fq);
-        if (t >= n || !ak) { mr = 0.f; for (int i = 0; i < 4; ++i) kx[r][i] = 0.f; }
-        if (t >= n || !aq) { mr2 = 0.f; for (int i = 0; i < 4; ++i) qx[r][i] = 0.f; }
-        if (lane == 0u && !ak) atomicOr(&s_bad[0][t >> 5], 1u << (t & 31u));
-        if (lane == 0u && !aq) atomicOr(&s_bad[1][t >> 5], 1u << (t & 31u));
-        mk = fmaxf(mk, mr); mq = fmaxf(mq, mr2);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { fk &= fabsf(kx[i][e]) < INFINITY; fq &= fabsf(qx[i][e]) < INFINITY; mk = fmaxf(mk, fabsf(kx[i][e])); mq = fmaxf(mq, fabsf(qx[i][e])); }
+    const uint32_t row_lanes = 0x01010101u << (lane & 7u), wk = __ballot_sync(0xffffffffu, !fk) & row_lanes, wq = __ballot_sync(0xffffffffu, !fq) & row_lanes;
+    if (wk) {                                    // a row that is not finite is taken out
+        mk = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) kx[i >> 3][i & 7] = 0.f;
+        if (lane < 8u) atomicOr(&s_bad[0][t >> 5], 1u << (t & 31u));
+    }
+    if (wq) {
+        mq = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) qx[i >> 3][i & 7] = 0.f;
+        if (lane < 8u) atomicOr(&s_bad[1][t >> 5], 1u << (t & 31u));
     }
     for (int w = 16; w; w >>= 1) { mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, w)); mq = fmaxf(mq, __shfl_xor_sync(0xffffffffu, mq, w)); }
     if (lane == 0u) { s_red[0][warp] = mk; s_red[1][warp] = mq; }
@@ -130,23 +150,34 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
     dc_scale(mq, up_q, f_q);
     uint8_t *const keys = ws + (slot * A.groups + kh) * dc_keys(DIG);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-        const uint32_t at = dc_tile_at(warp * 8u + r, lane >> 1) + (lane & 1u) * 8u;
-        auto put = [&](const float (&x)[4], float up, uint32_t tile) {
-            uint2 h, l;
-            dc_digits(x[0] * up, x[1] * up, h.x, l.x);
-            dc_digits(x[2] * up, x[3] * up, h.y, l.y);
-            *reinterpret_cast<uint2 *>(dig + tile * DC_TILE + at) = h;
-            *reinterpret_cast<uint2 *>(keys + tile * DC_TILE + at) = h;
-            if (DIG == 2) { *reinterpret_cast<uint2 *>(dig + (tile + 1u) * DC_TILE + at) = l; *reinterpret_cast<uint2 *>(keys + (tile + 1u) * DC_TILE + at) = l; }
+    for (uint32_t i = 0; i < 4u; ++i) {
+        auto put = [&](const float (&x)[8], float up, uint32_t row) {
+            const uint32_t at = dc_kq_at(row, (lane >> 3) + 4u * i);
+            uint4 h, l;
+            dc_digits(x[0] * up, x[1] * up, h.x, l.x); dc_digits(x[2] * up, x[3] * up, h.y, l.y);
+            dc_digits(x[4] * up, x[5] * up, h.z, l.z); dc_digits(x[6] * up, x[7] * up, h.w, l.w);
+            *reinterpret_cast<uint4 *>(dig + at) = h;
+            *reinterpret_cast<uint4 *>(keys + at) = h;
+            if (DIG == 2) { *reinterpret_cast<uint4 *>(dig + DC_KQ + at) = l; *reinterpret_cast<uint4 *>(keys + DC_KQ + at) = l; }
         };
-        put(kx[r], up_k, 0u);
-        put(qx[r], up_q, DIG);
+        put(kx[i], up_k, t);
+        put(qx[i], up_q, DC_T + t);
     }
     __syncthreads();
+    // the keys transposed: 8 x 8 blocks turned by ldmatrix; warp: eight tokens, four blocks of eight columns at a time
+#pragma unroll
+    for (uint32_t d = 0; d < (uint32_t)DIG; ++d)
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            uint32_t x[4];
+            dc_ldsm_t(x, dc_smem(dig) + d * DC_KQ + dc_kq_at(warp * 8u + (lane & 7u), i * 4u + (lane >> 3)));
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j)
+                *reinterpret_cast<uint32_t *>(keys + DIG * DC_KQ + d * DC_KT + dc_kq_at((i * 4u + j) * 8u + (lane >> 2), warp) + (lane & 3u) * 4u) = x[j];
+        }
     {   // warps 0-3: K K^T, 4-7: Q K^T; 16 rows each, the columns up to the diagonal
-        const uint32_t mt = warp & 3u, which = warp >> 2, a_at = dc_smem(dig) + which * DIG * DC_TILE, b_at = dc_smem(dig);
-        const uint32_t ar = mt * 16u + (lane & 15u), ac = lane >> 4, br = (lane & 7u) + (lane >> 4) * 8u, bc = (lane >> 3) & 1u;
+        const uint32_t mt = warp & 3u, which = warp >> 2, a_at = dc_smem(dig), b_at = a_at;
+        const uint32_t ar = which * DC_T + mt * 16u + (lane & 15u), ac = lane >> 4, br = (lane & 7u) + (lane >> 4) * 8u, bc = (lane >> 3) & 1u;
         float c[4][2][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -157,17 +188,17 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
 #pragma unroll 2
         for (uint32_t s = 0; s < 8u; ++s) {
             uint32_t ah[4], al[4];
-            dc_ldsm(ah, a_at + dc_tile_at(ar, 2u * s + ac));
-            if (DIG == 2) dc_ldsm(al, a_at + DC_TILE + dc_tile_at(ar, 2u * s + ac));
+            dc_ldsm(ah, a_at + dc_kq_at(ar, 2u * s + ac));
+            if (DIG == 2) dc_ldsm(al, a_at + DC_KQ + dc_kq_at(ar, 2u * s + ac));
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i)
                 if (i <= mt) {
                     uint32_t x[4];
-                    dc_ldsm(x, b_at + dc_tile_at(i * 16u + br, 2u * s + bc));
+                    dc_ldsm(x, b_at + dc_kq_at(i * 16u + br, 2u * s + bc));
                     dc_mma(c[i][0], ah, x[0], x[1]); dc_mma(c[i][1], ah, x[2], x[3]);
                     if (DIG == 2) {
                         dc_mma(c[i][0], al, x[0], x[1]); dc_mma(c[i][1], al, x[2], x[3]);
-                        dc_ldsm(x, b_at + DC_TILE + dc_tile_at(i * 16u + br, 2u * s + bc));
+                        dc_ldsm(x, b_at + DC_KQ + dc_kq_at(i * 16u + br, 2u * s + bc));
                         dc_mma(c[i][0], ah, x[0], x[1]); dc_mma(c[i][1], ah, x[2], x[3]);
                     }
                 }
@@ -210,6 +241,8 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
             double sum = g[1];
             for (int w = 1; w < 32; w <<= 1) { const double x = __shfl_up_sync(0xffffffffu, sum, w); if (lane >= (uint32_t)w) sum += x; }
             const double before = sum - g[1], last = __shfl_sync(0xffffffffu, sum, 31);
+            float most_dec = fmaxf(expf((float)(before + g[0])), expf((float)(before + g[1])));
+            for (int w = 16; w; w >>= 1) most_dec = fmaxf(most_dec, __shfl_xor_sync(0xffffffffu, most_dec, w));
             const uint32_t m0 = __ballot_sync(0xffffffffu, bad[0]), m1 = __ballot_sync(0xffffffffu, bad[1]);
             const uint32_t first0 = m0 ? 2u * ((uint32_t)__ffs((int)m0) - 1u) : (uint32_t)DC_T, first1 = m1 ? 2u * ((uint32_t)__ffs((int)m1) - 1u) + 1u : (uint32_t)DC_T;
 #pragma unroll
@@ -220,28 +253,32 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
                 meta->dec[t] = expf((float)G); meta->kdec[t] = expf((float)(last - G));
             }
             if (lane == 0u) {
-                meta->last = expf((float)last); meta->f_k = f_k; meta->f_q = f_q;
+                meta->last = expf((float)last); meta->f_k = f_k; meta->f_q = f_q; meta->most_dec = most_dec;
                 meta->nan_from = min(first0, first1); meta->bad_q[0] = s_bad[1][0]; meta->bad_q[1] = s_bad[1][1];
             }
         }
         dc_half_sync(half);
-        // A below the diagonal; P and its digits: pieces of eight columns, four a thread
+        // A below the diagonal; P and its digits: pieces of eight columns, four a thread, whose tokens run along the lanes
         float p[4][8], most = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t id = ht + i * 128u, t = id >> 3, s0 = (id & 7u) * 8u;
+            const uint32_t t = ht & 63u, s0 = (2u * i + (ht >> 6)) * 8u;
+            const float bt = s_beta[half][t];
+            const double Gt = s_cum[half][t];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t s = s0 + j;
-                p[i][j] = 0.f;
-                float a = 0.f;
-                if (s <= t) {
-                    const float ratio = s == t ? 1.f : expf((float)(s_cum[half][t] - s_cum[half][s]));
-                    p[i][j] = s_qk[t * DC_PITCH + s] * ratio;
-                    a = s_beta[half][t] * s_kk[t * DC_PITCH + s] * ratio;
-                    most = fmaxf(most, fabsf(p[i][j]));
+            for (int j = 0; j < 8; j += 4) {
+                const float4 qk = *reinterpret_cast<const float4 *>(s_qk + t * DC_PITCH + s0 + j), kk = *reinterpret_cast<const float4 *>(s_kk + t * DC_PITCH + s0 + j);
+                const float qv[4] = {qk.x, qk.y, qk.z, qk.w}, kv[4] = {kk.x, kk.y, kk.z, kk.w};
+                float a[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t s = s0 + j + e;
+                    const float ratio = s < t ? expf((float)(Gt - s_cum[half][s])) : 1.f;
+                    p[i][j + e] = s <= t ? qv[e] * ratio : 0.f;
+                    a[e] = s <= t ? bt * kv[e] * ratio : 0.f;
+                    most = fmaxf(most, fabsf(p[i][j + e]));
                 }
-                s_a[t * DC_PITCH + s] = a;
+                *reinterpret_cast<float4 *>(s_a + t * DC_PITCH + s0 + j) = make_float4(a[0], a[1], a[2], a[3]);
             }
         }
         most = dc_half_max(most, s_m, half);
@@ -256,7 +293,7 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
             *reinterpret_cast<uint4 *>(to + DC_SQ + dc_sq_at(t, piece)) = l;
         };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const uint32_t id = ht + i * 128u; put(p[i], up, id >> 3, id & 7u, rec + 2u * DC_SQ); }
+        for (uint32_t i = 0; i < 4u; ++i) put(p[i], up, ht & 63u, 2u * i + (ht >> 6), rec + 2u * DC_SQ);
         // the diagonal blocks of the inverse: warp hw has block hw, lane c column c
         {
             const uint32_t o = hw * 16u, c = lane & 15u;
@@ -302,61 +339,109 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
         most = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t id = ht + i * 128u, t = id >> 3, s0 = (id & 7u) * 8u;
+            const uint32_t t = ht & 63u, s0 = (2u * i + (ht >> 6)) * 8u;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t s = s0 + j;
-                p[i][j] = s <= t ? s_t[t * DC_PITCH + s] * s_beta[half][s] : 0.f;
-                most = fmaxf(most, fabsf(p[i][j]));
+            for (int j = 0; j < 8; j += 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(s_t + t * DC_PITCH + s0 + j);
+                const float v4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t s = s0 + j + e;
+                    p[i][j + e] = s <= t ? v4[e] * s_beta[half][s] : 0.f;
+                    most = fmaxf(most, fabsf(p[i][j + e]));
+                }
             }
         }
         most = dc_half_max(most, s_m, half);
         dc_scale(most, up, unit);
         if (ht == 0u) meta->f_t = unit;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const uint32_t id = ht + i * 128u; put(p[i], up, id >> 3, id & 7u, rec); }
+        for (uint32_t i = 0; i < 4u; ++i) put(p[i], up, ht & 63u, 2u * i + (ht >> 6), rec);
         dc_half_sync(half);
     }
 }
 
 // ---- the states through their chunks -------------------------------------------------------------------------------------------------------------
-// A warp has 16 rows of a state as accumulators of m16n8k16 (64 registers), and what is computed for a row needs no other row, so warps share nothing but the chunk's operands in shared memory
-// and meet once a chunk: S k and S q (operand A: the state's digits), R, D = T R (A: R's digits), the outputs (A: D's), the state (A: those of D times its decays). An accumulator's layout is that of
-// an operand A, so that nothing is exchanged between lanes. The scale of a row's digits is its own.
-// Chunk by chunk the operands come by bulk copies into one of two stages.
-constexpr uint32_t DC_SPIN_LIMIT = 1u << 22;     // polls of a try_wait that is itself limited in time: far beyond any real wait
+// A block has the 128 rows of one state: row j is lane j of tensor memory, and two threads (of warps w and w + 4) have it in registers, 64 columns each. A chunk is four products on tcgen05,
+// with an operand A that the threads write to tensor memory as digits (each row under a scale of its own) and an operand B that bulk copies bring to shared memory:
+//     M1  [S k | S q] = S [K | Q]^T      M2  D = R T^T      M4  D' K (the state's)      M3  D P^T (the outputs')
+// between them the threads make R of M1's result, D and D' = D exp(G_last - G) of M2's, the new S of M4's, the outputs of M1's and M3's. Of four further warps one issues the products and fetches their
+// operands (a tile again as soon as the product that reads it is done), one fetches the values, one stores the outputs. What bounds it is the chain M1, R, M2, D', M4, S: each link waits for the one before, so what is
+// not a link (the outputs, the digits of D, the largest of S) comes behind the hand-over of one. The scales of R and S come from bounds, which need no exchange between a row's two threads: up to 2^13
+// too large costs nothing, as two fp16 digits reach from 2^16 down to 2^-24.
+// The adder of the tensor cores truncates, so lower digits go first and M1's sums are kept in two halves of 64 columns each, which are added in fp32.
+constexpr uint32_t DC_THREADS = 384u, DC_ROW_WARPS = 8u, DC_CONTROL = 8u, DC_LOADER = 9u, DC_STORER = 10u;
+// registers: 384 threads are launched with 168 each, of which the four further warps keep 72 and the threads of the rows have 216 (256 x 216 + 128 x 72 = 384 x 168)
+constexpr uint32_t DC_REGS_ROWS = 216u, DC_REGS_CONTROL = 72u;
+static_assert(256u * DC_REGS_ROWS + 128u * DC_REGS_CONTROL <= 384u * 168u, "a split above the launch's registers waits forever");
+constexpr uint32_t DC_SPIN_LIMIT = 1u << 26;     // polls of some twenty cycles: more than half a second, far beyond any real wait
+enum : uint32_t { DT_S = 0, DT_M1 = 128, DT_D = 128, DT_DK = 192, DT_M4 = 256, DT_R = 384, DT_M3 = 384, DT_M2 = 448 };      // columns of tensor memory; M1: two accumulators of 128
+enum : uint32_t { DB_KQ, DB_T, DB_PK, DB_META0, DB_META1, DB_V, DB_M1, DB_M2, DB_M3, DB_M4, DB_OFREE, DB_R, DB_DK, DB_D, DB_S, DB_VFREE, DB_OUT, DB_PAIR, DB_COUNT = DB_PAIR + 4 };
+constexpr uint32_t dc_smem_bytes(int dig, uint32_t size) { return dc_keys(dig) + 4u * DC_SQ + 2u * (uint32_t)sizeof(DcMeta) + 2u * DC_T * DC_S * size; }
+static_assert(dc_smem_bytes(1, 2u) >= 114u * 1024u && dc_smem_bytes(2, 4u) < 220u * 1024u, "one block an SM: it takes all of the tensor memory");
 
-// the digits of x (rows g and g + 8 of a 16 x 16 step) as operand A
-__device__ __forceinline__ void dc_operand(const float (&x0)[4], const float (&x1)[4], float up0, float up1, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-    dc_digits(x0[0] * up0, x0[1] * up0, hi[0], lo[0]);
-    dc_digits(x0[2] * up1, x0[3] * up1, hi[1], lo[1]);
-    dc_digits(x1[0] * up0, x1[1] * up0, hi[2], lo[2]);
-    dc_digits(x1[2] * up1, x1[3] * up1, hi[3], lo[3]);
+__device__ __forceinline__ void dc_mma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_desc, uint32_t b_high, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 d;\n\tmov.b64 d, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %4, p;\n\t}\n"
+        :: "r"(d_tmem), "r"(a_tmem), "r"(b_desc), "r"(b_high), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void dc_row_scale(const float (&x)[N][4], float (&up)[2], float (&unit)[2]) {
-    float a = 0.f, b = 0.f;
+__device__ __forceinline__ void dc_ld16(uint32_t (&r)[16], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+                   "=r"(r[14]), "=r"(r[15]) : "r"(at));
+}
+__device__ __forceinline__ void dc_st16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                    "r"(r[14]), "r"(r[15]) : "memory");
+}
+// A warp's wait on an mbarrier, with one answer for all its lanes. It polls without being put to sleep (a chunk's chain has seven such waits); one that gives up raises the flag, which every other wait looks at.
+__device__ __forceinline__ bool dc_wait(uint32_t mbar, uint32_t parity, uint32_t fail) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 i, f;\n\tmov.u32 i, %4;\n"
+        "POLL_%=:\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\t"
+        "ld.volatile.shared.u32 f, [%3];\n\tsub.u32 i, i, 1;\n\tsetp.eq.u32 q, i, 0;\n\t@q st.volatile.shared.u32 [%3], 1;\n\tsetp.ne.or.u32 q, f, 0, q;\n\t@!q bra POLL_%=;\n"
+        "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done) : "r"(mbar), "r"(parity), "r"(fail), "n"(DC_SPIN_LIMIT) : "memory");
+    return __all_sync(0xffffffffu, done);
+}
+__device__ __forceinline__ void dc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// what a warp has stored to tensor memory (and read from it) is done with
+__device__ __forceinline__ void dc_hand_over(uint32_t mbar) {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0u) tc_arrive(mbar);
+}
+// 32 values x f as digits, upper ones to the columns from hi on, lower ones from lo on
+__device__ __forceinline__ void dc_put32(const float *x, float f, uint32_t hi, uint32_t lo) {
+    uint32_t h[16], l[16];
 #pragma unroll
-    for (int i = 0; i < N; ++i) { a = fmaxf(a, fmaxf(fabsf(x[i][0]), fabsf(x[i][1]))); b = fmaxf(b, fmaxf(fabsf(x[i][2]), fabsf(x[i][3]))); }
-#pragma unroll
-    for (int w = 1; w < 4; w <<= 1) { a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, w)); b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, w)); }
-    dc_scale(a, up[0], unit[0]);
-    dc_scale(b, up[1], unit[1]);
+    for (int i = 0; i < 16; ++i) {
+        const float2 y = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(f, f));
+        dc_digits(y.x, y.y, h[i], l[i]);
+    }
+    dc_st16(hi, h);
+    dc_st16(lo, l);
 }
 
-template <class T, int DIG, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 1) k_delta_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots) {
+template <class T, int DIG>
+__global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots) {
     pdl_prologue();
-    constexpr uint32_t KEYS = dc_keys(DIG), STAGE = KEYS + DC_REC;
+    constexpr uint32_t KEYS = dc_keys(DIG), VROW = DC_S * sizeof(T);
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ __align__(8) uint64_t s_full[2];
-    __shared__ uint32_t s_seq;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c2 = (lane & 3u) * 2u;
-    const uint32_t h = blockIdx.x / (8u / WARPS), j0 = (blockIdx.x % (8u / WARPS)) * (WARPS * 16u) + warp * 16u, kh = h / (A.rank / A.groups);
+    __shared__ __align__(8) uint64_t s_bar[DB_COUNT];
+    __shared__ float s_ex[3][2][DC_S];
+    __shared__ uint32_t s_from[2][DC_S], s_seq, tmem_slot;
+    __shared__ volatile uint32_t fail;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t h = blockIdx.x, kh = h / (A.rank / A.groups);
     // long sequences first: the block's sequence is the blockIdx.y-th longest (of many, they are taken as they come)
     uint32_t b = blockIdx.y + A.first_seq;
     if (n_seqs > 1u && n_seqs <= 1024u) {
-        for (uint32_t i = tid; i < n_seqs; i += WARPS * 32u) {
+        for (uint32_t i = tid; i < n_seqs; i += DC_THREADS) {
             const int64_t mine = (int64_t)A.cu[i + 1u] - A.cu[i];
             uint32_t before = 0u;
             for (uint32_t j = 0; j < n_seqs; ++j) { const int64_t other = (int64_t)A.cu[j + 1u] - A.cu[j]; before += other > mine || (other == mine && j < i); }
@@ -369,256 +454,301 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_delta_chunk(DeltaArgs A, uint
     if (lo < 0 || hi < lo || (uint32_t)hi > A.n_tokens) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
     const int32_t state_slot = delta_slot(A.slots, A.n_slots, b, A.status);
     if (state_slot < 0 || lo == hi) return;
-    const uint32_t len = (uint32_t)(hi - lo), chunks = (len + DC_T - 1u) / DC_T;
+    const uint32_t chunks = ((uint32_t)(hi - lo) + DC_T - 1u) / DC_T;
     const uint64_t slot0 = (uint64_t)(lo / DC_T) + b;
-    const uint8_t *const keys = ws + (slot0 * A.groups + kh) * KEYS, *const recs = ws + slots * A.groups * KEYS + (slot0 * A.rank + h) * DC_REC;
+    uint8_t *const s_kq = sm, *const s_kt = sm + DIG * DC_KQ, *const s_tt = sm + KEYS, *const s_pp = s_tt + 2u * DC_SQ, *const s_meta = s_tt + 4u * DC_SQ;
+    T *const s_v = reinterpret_cast<T *>(s_meta + 2u * sizeof(DcMeta)), *const s_out = s_v + DC_T * DC_S;          // [token][row]
+    auto bar = [&](uint32_t i) { return dc_smem(&s_bar[i]); };
     if (tid == 0u) {
-        for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(dc_smem(&s_full[i])));
+        fail = 0u;
+        for (uint32_t i = 0; i < DB_COUNT; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar(i)), "r"(i >= DB_PAIR ? 2u : i >= DB_R ? DC_ROW_WARPS : 1u));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    auto fetch = [&](uint32_t c) {               // by thread 0
-        const uint32_t bar = dc_smem(&s_full[c & 1u]), dst = dc_smem(sm) + (c & 1u) * STAGE;
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(STAGE) : "memory");
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                     :: "r"(dst), "l"(keys + (uint64_t)c * A.groups * KEYS), "r"(KEYS), "r"(bar) : "memory");
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                     :: "r"(dst + KEYS), "l"(recs + (uint64_t)c * A.rank * DC_REC), "r"(DC_REC), "r"(bar) : "memory");
-    };
-    auto wait = [&](uint32_t c) {
-        uint32_t done = 0;
-        for (uint32_t i = 0; i < DC_SPIN_LIMIT && !done; ++i)
-            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-                         : "=r"(done) : "r"(dc_smem(&s_full[c & 1u])), "r"((c >> 1) & 1u) : "memory");
-        return done != 0u;
-    };
-    if (tid == 0u) fetch(0u);
-    float *const state = A.state + (((uint64_t)(uint32_t)state_slot * A.rank + h) * DC_S + j0 + g) * DC_S + c2;      // rows g and g + 8, columns 8 i + c2, + 1
-    float s[16][4];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float2 x = *reinterpret_cast<const float2 *>(state + i * 8), y = *reinterpret_cast<const float2 *>(state + 8 * DC_S + i * 8);
-        s[i][0] = x.x; s[i][1] = x.y; s[i][2] = y.x; s[i][3] = y.y;
+    if (warp == DC_CONTROL) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(dc_smem(&tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    bool nan0 = false, nan1 = false;             // rows g, g + 8 are no numbers any more
-    {
-        bool f0 = true, f1 = true;
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0), fail_at = dc_smem(const_cast<uint32_t *>(&fail));
+    auto wait = [&](uint32_t i, uint32_t parity) { return dc_wait(bar(i), parity & 1u, fail_at); };
+    auto expect = [&](uint32_t i, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar(i)), "r"(bytes) : "memory"); };
+    auto copy = [&](uint32_t i, const void *dst, const void *src, uint32_t bytes) {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" :: "r"(dc_smem(dst)), "l"(src), "r"(bytes), "r"(bar(i)) : "memory");
+    };
+
+    if (warp >= DC_CONTROL) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(DC_REGS_CONTROL));
+        if (warp == DC_CONTROL) {
+            const uint32_t leader = tc_elect();
+            const uint8_t *key = ws + (slot0 * A.groups + kh) * KEYS, *rec = ws + slots * A.groups * KEYS + (slot0 * A.rank + h) * DC_REC;      // the next chunk's, as each is asked for
+            const uint64_t key_step = (uint64_t)A.groups * KEYS, rec_step = (uint64_t)A.rank * DC_REC;
+            auto get_kq = [&](uint32_t c) { if (lane == 0u) { expect(DB_KQ, DIG * DC_KQ); copy(DB_KQ, s_kq, key + c * key_step, DIG * DC_KQ); } };
+            auto get_t = [&](uint32_t c) { if (lane == 0u) { expect(DB_T, 2u * DC_SQ); copy(DB_T, s_tt, rec + c * rec_step, 2u * DC_SQ); } };
+            auto get_pk = [&](uint32_t c) {
+                if (lane == 0u) { expect(DB_PK, 2u * DC_SQ + DIG * DC_KT); copy(DB_PK, s_pp, rec + c * rec_step + 2u * DC_SQ, 2u * DC_SQ); copy(DB_PK, s_kt, key + c * key_step + DIG * DC_KQ, DIG * DC_KT); }
+            };
+            auto get_meta = [&](uint32_t c) {
+                if (lane == 0u) { expect(DB_META0 + (c & 1u), sizeof(DcMeta)); copy(DB_META0 + (c & 1u), s_meta + (c & 1u) * sizeof(DcMeta), rec + c * rec_step + 4u * DC_SQ, sizeof(DcMeta)); }
+            };
+            get_kq(0u); get_meta(0u); get_t(0u); get_pk(0u);
+            const uint64_t desc = tc_smem_desc(0u, 2048u, 128u), desc_sq = tc_smem_desc(0u, 1024u, 128u);
+            const uint32_t high = (uint32_t)(desc >> 32), wide = (uint32_t)desc, slim = (uint32_t)desc_sq;       // the upper words are alike
+            const uint32_t b_kq = wide | (dc_smem(s_kq) >> 4), b_kt = wide | (dc_smem(s_kt) >> 4), b_t = slim | (dc_smem(s_tt) >> 4), b_p = slim | (dc_smem(s_pp) >> 4);
+            // 128 columns of results += A B^T over 64 of k, lower digits first. a_lo: columns from A's upper to its lower digits, b_lo: 16-byte units from B's
+            auto square = [&](uint32_t d, uint32_t a, uint32_t a_lo, uint32_t bd, uint32_t b_lo) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { f0 &= fabsf(s[i][0]) < INFINITY && fabsf(s[i][1]) < INFINITY; f1 &= fabsf(s[i][2]) < INFINITY && fabsf(s[i][3]) < INFINITY; }
-        const uint32_t m0 = __ballot_sync(0xffffffffu, !f0), m1 = __ballot_sync(0xffffffffu, !f1), quad = 0xfu << (lane & 28u);
-        nan0 = m0 & quad; nan1 = m1 & quad;
-    }
-    const T *const v = reinterpret_cast<const T *>(A.v) + (uint64_t)h * DC_S + j0 + g;
-    T *const out = reinterpret_cast<T *>(A.out) + (uint64_t)h * DC_S + j0 + g;
-    const uint32_t br = (lane & 7u) + (lane >> 4) * 8u, bc = (lane >> 3) & 1u;       // operand B from rows [n][k]: 16 rows, two pieces
-    const uint32_t tr = (lane & 7u) + ((lane >> 3) & 1u) * 8u, tc = lane >> 4;       // from rows [k][n]: 16 rows, two pieces
-    bool failed = false;
+                for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + a_lo + 8u * k, bd + k * 256u, high, tc_idesc(128u), k ? 1u : 0u);
+                if (DIG == 2)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + 8u * k, bd + b_lo + k * 256u, high, tc_idesc(128u), 1u);
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + 8u * k, bd + k * 256u, high, tc_idesc(128u), 1u);
+            };
+            // the same with a lower triangle of 64: a step of 16 of k meets the rows from its own on
+            auto triangle = [&](uint32_t d, uint32_t a, uint32_t bd) {
+#pragma unroll
+                for (uint32_t pass = 0; pass < 3u; ++pass)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k)
+                        dc_mma_ts(leader, tmem + d + 16u * k, tmem + a + (pass == 0u ? 32u : 0u) + 8u * k, bd + (pass == 1u ? DC_SQ >> 4 : 0u) + k * (128u + 16u), high, tc_idesc(64u - 16u * k), pass | k ? 1u : 0u);
+            };
+            uint32_t c = 0u;
 #pragma unroll 1
-    for (uint32_t c = 0; c < chunks; ++c) {
-        __syncthreads();                         // the other stage's chunk has been worked on
-        if (tid == 0u && c + 1u < chunks) fetch(c + 1u);
-        const uint32_t t0 = (uint32_t)lo + c * DC_T, n = min((uint32_t)DC_T, (uint32_t)hi - t0);
-        // the chunk's values: token 8 i + c2 (+ 1), rows g and g + 8
-        float r[8][4];
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i)
-#pragma unroll
-            for (uint32_t e = 0; e < 2u; ++e) {
-                const uint32_t t = i * 8u + c2 + e;
-                r[i][e] = r[i][e + 2] = 0.f;
-                if (t < n) { r[i][e] = to_f32(v[(uint64_t)(t0 + t) * A.v_stride]); r[i][e + 2] = to_f32(v[(uint64_t)(t0 + t) * A.v_stride + 8u]); }
+            for (; c < chunks; ++c) {
+                const bool more = c + 1u < chunks;
+                if (!wait(DB_KQ, c) || !wait(DB_S, c) || (c && !wait(DB_M3, c - 1u))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                square(DT_M1, DT_S, 64u, b_kq, DC_KQ >> 4);
+                square(DT_M1 + 128u, DT_S + 32u, 64u, b_kq + 4u * 256u, DC_KQ >> 4);
+                tc_commit_if(leader, bar(DB_M1));
+                if (c) get_pk(c);
+                if (!wait(DB_M1, c)) break;
+                if (more) get_kq(c + 1u);
+                if (!wait(DB_T, c) || !wait(DB_R, c)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                triangle(DT_M2, DT_R, b_t);
+                tc_commit_if(leader, bar(DB_M2));
+                if (more) get_meta(c + 1u);
+                if (!wait(DB_M2, c)) break;
+                if (more) get_t(c + 1u);
+                if (!wait(DB_PK, c) || !wait(DB_DK, c)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                square(DT_M4, DT_DK, 32u, b_kt, DC_KT >> 4);
+                tc_commit_if(leader, bar(DB_M4));
+                if (!wait(DB_D, c)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                triangle(DT_M3, DT_D, b_p);
+                tc_commit_if(leader, bar(DB_M3));
             }
-        uint8_t *const st = sm + (c & 1u) * STAGE;
-        const uint32_t k_at = dc_smem(st), q_at = k_at + DIG * DC_TILE, t_at = k_at + KEYS, p_at = t_at + 2u * DC_SQ;
-        const DcMeta &M = *reinterpret_cast<const DcMeta *>(st + KEYS + 4u * DC_SQ);
-        if (!wait(c)) { failed = true; break; }
-        // the first token from which a row is no number (64: none)
-        uint32_t from0 = nan0 ? 0u : M.nan_from, from1 = nan1 ? 0u : M.nan_from;
-        {
-            bool fine = true;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) fine &= fabsf(r[i][e]) < INFINITY;
-            if (!__all_sync(0xffffffffu, fine)) {
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i)
-#pragma unroll
-                    for (uint32_t e = 0; e < 4u; ++e)
-                        if (!(fabsf(r[i][e]) < INFINITY)) {
-                            uint32_t &from = e < 2u ? from0 : from1;
-                            from = min(from, i * 8u + c2 + (e & 1u));
-                            r[i][e] = 0.f;
-                        }
-#pragma unroll
-                for (int w = 1; w < 4; w <<= 1) { from0 = min(from0, __shfl_xor_sync(0xffffffffu, from0, w)); from1 = min(from1, __shfl_xor_sync(0xffffffffu, from1, w)); }
+            if (!fail) wait(DB_M3, chunks - 1u);
+            // where a wait was given up, copies that nobody waits for may still be writing into this block's shared memory: every stage is waited for in both its phases
+            if (fail && lane == 0u) for (uint32_t i = DB_KQ; i <= DB_META1; ++i) { mbar_wait(bar(i), 0u); mbar_wait(bar(i), 1u); }
+        } else if (warp == DC_LOADER) {          // a chunk's values: a row of 128 a copy
+            const T *const v = reinterpret_cast<const T *>(A.v) + (uint64_t)(uint32_t)lo * A.v_stride + (uint64_t)h * DC_S;
+#pragma unroll 1
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T);
+                if (c && !wait(DB_VFREE, c - 1u)) break;
+                if (lane == 0u) expect(DB_V, n * VROW);
+                __syncwarp();
+                for (uint32_t t = lane; t < n; t += 32u) copy(DB_V, s_v + t * DC_S, v + (uint64_t)(c * DC_T + t) * A.v_stride, VROW);
             }
-            if (nan0)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i][0] = s[i][1] = 0.f;
-            if (nan1)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i][2] = s[i][3] = 0.f;
+            if (fail && lane == 0u) { mbar_wait(bar(DB_V), 0u); mbar_wait(bar(DB_V), 1u); }
+        } else if (warp == DC_STORER) {
+            T *const out = reinterpret_cast<T *>(A.out) + ((uint64_t)(uint32_t)lo * A.rank + h) * DC_S;
+#pragma unroll 1
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T);
+                if (!wait(DB_OUT, c)) break;
+                for (uint32_t t = lane; t < n; t += 32u)
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" :: "l"(out + (uint64_t)(c * DC_T + t) * A.rank * DC_S), "r"(dc_smem(s_out + t * DC_S)), "r"(VROW) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+                if (lane == 0u) tc_arrive(bar(DB_OFREE));
+            }
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
-        float up[2], unit[2], ks[8][4], o[8][4];
-        dc_row_scale(s, up, unit);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ks[i][e] = o[i][e] = 0.f;
-#pragma unroll
-        for (uint32_t k = 0; k < 8u; ++k) {      // 16 columns of the state
-            uint32_t ah[4], al[4];
-            dc_operand(s[2 * k], s[2 * k + 1], up[0], up[1], ah, al);
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {  // 16 tokens
-                uint32_t x[4], y[4];
-                dc_ldsm(x, k_at + dc_tile_at(i * 16u + br, 2u * k + bc));
-                dc_ldsm(y, q_at + dc_tile_at(i * 16u + br, 2u * k + bc));
-                dc_mma(ks[2 * i], ah, x[0], x[1]); dc_mma(ks[2 * i + 1], ah, x[2], x[3]);
-                dc_mma(o[2 * i], ah, y[0], y[1]); dc_mma(o[2 * i + 1], ah, y[2], y[3]);
-                dc_mma(ks[2 * i], al, x[0], x[1]); dc_mma(ks[2 * i + 1], al, x[2], x[3]);
-                dc_mma(o[2 * i], al, y[0], y[1]); dc_mma(o[2 * i + 1], al, y[2], y[3]);
-                if (DIG == 2) {
-                    dc_ldsm(x, k_at + DC_TILE + dc_tile_at(i * 16u + br, 2u * k + bc));
-                    dc_ldsm(y, q_at + DC_TILE + dc_tile_at(i * 16u + br, 2u * k + bc));
-                    dc_mma(ks[2 * i], ah, x[0], x[1]); dc_mma(ks[2 * i + 1], ah, x[2], x[3]);
-                    dc_mma(o[2 * i], ah, y[0], y[1]); dc_mma(o[2 * i + 1], ah, y[2], y[3]);
-                }
-            }
-        }
-        {   // R, and the state's part of the outputs
-            const float fk0 = unit[0] * M.f_k, fk1 = unit[1] * M.f_k, fq0 = unit[0] * M.f_q, fq1 = unit[1] * M.f_q;
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i)
-#pragma unroll
-                for (uint32_t e = 0; e < 2u; ++e) {
-                    const float dec = M.dec[i * 8u + c2 + e];
-                    r[i][e] = fmaf(-dec, ks[i][e] * fk0, r[i][e]); r[i][e + 2] = fmaf(-dec, ks[i][e + 2] * fk1, r[i][e + 2]);
-                    o[i][e] *= dec * fq0; o[i][e + 2] *= dec * fq1;
-                }
-        }
-        float d[8][4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[i][e] = 0.f;
-        // x += (digits of y) * (the lower triangle at `at`)
-        auto triangle = [&](float (&x)[8][4], const float (&y)[8][4], uint32_t at) {
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                uint32_t ah[4], al[4];
-                dc_operand(y[2 * k], y[2 * k + 1], up[0], up[1], ah, al);
-#pragma unroll
-                for (uint32_t i = k; i < 4u; ++i) {
-                    uint32_t z[4];
-                    dc_ldsm(z, at + dc_sq_at(i * 16u + br, 2u * k + bc));
-                    dc_mma(x[2 * i], ah, z[0], z[1]); dc_mma(x[2 * i + 1], ah, z[2], z[3]);
-                    dc_mma(x[2 * i], al, z[0], z[1]); dc_mma(x[2 * i + 1], al, z[2], z[3]);
-                    dc_ldsm(z, at + DC_SQ + dc_sq_at(i * 16u + br, 2u * k + bc));
-                    dc_mma(x[2 * i], ah, z[0], z[1]); dc_mma(x[2 * i + 1], ah, z[2], z[3]);
-                }
-            }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(DC_REGS_ROWS));
+        const uint32_t w = warp & 3u, hf = warp >> 2, j = w * 32u + lane, mine = tmem + ((w * 32u) << 16);
+        bool ok = true;
+        uint32_t met = 0u;
+        auto both = [&](float x, uint32_t i) {   // the larger of the row's two; the two warps meet on an mbarrier, whose wait is bounded like the others
+            s_ex[i][hf][j] = x;
+            __syncwarp();
+            if (lane == 0u) tc_arrive(bar(DB_PAIR + w));
+            ok &= wait(DB_PAIR + w, met++);
+            return fmaxf(x, s_ex[i][hf ^ 1u][j]);
         };
-        dc_row_scale(r, up, unit);
-        triangle(d, r, t_at);
+        auto load32 = [&](float (&x)[32], uint32_t col) {
+            uint32_t y[2][16];
+            dc_ld16(y[0], mine + col);
+            dc_ld16(y[1], mine + col + 16u);
+            dc_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { d[i][0] *= unit[0] * M.f_t; d[i][1] *= unit[0] * M.f_t; d[i][2] *= unit[1] * M.f_t; d[i][3] *= unit[1] * M.f_t; }
-        dc_row_scale(d, up, unit);
+            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(y[i >> 4][i & 15]);
+        };
+        float *const state = A.state + (((uint64_t)(uint32_t)state_slot * A.rank + h) * DC_S + j) * DC_S + hf * 64u;
+        float s[64], most_s = 0.f, up, unit_s;
+        uint32_t nan = 0u;                       // the row is no number any more
+        auto put_s = [&](float bound) {
+            dc_scale(bound, up, unit_s);
+            dc_put32(s, up, mine + DT_S + hf * 32u, mine + DT_S + 64u + hf * 32u);
+            dc_put32(s + 32, up, mine + DT_S + hf * 32u + 16u, mine + DT_S + 64u + hf * 32u + 16u);
+            dc_hand_over(bar(DB_S));
+        };
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r[i][e] = 0.f;
-        triangle(r, d, p_at);
-        {
-            const float f0 = unit[0] * M.f_p, f1 = unit[1] * M.f_p;
-            const bool numbers = from0 >= (uint32_t)DC_T && from1 >= (uint32_t)DC_T && !(M.bad_q[0] | M.bad_q[1]);
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i)
-#pragma unroll
-                for (uint32_t e = 0; e < 2u; ++e) {
-                    const uint32_t t = i * 8u + c2 + e;
-                    float y0 = A.scale * fmaf(r[i][e], f0, o[i][e]), y1 = A.scale * fmaf(r[i][e + 2], f1, o[i][e + 2]);
-                    if (!numbers) {
-                        const bool bad = (M.bad_q[t >> 5] >> (t & 31u)) & 1u;
-                        if (bad || t >= from0) y0 = NAN;
-                        if (bad || t >= from1) y1 = NAN;
-                    }
-                    if (t < n) {
-                        T *const p = out + (uint64_t)(t0 + t) * A.rank * DC_S;
-                        p[0] = from_f32<T>(y0); p[8] = from_f32<T>(y1);
-                    }
-                }
+        for (int i = 0; i < 64; i += 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(state + i);
+            s[i] = x.x; s[i + 1] = x.y; s[i + 2] = x.z; s[i + 3] = x.w;
         }
-        // the state
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i)
+        for (int i = 0; i < 64; ++i) { nan |= !(fabsf(s[i]) < INFINITY); most_s = fmaxf(most_s, fabsf(s[i])); }
+        s_from[hf][j] = nan;
+        most_s = both(most_s, 0u);
+        nan |= s_from[hf ^ 1u][j];
+        if (nan) {
+            most_s = 0.f;
 #pragma unroll
-            for (uint32_t e = 0; e < 2u; ++e) { const float w = M.kdec[i * 8u + c2 + e]; d[i][e] *= w; d[i][e + 2] *= w; }
-        dc_row_scale(d, up, unit);
-        uint32_t dh[4][4], dl[4][4];
+            for (int i = 0; i < 64; ++i) s[i] = 0.f;
+        }
+        put_s(most_s);
+#pragma unroll 1
+        for (uint32_t c = 0; ok && c < chunks; ++c) {
+            const DcMeta &M = *reinterpret_cast<const DcMeta *>(s_meta + (c & 1u) * sizeof(DcMeta));
+            float r[32], o[32], x[32], unit, most_v = 0.f;
+            // the chunk's values, and what they say of R's scale and of the first token from which the row is no number (64: none)
+            if (!(ok = wait(DB_META0 + (c & 1u), c >> 1) && wait(DB_V, c))) break;
+            uint32_t from = nan ? 0u : M.nan_from;
+            {
+                const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T);
+                bool fine = true;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dc_operand(d[2 * k], d[2 * k + 1], up[0], up[1], dh[k], dl[k]);
-        const float f0 = unit[0] * M.f_k, f1 = unit[1] * M.f_k, last = M.last;
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {      // 32 columns
-            float x[4][4];
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[a][e] = 0.f;
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k)
-#pragma unroll
-                for (uint32_t a = 0; a < 2u; ++a) {
-                    uint32_t y[4];
-                    dc_ldsm_t(y, k_at + dc_tile_at(k * 16u + tr, i * 4u + a * 2u + tc));
-                    dc_mma(x[2 * a], dh[k], y[0], y[1]); dc_mma(x[2 * a + 1], dh[k], y[2], y[3]);
-                    dc_mma(x[2 * a], dl[k], y[0], y[1]); dc_mma(x[2 * a + 1], dl[k], y[2], y[3]);
-                    if (DIG == 2) {
-                        dc_ldsm_t(y, k_at + DC_TILE + dc_tile_at(k * 16u + tr, i * 4u + a * 2u + tc));
-                        dc_mma(x[2 * a], dh[k], y[0], y[1]); dc_mma(x[2 * a + 1], dh[k], y[2], y[3]);
-                    }
+                for (uint32_t i = 0; i < 32u; ++i) {
+                    r[i] = to_f32(s_v[(hf * 32u + i) * DC_S + j]);
+                    if (hf * 32u + i >= n) r[i] = 0.f;
+                    fine &= fabsf(r[i]) < INFINITY;
                 }
+                if (!fine)
 #pragma unroll
-            for (uint32_t a = 0; a < 4u; ++a) {
-                float (&y)[4] = s[4 * i + a];
-                y[0] = fmaf(x[a][0], f0, y[0] * last); y[1] = fmaf(x[a][1], f0, y[1] * last);
-                y[2] = fmaf(x[a][2], f1, y[2] * last); y[3] = fmaf(x[a][3], f1, y[3] * last);
+                    for (uint32_t i = 0; i < 32u; ++i) if (!(fabsf(r[i]) < INFINITY)) { from = min(from, hf * 32u + i); r[i] = 0.f; }
+#pragma unroll
+                for (uint32_t i = 0; i < 32u; ++i) most_v = fmaxf(most_v, fabsf(r[i]));
             }
-        }
-        nan0 = from0 < (uint32_t)DC_T; nan1 = from1 < (uint32_t)DC_T;
-    }
-    if (failed) {                                // a copy never came: the next one is waited for, nothing more is written
-        if (A.status && lane == 0u) A.status[ST_TIMEOUT] = 1u;
-        for (uint32_t c = 0; c < chunks; ++c) if (!wait(c)) break;
-        return;
-    }
+            __syncwarp();
+            if (lane == 0u) tc_arrive(bar(DB_VFREE));
+            s_from[hf][j] = from;
+            most_v = both(most_v, 1u);
+            if (!ok) break;
+            from = min(from, s_from[hf ^ 1u][j]);
+            const float most_k = 32768.f * M.f_k;        // no key is larger
+            dc_scale(fminf(most_v + M.most_dec * (128.f * most_s) * most_k, 3e38f), up, unit);
+            if (!(ok = wait(DB_M1, c))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            {
+                load32(o, DT_M1 + hf * 32u);
+                load32(x, DT_M1 + 128u + hf * 32u);
+                const float f = -unit_s * M.f_k;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        *reinterpret_cast<float2 *>(state + i * 8) = nan0 ? make_float2(NAN, NAN) : make_float2(s[i][0], s[i][1]);
-        *reinterpret_cast<float2 *>(state + 8 * DC_S + i * 8) = nan1 ? make_float2(NAN, NAN) : make_float2(s[i][2], s[i][3]);
+                for (uint32_t i = 0; i < 32u; ++i) r[i] = fmaf(M.dec[hf * 32u + i] * f, o[i] + x[i], r[i]);
+            }
+            dc_put32(r, up, mine + DT_R + hf * 16u, mine + DT_R + 32u + hf * 16u);
+            dc_hand_over(bar(DB_R));
+            {   // the state's part of the outputs
+                load32(o, DT_M1 + 64u + hf * 32u);
+                load32(x, DT_M1 + 192u + hf * 32u);
+                const float f = unit_s * M.f_q;
+#pragma unroll
+                for (uint32_t i = 0; i < 32u; ++i) o[i] = (M.dec[hf * 32u + i] * f) * (o[i] + x[i]);
+            }
+            if (!(ok = wait(DB_M2, c))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            load32(x, DT_M2 + hf * 32u);
+            float f4, most_d = 0.f, most_dk = 0.f;
+            {
+                const float f = unit * M.f_t;
+#pragma unroll
+                for (uint32_t i = 0; i < 32u; ++i) {
+                    x[i] *= f; r[i] = x[i] * M.kdec[hf * 32u + i];
+                    most_d = fmaxf(most_d, fabsf(x[i])); most_dk = fmaxf(most_dk, fabsf(r[i]));
+                }
+                s_ex[2][hf][j] = most_d;
+                most_dk = both(most_dk, 0u);
+                if (!ok) break;
+                most_d = fmaxf(most_d, s_ex[2][hf ^ 1u][j]);
+                dc_scale(most_dk, up, f4);
+                dc_put32(r, up, mine + DT_DK + hf * 16u, mine + DT_DK + 32u + hf * 16u);
+                dc_hand_over(bar(DB_DK));
+                dc_scale(most_d, up, unit);
+                dc_put32(x, up, mine + DT_D + hf * 16u, mine + DT_D + 32u + hf * 16u);
+                dc_hand_over(bar(DB_D));
+                unit *= M.f_p;                   // of M3's result
+                f4 *= M.f_k;                     // of M4's
+            }
+            const float last = M.last;
+            if (!(ok = wait(DB_M4, c))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 64; i += 32) {
+                load32(x, DT_M4 + hf * 64u + i);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) s[i + e] = fmaf(x[e], f4, s[i + e] * last);
+            }
+            nan = from < (uint32_t)DC_T;
+            if (c + 1u < chunks) {
+                put_s(fminf(last * most_s + 64.f * most_dk * most_k, 3e38f));
+                most_s = 0.f;                    // its own largest, for the bounds of the next chunk
+#pragma unroll
+                for (int i = 0; i < 64; ++i) most_s = fmaxf(most_s, fabsf(s[i]));
+            }
+            if (!(ok = wait(DB_M3, c) && (c == 0u || wait(DB_OFREE, c - 1u)))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            load32(x, DT_M3 + hf * 32u);
+            const uint32_t bad_q = M.bad_q[hf];
+            unit *= A.scale;
+#pragma unroll
+            for (uint32_t i = 0; i < 32u; ++i) x[i] = fmaf(x[i], unit, A.scale * o[i]);
+            if (bad_q || from < (uint32_t)DC_T)
+#pragma unroll
+                for (uint32_t i = 0; i < 32u; ++i) if (((bad_q >> i) & 1u) || hf * 32u + i >= from) x[i] = NAN;
+#pragma unroll
+            for (uint32_t i = 0; i < 32u; ++i) s_out[(hf * 32u + i) * DC_S + j] = from_f32<T>(x[i]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the bulk stores come behind these
+            __syncwarp();
+            if (lane == 0u) tc_arrive(bar(DB_OUT));
+            if (c + 1u < chunks) { most_s = both(most_s, 2u); if (!ok) break; }
+        }
+        if (ok)
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4 *>(state + i) = nan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (fail && tid == 0u && A.status) A.status[ST_TIMEOUT] = 1u;
+    if (warp == DC_CONTROL) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
 }
 
 uint64_t delta_chunk_workspace(uint32_t type, uint32_t groups, uint32_t rank, uint32_t n_tokens, uint32_t n_seqs) {
     return dc_slots(n_tokens, n_seqs) * ((uint64_t)groups * dc_keys(type == VT_F32 ? 2 : 1) + (uint64_t)rank * DC_REC);
 }
 
-template <class T, int DIG, int WARPS> static int launch_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, cudaStream_t s) {
-    constexpr size_t smem = 2u * (dc_keys(DIG) + DC_REC);
+template <class T, int DIG> static int launch_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, cudaStream_t s) {
     static std::atomic<uint64_t> set{0};
-    if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_chunk<T, DIG, WARPS>), smem, set)) return 0;
+    if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_chunk<T, DIG>), dc_smem_bytes(DIG, sizeof(T)), set)) return 0;
     for (uint32_t b = 0; b < n_seqs; b += 65535u) {
         A.first_seq = b;
-        RC_LAUNCH((k_delta_chunk<T, DIG, WARPS>), dim3(A.rank * (8u / WARPS), n_seqs - b < 65535u ? n_seqs - b : 65535u), WARPS * 32, smem, s, A, n_seqs, ws, slots);
+        RC_LAUNCH((k_delta_chunk<T, DIG>), dim3(A.rank, n_seqs - b < 65535u ? n_seqs - b : 65535u), DC_THREADS, dc_smem_bytes(DIG, sizeof(T)), s, A, n_seqs, ws, slots);
         RC_LAUNCHED();
     }
     return 1;
 }
 template <class T, int DIG> static int launch_chunks(const DeltaArgs &A, uint32_t n_seqs, uint8_t *ws, cudaStream_t s) {
     const uint64_t slots = dc_slots(A.n_tokens, n_seqs);
-    constexpr uint32_t region = 4u * DC_MAT > dc_keys(DIG) ? 4u * DC_MAT : dc_keys(DIG);
+    constexpr uint32_t region = 4u * DC_MAT > DIG * DC_KQ ? 4u * DC_MAT : DIG * DC_KQ;
     constexpr size_t smem = 2u * DC_MAT + region;
     static std::atomic<uint64_t> set{0};
     if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_prep<T, DIG>), smem, set)) return 0;
@@ -628,8 +758,7 @@ template <class T, int DIG> static int launch_chunks(const DeltaArgs &A, uint32_
     RC_LAUNCHED();
     prof_end(s);
     prof_begin("delta_chunk", s);
-    const uint64_t heads = (uint64_t)n_seqs * A.rank;
-    const int ok = heads * 4u <= sm_count() ? launch_chunk<T, DIG, 2>(A, n_seqs, ws, slots, s) : launch_chunk<T, DIG, 8>(A, n_seqs, ws, slots, s);
+    const int ok = launch_chunk<T, DIG>(A, n_seqs, ws, slots, s);
     prof_end(s);
     return ok;
 }
