@@ -68,14 +68,38 @@ __device__ __forceinline__ void dc_mma(float (&c)[4], const uint32_t (&a)[4], ui
 constexpr uint32_t DC_PITCH = 68u;               // floats of a row of the 64 x 64 matrices in shared memory
 constexpr uint32_t DC_MAT = DC_T * DC_PITCH * 4u;
 __device__ __forceinline__ void dc_half_sync(uint32_t half) { asm volatile("bar.sync %0, 128;" :: "r"(half + 1u) : "memory"); }
-// the largest over half a block; s: four floats of its own
-__device__ __forceinline__ float dc_half_max(float x, float *s, uint32_t half) {
-    for (int w = 16; w; w >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-    if ((threadIdx.x & 31u) == 0u) s[(threadIdx.x >> 5) & 3u] = x;
-    dc_half_sync(half);
-    x = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    dc_half_sync(half);
-    return x;
+// e^x for x <= 0 (and moderate x above): the error of the argument is |x| 2^-24, of a result e^x
+__device__ __forceinline__ float dc_exp(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896340736f)); return r; }
+// The digits of a 16 x 16 block in the accumulator layout (8 values a lane) as operand A, under the block's own power of two
+__device__ __forceinline__ float dc_block_operand(const float (&x)[2][4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    float most = 0.f, up, unit;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[i][e]));
+    dc_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))), up, unit);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        dc_digits(x[i][0] * up, x[i][1] * up, hi[2 * i], lo[2 * i]);
+        dc_digits(x[i][2] * up, x[i][3] * up, hi[2 * i + 1], lo[2 * i + 1]);
+    }
+    return unit;
+}
+// c += (hi + lo) * B, B[k][n] = m[n][k] a block of a matrix in shared memory, its digits under `up`
+__device__ __forceinline__ void dc_block_product(float (&c)[2][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], const float *m, float up) {
+    const uint32_t g = (threadIdx.x & 31u) >> 2, c2 = (threadIdx.x & 3u) * 2u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                // n: rows 8 i .. 8 i + 7 of the block
+        uint32_t bh[2], bl[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float2 x = *reinterpret_cast<const float2 *>(m + (i * 8 + g) * DC_PITCH + k * 8 + c2);
+            dc_digits(x.x * up, x.y * up, bh[k], bl[k]);
+        }
+        dc_mma(c[i], lo, bh[0], bh[1]);
+        dc_mma(c[i], hi, bl[0], bl[1]);
+        dc_mma(c[i], hi, bh[0], bh[1]);
+    }
 }
 
 template <class T, int DIG>
@@ -84,8 +108,10 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
     extern __shared__ __align__(128) uint8_t sm[];
     float *const s_kk = reinterpret_cast<float *>(sm), *const s_qk = s_kk + DC_T * DC_PITCH;
     uint8_t *const dig = sm + 2u * DC_MAT;       // the digits; later the halves' matrices A and T
-    __shared__ float s_red[2][8], s_max[2][4], s_beta[2][DC_T];
-    __shared__ double s_cum[2][DC_T];
+    __shared__ float s_red[2][8], s_beta[2][DC_T];
+    __shared__ float2 s_max[2][4];
+    __shared__ float s_d[2][4];
+    __shared__ float2 s_cum[2][DC_T];            // the sums of the gates, each as a float and what it lacks
     __shared__ uint32_t s_bad[2][2];             // tokens whose key or query is not finite
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, kh = blockIdx.y, width = A.rank / A.groups;
     const uint64_t slot = blockIdx.x;
@@ -106,23 +132,34 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
     // rows 8 warp .. 8 warp + 7 of K and Q: a lane has row lane % 8 and the 8-value pieces lane / 8 + 4 i
     const uint32_t t = warp * 8u + (lane & 7u);
     float kx[4][8], qx[4][8], mk = 0.f, mq = 0.f;
+    const uint32_t half = tid >> 7, ht = tid & 127u, hw = ht >> 5;       // from the decays on, half a block has a value head
+    float g_raw[2] = {0.f, 0.f}, b_raw[2] = {0.f, 0.f};      // the gates and betas of the half's first value head, tokens 2 lane and 2 lane + 1
+    {
+        constexpr int P = 8 * sizeof(T) / 16;    // loads of eight values
+        uint4 rk[4][P], rq[4][P];
+        const T *const k = reinterpret_cast<const T *>(A.k) + (uint64_t)(t0 + min(t, n - 1u)) * A.k_stride + kh * DC_S + (lane >> 3) * 8u;
+        const T *const q = reinterpret_cast<const T *>(A.q) + (uint64_t)(t0 + min(t, n - 1u)) * A.q_stride + kh * DC_S + (lane >> 3) * 8u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < P; ++e) { rk[i][e] = reinterpret_cast<const uint4 *>(k + i * 32)[e]; rq[i][e] = reinterpret_cast<const uint4 *>(q + i * 32)[e]; }
+        if (hw == 0u && half < width)
+#pragma unroll
+            for (uint32_t i = 0; i < 2u; ++i)
+                if (lane * 2u + i < n) {
+                    g_raw[i] = A.gate[(uint64_t)(t0 + lane * 2u + i) * A.rank + kh * width + half];
+                    b_raw[i] = A.beta[(uint64_t)(t0 + lane * 2u + i) * A.rank + kh * width + half];
+                }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T *const pk = reinterpret_cast<const T *>(rk[i]), *const pq = reinterpret_cast<const T *>(rq[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { kx[i][e] = t < n ? to_f32(pk[e]) : 0.f; qx[i][e] = t < n ? to_f32(pq[e]) : 0.f; }
+        }
+    }
     if (tid < 4u) s_bad[tid >> 1][tid & 1u] = 0u;
     __syncthreads();
     bool fk = true, fq = true;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        constexpr int N = 16 / sizeof(T) < 8 ? 4 : 8;
-#pragma unroll
-        for (int e = 0; e < 8; e += N) {
-            const uint32_t col = kh * DC_S + (lane >> 3) * 8u + i * 32u + e;
-            if (t < n) {
-                load_vals<N>(reinterpret_cast<const T *>(A.k) + (uint64_t)(t0 + t) * A.k_stride + col, *reinterpret_cast<float (*)[N]>(&kx[i][e]));
-                load_vals<N>(reinterpret_cast<const T *>(A.q) + (uint64_t)(t0 + t) * A.q_stride + col, *reinterpret_cast<float (*)[N]>(&qx[i][e]));
-            } else
-#pragma unroll
-                for (int j = 0; j < N; ++j) kx[i][e + j] = qx[i][e + j] = 0.f;
-        }
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -175,6 +212,55 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
             for (uint32_t j = 0; j < 4u; ++j)
                 *reinterpret_cast<uint32_t *>(keys + DIG * DC_KQ + d * DC_KT + dc_kq_at((i * 4u + j) * 8u + (lane >> 2), warp) + (lane & 3u) * 4u) = x[j];
         }
+    // The decays of a value head, by one warp: tokens 2 lane and 2 lane + 1. The sums of the gates are kept as a float and what it lacks: differences of long sums are wanted to 2^-24 of themselves.
+    auto decays = [&](uint32_t v) {
+        const uint32_t h = kh * width + v;
+        DcMeta *const meta = reinterpret_cast<DcMeta *>(ws + slots * A.groups * dc_keys(DIG) + (slot * A.rank + h) * DC_REC + 4u * DC_SQ);
+        auto add = [](float2 x, float2 y) {      // (x.x + x.y) + (y.x + y.y)
+            const float s = x.x + y.x, z = s - x.x, e = ((x.x - (s - z)) + (y.x - z)) + (x.y + y.y), r = s + e;
+            return make_float2(r, e - (r - s));
+        };
+        float2 g[2];
+        float bt[2];
+        bool bad[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t t = lane * 2u + i;
+            float gv = g_raw[i], bv = b_raw[i];
+            if (v >= 2u) {
+                gv = bv = 0.f;
+                if (t < n) { gv = A.gate[(uint64_t)(t0 + t) * A.rank + h]; bv = A.beta[(uint64_t)(t0 + t) * A.rank + h]; }
+            }
+            bad[i] = !(gv < INFINITY) || !(fabsf(bv) < INFINITY) || ((s_bad[0][t >> 5] >> (t & 31u)) & 1u);
+            gv = gv < -200.f ? -200.f : gv;      // exp is 0 from -104 on; -infinity cuts the past off
+            g[i] = make_float2(bad[i] ? 0.f : gv, 0.f); bt[i] = bad[i] ? 0.f : bv;
+        }
+        g[1] = add(g[0], g[1]);
+        float2 sum = g[1];
+        for (int w = 1; w < 32; w <<= 1) {
+            const float2 x = make_float2(__shfl_up_sync(0xffffffffu, sum.x, w), __shfl_up_sync(0xffffffffu, sum.y, w));
+            if (lane >= (uint32_t)w) sum = add(x, sum);
+        }
+        const float2 last = make_float2(__shfl_sync(0xffffffffu, sum.x, 31), __shfl_sync(0xffffffffu, sum.y, 31));
+        float2 before = make_float2(__shfl_up_sync(0xffffffffu, sum.x, 1), __shfl_up_sync(0xffffffffu, sum.y, 1));
+        if (lane == 0u) before = make_float2(0.f, 0.f);
+        const float2 G[2] = {add(before, g[0]), sum};
+        const uint32_t m0 = __ballot_sync(0xffffffffu, bad[0]), m1 = __ballot_sync(0xffffffffu, bad[1]);
+        const uint32_t first0 = m0 ? 2u * ((uint32_t)__ffs((int)m0) - 1u) : (uint32_t)DC_T, first1 = m1 ? 2u * ((uint32_t)__ffs((int)m1) - 1u) + 1u : (uint32_t)DC_T;
+        float dec[2], kdec[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            dec[i] = expf(G[i].x + G[i].y); kdec[i] = expf((last.x - G[i].x) + (last.y - G[i].y));
+            s_cum[v & 1u][lane * 2u + i] = G[i]; s_beta[v & 1u][lane * 2u + i] = bt[i];
+        }
+        *reinterpret_cast<float2 *>(&meta->dec[lane * 2u]) = make_float2(dec[0], dec[1]);
+        *reinterpret_cast<float2 *>(&meta->kdec[lane * 2u]) = make_float2(kdec[0], kdec[1]);
+        const float most_dec = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(dec[0], dec[1]))));
+        if (lane == 0u) {
+            meta->last = expf(last.x + last.y); meta->f_k = f_k; meta->f_q = f_q; meta->most_dec = most_dec;
+            meta->nan_from = min(first0, first1); meta->bad_q[0] = s_bad[1][0]; meta->bad_q[1] = s_bad[1][1];
+        }
+    };
     {   // warps 0-3: K K^T, 4-7: Q K^T; 16 rows each, the columns up to the diagonal
         const uint32_t mt = warp & 3u, which = warp >> 2, a_at = dc_smem(dig), b_at = a_at;
         const uint32_t ar = which * DC_T + mt * 16u + (lane & 15u), ac = lane >> 4, br = (lane & 7u) + (lane >> 4) * 8u, bc = (lane >> 3) & 1u;
@@ -185,7 +271,7 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[i][j][e] = 0.f;
-#pragma unroll 2
+#pragma unroll 4
         for (uint32_t s = 0; s < 8u; ++s) {
             uint32_t ah[4], al[4];
             dc_ldsm(ah, a_at + dc_kq_at(ar, 2u * s + ac));
@@ -216,55 +302,26 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
                     *reinterpret_cast<float2 *>(p + 8u * DC_PITCH) = make_float2(c[i][j][2] * f * f_k, c[i][j][3] * f * f_k);
                 }
     }
+    if (hw == 0u && half < width) decays(half);      // the warps with the fewest products
     __syncthreads();
-    const uint32_t half = tid >> 7, ht = tid & 127u, hw = ht >> 5;
     float *const s_a = reinterpret_cast<float *>(dig + half * 2u * DC_MAT), *const s_t = s_a + DC_T * DC_PITCH;
-    float *const s_m = s_max[half];
+    float2 *const s_m = s_max[half];
     for (uint32_t v = half; v < width; v += 2u) {
         const uint32_t h = kh * width + v;
         uint8_t *const rec = ws + slots * A.groups * dc_keys(DIG) + (slot * A.rank + h) * DC_REC;
         DcMeta *const meta = reinterpret_cast<DcMeta *>(rec + 4u * DC_SQ);
-        if (hw == 0u) {                          // tokens 2 lane and 2 lane + 1
-            double g[2];
-            float bt[2];
-            bool bad[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t t = lane * 2u + i;
-                float gv = 0.f, bv = 0.f;
-                if (t < n) { gv = A.gate[(uint64_t)(t0 + t) * A.rank + h]; bv = A.beta[(uint64_t)(t0 + t) * A.rank + h]; }
-                gv = gv < -200.f ? -200.f : gv;  // exp is 0 from -104 on; -infinity cuts the past off
-                bad[i] = !(gv < INFINITY) || !(fabsf(bv) < INFINITY) || ((s_bad[0][t >> 5] >> (t & 31u)) & 1u);
-                g[i] = bad[i] ? 0.0 : (double)gv; bt[i] = bad[i] ? 0.f : bv;
-            }
-            g[1] += g[0];
-            double sum = g[1];
-            for (int w = 1; w < 32; w <<= 1) { const double x = __shfl_up_sync(0xffffffffu, sum, w); if (lane >= (uint32_t)w) sum += x; }
-            const double before = sum - g[1], last = __shfl_sync(0xffffffffu, sum, 31);
-            float most_dec = fmaxf(expf((float)(before + g[0])), expf((float)(before + g[1])));
-            for (int w = 16; w; w >>= 1) most_dec = fmaxf(most_dec, __shfl_xor_sync(0xffffffffu, most_dec, w));
-            const uint32_t m0 = __ballot_sync(0xffffffffu, bad[0]), m1 = __ballot_sync(0xffffffffu, bad[1]);
-            const uint32_t first0 = m0 ? 2u * ((uint32_t)__ffs((int)m0) - 1u) : (uint32_t)DC_T, first1 = m1 ? 2u * ((uint32_t)__ffs((int)m1) - 1u) + 1u : (uint32_t)DC_T;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t t = lane * 2u + i;
-                const double G = before + g[i];
-                s_cum[half][t] = G; s_beta[half][t] = bt[i];
-                meta->dec[t] = expf((float)G); meta->kdec[t] = expf((float)(last - G));
-            }
-            if (lane == 0u) {
-                meta->last = expf((float)last); meta->f_k = f_k; meta->f_q = f_q; meta->most_dec = most_dec;
-                meta->nan_from = min(first0, first1); meta->bad_q[0] = s_bad[1][0]; meta->bad_q[1] = s_bad[1][1];
-            }
-        }
+        if (v >= 2u && hw == 0u) decays(v);      // of the first two: ahead of the barrier above
         dc_half_sync(half);
         // A below the diagonal; P and its digits: pieces of eight columns, four a thread, whose tokens run along the lanes
-        float p[4][8], most = 0.f;
+        float p[4][8], most = 0.f, most_a = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t t = ht & 63u, s0 = (2u * i + (ht >> 6)) * 8u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[i][j] = 0.f;
+            if (s0 > (t | 31u)) continue;        // the whole warp's tokens lie before the piece
             const float bt = s_beta[half][t];
-            const double Gt = s_cum[half][t];
+            const float2 Gt = s_cum[half][t];
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {
                 const float4 qk = *reinterpret_cast<const float4 *>(s_qk + t * DC_PITCH + s0 + j), kk = *reinterpret_cast<const float4 *>(s_kk + t * DC_PITCH + s0 + j);
@@ -273,17 +330,23 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t s = s0 + j + e;
-                    const float ratio = s < t ? expf((float)(Gt - s_cum[half][s])) : 1.f;
+                    const float2 Gs = s_cum[half][s];
+                    const float ratio = dc_exp((Gt.x - Gs.x) + (Gt.y - Gs.y));
                     p[i][j + e] = s <= t ? qv[e] * ratio : 0.f;
-                    a[e] = s <= t ? bt * kv[e] * ratio : 0.f;
-                    most = fmaxf(most, fabsf(p[i][j + e]));
+                    a[e] = s < t ? bt * kv[e] * ratio : 0.f;
+                    most = fmaxf(most, fabsf(p[i][j + e])); most_a = fmaxf(most_a, fabsf(a[e]));
                 }
                 *reinterpret_cast<float4 *>(s_a + t * DC_PITCH + s0 + j) = make_float4(a[0], a[1], a[2], a[3]);
             }
         }
-        most = dc_half_max(most, s_m, half);
-        float up, unit;
+        for (int w = 16; w; w >>= 1) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w)); most_a = fmaxf(most_a, __shfl_xor_sync(0xffffffffu, most_a, w)); }
+        if (lane == 0u) s_m[hw] = make_float2(most, most_a);
+        dc_half_sync(half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { most = fmaxf(most, s_m[i].x); most_a = fmaxf(most_a, s_m[i].y); }
+        float up, unit, up_a, unit_a;
         dc_scale(most, up, unit);
+        dc_scale(most_a, up_a, unit_a);
         if (ht == 0u) meta->f_p = unit;
         auto put = [&](const float (&x)[8], float f, uint32_t t, uint32_t piece, uint8_t *to) {
             uint4 h, l;
@@ -305,37 +368,70 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
                 for (int k = 0; k < r; ++k) e = fmaf(-s_a[(o + r) * DC_PITCH + o + k], x[k], e);
                 x[r] = e;
             }
+            float most_t = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most_t = fmaxf(most_t, fabsf(x[r]));
             if (lane < 16u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s_t[(o + r) * DC_PITCH + o + c] = x[r];
+            most_t = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_t)));
+            if (lane == 0u) s_d[half][hw] = most_t;
         }
         dc_half_sync(half);
-        // the others: 64 threads a block, a row and four columns each; first M = sum_k A_ik T_kj, kept where T_ij will be, then -T_ii M
-        const uint32_t br = (ht & 63u) >> 2, bc = (ht & 3u) * 4u;
-#pragma unroll 1
-        for (uint32_t d = 1; d < 4u; ++d)
-#pragma unroll 1
-            for (uint32_t first = 0; first < 4u - d; first += 2u) {
-                const uint32_t j = first + (ht >> 6), i = j + d;
-                const bool on = i < 4u;
-                float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
-                auto fma4 = [&](float a, const float *t) { const float4 y = *reinterpret_cast<const float4 *>(t); m.x = fmaf(a, y.x, m.x); m.y = fmaf(a, y.y, m.y); m.z = fmaf(a, y.z, m.z); m.w = fmaf(a, y.w, m.w); };
-                float *const at = s_t + (i * 16u + br) * DC_PITCH + j * 16u + bc;
-                if (on) {
-#pragma unroll 8
-                    for (uint32_t k = j * 16u; k < i * 16u; ++k) fma4(s_a[(i * 16u + br) * DC_PITCH + k], s_t + k * DC_PITCH + j * 16u + bc);
-                    *reinterpret_cast<float4 *>(at) = m;
-                }
-                dc_half_sync(half);
-                m = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (on) {
+        // The others, a column of blocks a warp: X_i = T_ij^T = -(sum_{k < i} X_k A_ik^T) T_ii^T. Transposed, an accumulator is the next product's operand A and rows of A and T_ii are operand B.
+        {
+            float up_t, unit_t;
+            float diag = 0.f;
 #pragma unroll
-                    for (uint32_t k = 0; k < 16u; ++k) fma4(-s_t[(i * 16u + br) * DC_PITCH + i * 16u + k], s_t + (i * 16u + k) * DC_PITCH + j * 16u + bc);
+            for (int i = 0; i < 4; ++i) diag = fmaxf(diag, s_d[half][i]);
+            dc_scale(diag, up_t, unit_t);
+            const uint32_t j = hw, g = lane >> 2, c2 = (lane & 3u) * 2u;
+            uint32_t xh[3][4], xl[3][4];
+            float f[3], x[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)          // X_j = T_jj^T
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = s_t[(j * 16u + i * 8u + c2 + (e & 1)) * DC_PITCH + j * 16u + g + (e >> 1) * 8u];
+#pragma unroll
+            for (uint32_t d = 0; d < 3u; ++d) {  // block row i = j + d + 1
+                const uint32_t i = j + d + 1u;
+                if (i >= 4u) break;
+                f[d] = dc_block_operand(x, xh[d], xl[d]);
+                float m[2][4];
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m[a][e] = 0.f;
+#pragma unroll
+                for (uint32_t k = 0; k <= d; ++k) {
+                    float y[2][4];
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[a][e] = 0.f;
+                    dc_block_product(y, xh[k], xl[k], s_a + i * 16u * DC_PITCH + (j + k) * 16u, up_a);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) m[a][e] = fmaf(y[a][e], f[k] * unit_a, m[a][e]);
                 }
-                dc_half_sync(half);
-                if (on) *reinterpret_cast<float4 *>(at) = m;
-                dc_half_sync(half);
+                uint32_t mh[4], ml[4];
+                const float fm = -dc_block_operand(m, mh, ml) * unit_t;
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[a][e] = 0.f;
+                dc_block_product(x, mh, ml, s_t + i * 16u * DC_PITCH + i * 16u, up_t);
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[a][e] *= fm;
+                        s_t[(i * 16u + a * 8u + c2 + (e & 1)) * DC_PITCH + j * 16u + g + (e >> 1) * 8u] = x[a][e];
+                    }
             }
+        }
+        dc_half_sync(half);
         most = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -352,7 +448,10 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
                 }
             }
         }
-        most = dc_half_max(most, s_m, half);
+        for (int w = 16; w; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+        if (lane == 0u) s_d[half][hw] = most;
+        dc_half_sync(half);
+        most = fmaxf(fmaxf(s_d[half][0], s_d[half][1]), fmaxf(s_d[half][2], s_d[half][3]));
         dc_scale(most, up, unit);
         if (ht == 0u) meta->f_t = unit;
 #pragma unroll
@@ -433,7 +532,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
     constexpr uint32_t KEYS = dc_keys(DIG), VROW = DC_S * sizeof(T);
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ __align__(8) uint64_t s_bar[DB_COUNT];
-    __shared__ float s_ex[3][2][DC_S];
+    __shared__ float s_ex[4][2][DC_S];
     __shared__ uint32_t s_from[2][DC_S], s_seq, tmem_slot;
     __shared__ volatile uint32_t fail;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -626,24 +725,29 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             uint32_t from = nan ? 0u : M.nan_from;
             {
                 const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T);
-                bool fine = true;
 #pragma unroll
-                for (uint32_t i = 0; i < 32u; ++i) {
-                    r[i] = to_f32(s_v[(hf * 32u + i) * DC_S + j]);
-                    if (hf * 32u + i >= n) r[i] = 0.f;
-                    fine &= fabsf(r[i]) < INFINITY;
+                for (uint32_t i = 0; i < 32u; ++i) r[i] = to_f32(s_v[(hf * 32u + i) * DC_S + j]);
+                __syncwarp();
+                if (lane == 0u) tc_arrive(bar(DB_VFREE));
+                if (n < (uint32_t)DC_T)
+#pragma unroll
+                    for (uint32_t i = 0; i < 32u; ++i) if (hf * 32u + i >= n) r[i] = 0.f;
+#pragma unroll
+                for (uint32_t i = 0; i < 32u; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most_v) : "f"(fabsf(r[i])));
+                if (!(most_v < INFINITY)) {
+                    most_v = 0.f;
+#pragma unroll
+                    for (uint32_t i = 0; i < 32u; ++i) {
+                        if (!(fabsf(r[i]) < INFINITY)) { from = min(from, hf * 32u + i); r[i] = 0.f; }
+                        most_v = fmaxf(most_v, fabsf(r[i]));
+                    }
                 }
-                if (!fine)
-#pragma unroll
-                    for (uint32_t i = 0; i < 32u; ++i) if (!(fabsf(r[i]) < INFINITY)) { from = min(from, hf * 32u + i); r[i] = 0.f; }
-#pragma unroll
-                for (uint32_t i = 0; i < 32u; ++i) most_v = fmaxf(most_v, fabsf(r[i]));
             }
-            __syncwarp();
-            if (lane == 0u) tc_arrive(bar(DB_VFREE));
             s_from[hf][j] = from;
+            s_ex[2][hf][j] = most_s;
             most_v = both(most_v, 1u);
             if (!ok) break;
+            most_s = fmaxf(most_s, s_ex[2][hf ^ 1u][j]);
             from = min(from, s_from[hf ^ 1u][j]);
             const float most_k = 32768.f * M.f_k;        // no key is larger
             dc_scale(fminf(most_v + M.most_dec * (128.f * most_s) * most_k, 3e38f), up, unit);
@@ -676,10 +780,10 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
                     x[i] *= f; r[i] = x[i] * M.kdec[hf * 32u + i];
                     most_d = fmaxf(most_d, fabsf(x[i])); most_dk = fmaxf(most_dk, fabsf(r[i]));
                 }
-                s_ex[2][hf][j] = most_d;
+                s_ex[3][hf][j] = most_d;
                 most_dk = both(most_dk, 0u);
                 if (!ok) break;
-                most_d = fmaxf(most_d, s_ex[2][hf ^ 1u][j]);
+                most_d = fmaxf(most_d, s_ex[3][hf ^ 1u][j]);
                 dc_scale(most_dk, up, f4);
                 dc_put32(r, up, mine + DT_DK + hf * 16u, mine + DT_DK + 32u + hf * 16u);
                 dc_hand_over(bar(DB_DK));
@@ -720,7 +824,6 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the bulk stores come behind these
             __syncwarp();
             if (lane == 0u) tc_arrive(bar(DB_OUT));
-            if (c + 1u < chunks) { most_s = both(most_s, 2u); if (!ok) break; }
         }
         if (ok)
 #pragma unroll
