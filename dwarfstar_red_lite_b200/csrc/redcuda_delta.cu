@@ -132,8 +132,9 @@ template <bool STEP> static int launch_scan_t(const DeltaArgs &A, uint32_t type,
     return type == VT_F32 ? launch_scan_s<float, STEP>(A, S, n_seqs, s) : type == VT_F16 ? launch_scan_s<__half, STEP>(A, S, n_seqs, s) : launch_scan_s<__nv_bfloat16, STEP>(A, S, n_seqs, s);
 }
 
-// In chunks on the tensor cores, or a token at a time
-static bool delta_in_chunks(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs) { return d->d_state == 128u && n_tokens >= 16u * (uint64_t)n_seqs; }
+// In chunks on the tensor cores, or a token at a time: a chunk costs the same whatever it holds, and the first one of a call 20 us. us with 32 heads, a token at a time -> in chunks, F32 (BF16):
+// 1 sequence of 32 tokens 12 -> 27 (16 -> 23), of 64 21 -> 30 (30 -> 24), of 128 40 -> 33 (58 -> 28); 16 of 16 43 -> 76 (49 -> 67), of 32 79 -> 79 (92 -> 68), of 64 161 -> 86 (177 -> 71); 64 of 32 316 -> 304 (371 -> 264).
+static bool delta_in_chunks(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs) { return d->d_state == 128u && n_tokens >= 32u * (uint64_t)n_seqs + 32u; }
 
 // What a call's arguments have to be; fills the strides. rows: tokens of q, k, v and out
 static int delta_check(const redcuda_delta_dims *d, const char *who, uint32_t rows, uint32_t n_seqs, uint32_t n_slots, DeltaArgs &A) {

@@ -465,19 +465,21 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
 // with an operand A that the threads write to tensor memory as digits (each row under a scale of its own) and an operand B that bulk copies bring to shared memory:
 //     M1  [S k | S q] = S [K | Q]^T      M2  D = R T^T      M4  D' K (the state's)      M3  D P^T (the outputs')
 // between them the threads make R of M1's result, D and D' = D exp(G_last - G) of M2's, the new S of M4's, the outputs of M1's and M3's. Of four further warps one issues the products and fetches their
-// operands (a tile again as soon as the product that reads it is done), one fetches the values, one stores the outputs. What bounds it is the chain M1, R, M2, D', M4, S: each link waits for the one before, so what is
+// operands (a tile again as soon as the product that reads it is done), one fetches the values, two store the outputs. What bounds it is the chain M1, R, M2, D', M4, S: each link waits for the one before, so what is
 // not a link (the outputs, the digits of D, the largest of S) comes behind the hand-over of one. The scales of R and S come from bounds, which need no exchange between a row's two threads: up to 2^13
 // too large costs nothing, as two fp16 digits reach from 2^16 down to 2^-24.
 // The adder of the tensor cores truncates, so lower digits go first and M1's sums are kept in two halves of 64 columns each, which are added in fp32.
-constexpr uint32_t DC_THREADS = 384u, DC_ROW_WARPS = 8u, DC_CONTROL = 8u, DC_LOADER = 9u, DC_STORER = 10u;
+constexpr uint32_t DC_THREADS = 384u, DC_ROW_WARPS = 8u, DC_CONTROL = 8u, DC_LOADER = 9u, DC_STORER = 10u;        // 10 and 11 store
 // registers: 384 threads are launched with 168 each, of which the four further warps keep 72 and the threads of the rows have 216 (256 x 216 + 128 x 72 = 384 x 168)
 constexpr uint32_t DC_REGS_ROWS = 216u, DC_REGS_CONTROL = 72u;
 static_assert(256u * DC_REGS_ROWS + 128u * DC_REGS_CONTROL <= 384u * 168u, "a split above the launch's registers waits forever");
 constexpr uint32_t DC_SPIN_LIMIT = 1u << 26;     // polls of some twenty cycles: more than half a second, far beyond any real wait
 enum : uint32_t { DT_S = 0, DT_M1 = 128, DT_D = 128, DT_DK = 192, DT_M4 = 256, DT_R = 384, DT_M3 = 384, DT_M2 = 448 };      // columns of tensor memory; M1: two accumulators of 128
-enum : uint32_t { DB_KQ, DB_T, DB_PK, DB_META0, DB_META1, DB_V, DB_M1, DB_M2, DB_M3, DB_M4, DB_OFREE, DB_R, DB_DK, DB_D, DB_S, DB_VFREE, DB_OUT, DB_PAIR, DB_COUNT = DB_PAIR + 4 };
+enum : uint32_t { DB_KQ, DB_T, DB_PK, DB_META0, DB_META1, DB_V, DB_M1, DB_M2, DB_M3, DB_M4, DB_OFREE, DB_R, DB_DK, DB_D, DB_S, DB_VFREE, DB_OUT, DB_END, DB_PAIR, DB_COUNT = DB_PAIR + 4 };
+constexpr uint32_t DC_SROW = DC_S * 4u + 16u;    // a row of the state on its way through shared memory, 16 bytes further apart than it is long: a quarter warp's rows lie in different banks
 constexpr uint32_t dc_smem_bytes(int dig, uint32_t size) { return dc_keys(dig) + 4u * DC_SQ + 2u * (uint32_t)sizeof(DcMeta) + 2u * DC_T * DC_S * size; }
 static_assert(dc_smem_bytes(1, 2u) >= 114u * 1024u && dc_smem_bytes(2, 4u) < 220u * 1024u, "one block an SM: it takes all of the tensor memory");
+static_assert(dc_smem_bytes(1, 2u) - DC_KQ >= DC_S * DC_SROW && dc_keys(1) + 4u * DC_SQ >= DC_S * DC_SROW, "the state comes in behind KQ and leaves over the operands");
 
 __device__ __forceinline__ void dc_mma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_desc, uint32_t b_high, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
     auto bar = [&](uint32_t i) { return dc_smem(&s_bar[i]); };
     if (tid == 0u) {
         fail = 0u;
-        for (uint32_t i = 0; i < DB_COUNT; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar(i)), "r"(i >= DB_PAIR ? 2u : i >= DB_R ? DC_ROW_WARPS : 1u));
+        for (uint32_t i = 0; i < DB_COUNT; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar(i)), "r"(i >= DB_PAIR || i == DB_OFREE ? 2u : i >= DB_R ? DC_ROW_WARPS : i == DB_V ? 32u : 1u));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -592,7 +594,8 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             auto get_meta = [&](uint32_t c) {
                 if (lane == 0u) { expect(DB_META0 + (c & 1u), sizeof(DcMeta)); copy(DB_META0 + (c & 1u), s_meta + (c & 1u) * sizeof(DcMeta), rec + c * rec_step + 4u * DC_SQ, sizeof(DcMeta)); }
             };
-            get_kq(0u); get_meta(0u); get_t(0u); get_pk(0u);
+            get_kq(0u);
+            if (wait(DB_S, 0u)) { get_meta(0u); get_t(0u); get_pk(0u); }         // over the state, which has been read
             const uint64_t desc = tc_smem_desc(0u, 2048u, 128u), desc_sq = tc_smem_desc(0u, 1024u, 128u);
             const uint32_t high = (uint32_t)(desc >> 32), wide = (uint32_t)desc, slim = (uint32_t)desc_sq;       // the upper words are alike
             const uint32_t b_kq = wide | (dc_smem(s_kq) >> 4), b_kt = wide | (dc_smem(s_kt) >> 4), b_t = slim | (dc_smem(s_tt) >> 4), b_p = slim | (dc_smem(s_pp) >> 4);
@@ -645,31 +648,33 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             if (!fail) wait(DB_M3, chunks - 1u);
             // where a wait was given up, copies that nobody waits for may still be writing into this block's shared memory: every stage is waited for in both its phases
             if (fail && lane == 0u) for (uint32_t i = DB_KQ; i <= DB_META1; ++i) { mbar_wait(bar(i), 0u); mbar_wait(bar(i), 1u); }
-        } else if (warp == DC_LOADER) {          // a chunk's values: a row of 128 a copy
+        } else if (warp == DC_LOADER) {          // a chunk's values, 16 bytes a lane and copy (bulk copies of a row each take some hundred cycles apiece)
+            constexpr uint32_t PIECES = VROW / 16u;
             const T *const v = reinterpret_cast<const T *>(A.v) + (uint64_t)(uint32_t)lo * A.v_stride + (uint64_t)h * DC_S;
 #pragma unroll 1
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T);
-                if (c && !wait(DB_VFREE, c - 1u)) break;
-                if (lane == 0u) expect(DB_V, n * VROW);
-                __syncwarp();
-                for (uint32_t t = lane; t < n; t += 32u) copy(DB_V, s_v + t * DC_S, v + (uint64_t)(c * DC_T + t) * A.v_stride, VROW);
+                const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T) * PIECES;
+                if (c ? !wait(DB_VFREE, c - 1u) : !wait(DB_S, 0u)) break;      // ahead of the first chunk the state is there
+#pragma unroll 4
+                for (uint32_t i = lane; i < n; i += 32u)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dc_smem(s_v) + i * 16u), "l"(v + (uint64_t)(c * DC_T + i / PIECES) * A.v_stride + i % PIECES * (16u / sizeof(T))) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar(DB_V)) : "memory");
             }
-            if (fail && lane == 0u) { mbar_wait(bar(DB_V), 0u); mbar_wait(bar(DB_V), 1u); }
-        } else if (warp == DC_STORER) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {                                 // the outputs, every other row a warp
+            constexpr uint32_t PIECES = VROW / 16u;
+            const uint32_t first = (warp - DC_STORER) * 32u + lane;
             T *const out = reinterpret_cast<T *>(A.out) + ((uint64_t)(uint32_t)lo * A.rank + h) * DC_S;
 #pragma unroll 1
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T);
+                const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T) * PIECES;
                 if (!wait(DB_OUT, c)) break;
-                for (uint32_t t = lane; t < n; t += 32u)
-                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" :: "l"(out + (uint64_t)(c * DC_T + t) * A.rank * DC_S), "r"(dc_smem(s_out + t * DC_S)), "r"(VROW) : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+#pragma unroll 4
+                for (uint32_t i = first; i < n; i += 64u)
+                    *reinterpret_cast<uint4 *>(out + (uint64_t)(c * DC_T + i / PIECES) * A.rank * DC_S + i % PIECES * (16u / sizeof(T))) = *reinterpret_cast<const uint4 *>(s_out + i * (16u / sizeof(T)));
                 __syncwarp();
                 if (lane == 0u) tc_arrive(bar(DB_OFREE));
             }
-            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(DC_REGS_ROWS));
@@ -691,7 +696,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
 #pragma unroll
             for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(y[i >> 4][i & 15]);
         };
-        float *const state = A.state + (((uint64_t)(uint32_t)state_slot * A.rank + h) * DC_S + j) * DC_S + hf * 64u;
+        float *const state = A.state + ((uint64_t)(uint32_t)state_slot * A.rank + h) * DC_S * DC_S;
         float s[64], most_s = 0.f, up, unit_s;
         uint32_t nan = 0u;                       // the row is no number any more
         auto put_s = [&](float bound) {
@@ -700,11 +705,14 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             dc_put32(s + 32, up, mine + DT_S + hf * 32u + 16u, mine + DT_S + 64u + hf * 32u + 16u);
             dc_hand_over(bar(DB_S));
         };
+        // a warp reads a row at a time and has it from shared memory a row a lane
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(state + i);
-            s[i] = x.x; s[i + 1] = x.y; s[i + 2] = x.z; s[i + 3] = x.w;
-        }
+        for (int i = 0; i < 16; ++i) *reinterpret_cast<float4 *>(&s[4 * i]) = *reinterpret_cast<const float4 *>(state + (i * 8u + warp) * DC_S + lane * 4u);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) *reinterpret_cast<float4 *>(s_kt + (i * 8u + warp) * DC_SROW + lane * 16u) = *reinterpret_cast<const float4 *>(&s[4 * i]);
+        asm volatile("bar.sync 1, 256;" ::: "memory");         // all eight warps of the rows come here
+#pragma unroll
+        for (int i = 0; i < 16; ++i) *reinterpret_cast<float4 *>(&s[4 * i]) = *reinterpret_cast<const float4 *>(s_kt + j * DC_SROW + hf * 256u + i * 16u);
 #pragma unroll
         for (int i = 0; i < 64; ++i) { nan |= !(fabsf(s[i]) < INFINITY); most_s = fmaxf(most_s, fabsf(s[i])); }
         s_from[hf][j] = nan;
@@ -715,6 +723,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
 #pragma unroll
             for (int i = 0; i < 64; ++i) s[i] = 0.f;
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // copies into where the state was come behind its reading
         put_s(most_s);
 #pragma unroll 1
         for (uint32_t c = 0; ok && c < chunks; ++c) {
@@ -821,13 +830,19 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
                 for (uint32_t i = 0; i < 32u; ++i) if (((bad_q >> i) & 1u) || hf * 32u + i >= from) x[i] = NAN;
 #pragma unroll
             for (uint32_t i = 0; i < 32u; ++i) s_out[(hf * 32u + i) * DC_S + j] = from_f32<T>(x[i]);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the bulk stores come behind these
             __syncwarp();
             if (lane == 0u) tc_arrive(bar(DB_OUT));
         }
-        if (ok)
+        if (ok) {                                // every product has been waited for: the operands' shared memory is free
 #pragma unroll
-            for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4 *>(state + i) = nan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+            for (int i = 0; i < 16; ++i)
+                *reinterpret_cast<float4 *>(sm + j * DC_SROW + hf * 256u + i * 16u) = nan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+            __syncwarp();
+            if (lane == 0u) tc_arrive(bar(DB_END));
+            if (wait(DB_END, 0u))
+#pragma unroll
+                for (int i = 0; i < 16; ++i) *reinterpret_cast<float4 *>(state + (i * 8u + warp) * DC_S + lane * 4u) = *reinterpret_cast<const float4 *>(sm + (i * 8u + warp) * DC_SROW + lane * 16u);
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
