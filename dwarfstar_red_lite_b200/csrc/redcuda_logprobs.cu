@@ -9,13 +9,14 @@
 
 #include <cooperative_groups.h>
 #include <math.h>
+#include <type_traits>
 
 namespace rc {
 
 namespace cg = cooperative_groups;
 
 constexpr int LP_WARPS = 8, LP_CLUSTER = 8, LP_UNROLL = 4;
-static_assert(REDCUDA_MAX_ALTERNATIVES <= 32u && LP_WARPS == 8, "a list is one key a lane; eight floors are read at once");
+static_assert(REDCUDA_MAX_ALTERNATIVES <= 32u && LP_WARPS == 8 && LP_CLUSTER == LP_WARPS, "a list is one key a lane; eight floors are read at once; a warp for every list");
 
 struct LogprobArgs {
     const void *x;
@@ -79,19 +80,46 @@ __device__ __forceinline__ uint64_t lp_merge(uint64_t a, uint64_t b) {       // 
     return key;
 }
 
-// What bounds it is the row's bytes, if a value takes no more than the eight instructions it has here (of which one is an exponential, a
+// Sixteen bytes of logits as floats, and the largest of them (a NaN counts as none)
+__device__ __forceinline__ void lp_unpack(uint4 w, float (&v)[4]) { v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w); }
+template <class T> __device__ __forceinline__ void lp_unpack(uint4 w, float (&v)[8]) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        } else {
+            v[2 * i] = __uint_as_float(x[i] << 16); v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+        }
+    }
+}
+template <class T> __device__ __forceinline__ float lp_most(uint4 w) {
+    if constexpr (sizeof(T) == 4) {
+        return fmaxf(fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w))), -INFINITY);
+    } else {
+        using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        auto pair = [](const uint32_t &x) { return *reinterpret_cast<const P *>(&x); };
+        const P m = __hmax2(__hmax2(pair(w.x), pair(w.y)), __hmax2(pair(w.z), pair(w.w)));
+        return fmaxf(fmaxf(to_f32(m.x), to_f32(m.y)), -INFINITY);
+    }
+}
+
+// What bounds it is the row's bytes, if a value takes no more than the seven instructions it has here (of which one is an exponential, a
 // sixteenth of the fp32 rate). The alternatives therefore cost one comparison a lane and round of LP_UNROLL pieces: a warp keeps its 32 largest keys, one a
 // lane, and looks at single values only where the largest of a lane's round reaches what is known to be among the row's n largest. That is the n-th of the warp's own,
-// or the least of the warps' ceil(n / LP_WARPS)-th largest, which every warp publishes (n values are at least that large; a stale one is a lower bound too).
+// or the least of the warps' ceil(n / LP_WARPS)-th largest, which every warp publishes (n values are at least that large; a stale one is a lower bound too), or in a warp's first
+// round the n-th of its lanes' largest.
 template <class T>
 __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs A) {
     pdl_prologue();
-    constexpr int VEC = 16 / sizeof(T), U = LP_UNROLL, NV = U * VEC;
+    constexpr int VEC = 16 / sizeof(T), U = LP_UNROLL;
     constexpr float LOG2E = 1.44269504088896340736f;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank(), row = blockIdx.x / parts;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, n = A.top_n;
     __shared__ uint64_t s_keys[LP_WARPS][32], s_best[LP_CLUSTER][32];
+    __shared__ uint16_t s_cand[LP_WARPS][32 * U * VEC];
     __shared__ LpSums s_sums[LP_WARPS], s_parts[LP_CLUSTER];
     __shared__ __align__(16) float s_floor[LP_WARPS];
     const T *x = reinterpret_cast<const T *>(A.x) + (uint64_t)row * A.row_stride;
@@ -104,7 +132,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
     float m = -INFINITY;                         // a lane's sums are kept in two halves each
     float2 s2 = make_float2(0.f, 0.f), u2 = make_float2(0.f, 0.f);
     uint64_t best = 0ull, least = 0ull;          // lane i: the i-th largest key; the n-th
-    float bar = n ? -INFINITY : INFINITY;        // values below it are not among the row's n largest
+    float bar = -INFINITY;                       // values below it are not among the row's n largest
     const uint32_t share = (n + LP_WARPS - 1u) / LP_WARPS;
     auto listed = [&]() {                        // the list has changed
         least = __shfl_sync(0xffffffffu, best, (int)n - 1);
@@ -114,7 +142,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
     auto offer = [&](uint64_t key) {             // a key of each lane, 0: none
         uint32_t todo = __ballot_sync(0xffffffffu, key > least);
         if (!todo) return;
-        if (__popc(todo) > 4) {
+        if (__popc(todo) > 6) {
             best = lp_merge(best, lp_sort(key));
         } else {
             for (; todo; todo &= todo - 1u) {
@@ -130,49 +158,81 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
         s2.x *= f; s2.y *= f;
         m = to;
     };
+    bool fresh = true;
     for (uint32_t p = p0 + warp * (32u * U); p < p1; p += LP_WARPS * 32u * U) {
-        float v[NV];
+        const uint4 *const at = reinterpret_cast<const uint4 *>(x + head) + p + lane;
+        uint4 w[U];
+        if (p + 32u * U <= p1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (p + u * 32u + lane < p1) load_vals<VEC>(x + head + (uint64_t)(p + u * 32u + lane) * VEC, *reinterpret_cast<float (*)[VEC]>(&v[u * VEC]));
-            else
+            for (int u = 0; u < U; ++u) w[u] = at[u * 32];
+        } else {
+            const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;       // -infinity
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[u * VEC + i] = -INFINITY;
+            for (int u = 0; u < U; ++u) w[u] = p + u * 32u + lane < p1 ? at[u * 32] : make_uint4(low, low, low, low);
         }
-        float most = v[0];
+        float top[U], most = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < NV; ++i) most = fmaxf(most, v[i]);
+        for (int u = 0; u < U; ++u) { top[u] = lp_most<T>(w[u]); most = fmaxf(most, top[u]); }
         if (__any_sync(0xffffffffu, most > m)) rescale(fmaxf(m, most));
         const float base = m == -INFINITY ? 0.f : m;
         const float2 nb = make_float2(-base, -base), l2 = make_float2(LOG2E, LOG2E);
 #pragma unroll
-        for (int i = 0; i < NV; i += 2) {
-            float2 d = __fadd2_rn(make_float2(v[i], v[i + 1]), nb);
-            d = make_float2(max_nan(d.x, -150.f), max_nan(d.y, -150.f));       // of a probability that is 0, e d = 0; of a NaN, a NaN
-            float2 e = __fmul2_rn(d, l2);
-            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-            s2 = __fadd2_rn(s2, e);
-            u2 = __ffma2_rn(e, d, u2);
-        }
-        const float4 f0 = lp_floor(&s_floor[0]), f1 = lp_floor(&s_floor[4]);
-        if (n) bar = fmaxf(fmaxf(bar, fminf(fminf(fminf(f0.x, f0.y), fminf(f0.z, f0.w)), fminf(fminf(f1.x, f1.y), fminf(f1.z, f1.w)))), least ? lp_value(least) : -INFINITY);
-        if (__any_sync(0xffffffffu, most >= bar)) {
-            // a lane's largest first, which lifts the bar for its others
-            uint32_t todo = 0u, top = ~0u;
+        for (int u = 0; u < U; ++u) {
+            float v[VEC];
+            if constexpr (sizeof(T) == 4) lp_unpack(w[u], v); else lp_unpack<T>(w[u], v);
 #pragma unroll
-            for (int i = NV - 1; i >= 0; --i) if (v[i] == most && p + (i / VEC) * 32u + lane < p1) top = (uint32_t)i;
-            auto index = [&](uint32_t i) { return head + (p + (i / VEC) * 32u + lane) * VEC + i % VEC; };
-            offer(top != ~0u && most >= bar ? lp_key(most, index(top)) : 0ull);
-            const float now = fmaxf(bar, least ? lp_value(least) : -INFINITY);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) if (v[i] >= now && (uint32_t)i != top && p + (i / VEC) * 32u + lane < p1) todo |= 1u << i;
-            while (__any_sync(0xffffffffu, todo)) {
-                uint64_t key = 0ull;
-                if (todo) { const uint32_t i = (uint32_t)__ffs((int)todo) - 1u; key = lp_key(to_f32(x[index(i)]), index(i)); }
-                offer(key);
-                todo &= todo - 1u;
+            for (int i = 0; i < VEC; i += 2) {
+                float2 d = __fadd2_rn(make_float2(v[i], v[i + 1]), nb);
+                d = make_float2(max_nan(d.x, -150.f), max_nan(d.y, -150.f));       // of a probability that is 0, e d = 0; of a NaN, a NaN
+                float2 e = __fmul2_rn(d, l2);
+                e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                s2 = __fadd2_rn(s2, e);
+                u2 = __ffma2_rn(e, d, u2);
             }
         }
+        if (n == 0u) continue;
+        const float4 f0 = lp_floor(&s_floor[0]), f1 = lp_floor(&s_floor[4]);
+        // Other warps write the floors meanwhile, and a 16-byte read of a warp is not one access: its lanes may see different ones. One lane's is taken, as the warp branches on it.
+        bar = __shfl_sync(0xffffffffu, fmaxf(bar, fminf(fminf(fminf(f0.x, f0.y), fminf(f0.z, f0.w)), fminf(fminf(f1.x, f1.y), fminf(f1.z, f1.w)))), 0);
+        if (fresh) {                             // the n-th of the lanes' largest
+            fresh = false;
+            float y = most;
+#pragma unroll
+            for (uint32_t run = 2; run <= 32; run <<= 1)
+#pragma unroll
+                for (uint32_t k = run >> 1; k; k >>= 1) {
+                    const float o = __shfl_xor_sync(0xffffffffu, y, k);
+                    y = ((lane & k) == 0u) == ((lane & run) == 0u || run == 32u) ? fmaxf(y, o) : fminf(y, o);
+                }
+            bar = fmaxf(bar, __shfl_sync(0xffffffffu, y, (int)n - 1));
+        }
+        // what equals the n-th of earlier rounds has a larger index
+        if (!__any_sync(0xffffffffu, most >= bar && (least == 0ull || most > lp_value(least)))) continue;
+        // the places of the values that reach the bar, then the values themselves, 32 at a time
+        uint32_t count = 0u;
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (!__any_sync(0xffffffffu, top[u] >= bar)) continue;
+            float v[VEC];
+            if constexpr (sizeof(T) == 4) lp_unpack(w[u], v); else lp_unpack<T>(w[u], v);
+            const bool have = p + u * 32u + lane < p1;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const bool in = have && v[i] >= bar;
+                const uint32_t who = __ballot_sync(0xffffffffu, in);
+                if (in) s_cand[warp][count + __popc(who & ((1u << lane) - 1u))] = (uint16_t)((u * 32u + lane) * VEC + i);
+                count += __popc(who);
+            }
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (uint32_t k = lane; k - lane < count; k += 32u) {
+            uint64_t key = 0ull;
+            if (k < count) { const uint32_t i = head + p * VEC + s_cand[warp][k]; key = lp_key(to_f32(x[i]), i); }
+            offer(key);
+        }
+        if (least) bar = fmaxf(bar, lp_value(least));
     }
     if (part == 0u && warp == 0u) {              // the single values at both ends
         const uint32_t tail = head + pieces * VEC, ends = head + A.vocab - tail;
@@ -193,7 +253,16 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
     }
     if (lane == 0u) s_sums[warp] = S;
     s_keys[warp][lane] = best;
-    cluster.sync();                              // and the other blocks have begun: their shared memory may be written
+    // the lists of a block, and then of a cluster, two and two
+    auto gather = [&](uint64_t (&list)[LP_WARPS][32], uint32_t lists) {
+        for (uint32_t half = LP_WARPS / 2; half; half >>= 1) {
+            if (warp < half && warp + half < lists) { best = lp_merge(best, list[warp + half][lane]); list[warp][lane] = best; }
+            __syncthreads();
+        }
+    };
+    __syncthreads();
+    if (n) gather(s_keys, LP_WARPS);
+    if (parts > 1u) cluster.sync();              // the other blocks have begun: their shared memory may be written
     if (warp == 0u) {
         S = lane < LP_WARPS ? s_sums[lane] : LpSums{-INFINITY, 0.f, 0.f};
 #pragma unroll
@@ -201,15 +270,20 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
             const LpSums o{__shfl_xor_sync(0xffffffffu, S.m, w), __shfl_xor_sync(0xffffffffu, S.s, w), __shfl_xor_sync(0xffffffffu, S.u, w)};
             S = lp_join(S, o);
         }
-        if (n) {
-#pragma unroll
-            for (int w = 1; w < LP_WARPS; ++w) best = lp_merge(best, s_keys[w][lane]);
-            if (parts > 1u) cluster.map_shared_rank(s_best[part], 0)[lane] = best;
+        if (parts > 1u) {
+            if (n) cluster.map_shared_rank(s_best[part], 0)[lane] = best;
+            if (lane == 0u) *cluster.map_shared_rank(&s_parts[part], 0) = S;
         }
-        if (parts > 1u && lane == 0u) *cluster.map_shared_rank(&s_parts[part], 0) = S;
     }
-    if (parts > 1u) cluster.sync();
-    if (part != 0u || warp != 0u) return;
+    if (parts > 1u) {
+        cluster.sync();
+        if (part != 0u) return;
+        if (n) {
+            best = warp < parts ? s_best[warp][lane] : 0ull;
+            gather(s_best, parts);
+        }
+    }
+    if (warp != 0u) return;
     if (parts > 1u) {
         S = lane < parts ? s_parts[lane] : LpSums{-INFINITY, 0.f, 0.f};
 #pragma unroll
@@ -217,7 +291,6 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
             const LpSums o{__shfl_xor_sync(0xffffffffu, S.m, w), __shfl_xor_sync(0xffffffffu, S.s, w), __shfl_xor_sync(0xffffffffu, S.u, w)};
             S = lp_join(S, o);
         }
-        if (n) for (uint32_t w = 1; w < parts; ++w) best = lp_merge(best, s_best[w][lane]);
     }
     S.m = __shfl_sync(0xffffffffu, S.m, 0); S.s = __shfl_sync(0xffffffffu, S.s, 0); S.u = __shfl_sync(0xffffffffu, S.u, 0);
     const float ls = logf(S.s);                  // nothing left: m = -infinity, s = 0
