@@ -72,6 +72,8 @@ template <class C> static int launch_append_rows(const AppendArgs &A, uint32_t i
 // With x_p = scale log2(e) q . k_p, a part of the positions is summed up as m = max x_p, l = sum 2^(x_p - m), O = sum 2^(x_p - m) v_p; parts are joined
 // by rescaling to the common m, and out = O / l.
 //
+// What bounds it is the cache's bytes (504 MB of two long documents: 89 us, 5.6 TB/s; 77 us at the measured copy rate) and, for short sequences, the beginning and end of each head (some 3 us
+// a block: lengths, page table, queries, rows, each a read that waits for the one before).
 // The work is cut by bytes: a tile is 16 KB of K and V of one K/V head, all tiles of all (sequence, K/V head, group of 8 query heads) are
 // counted through in that order, and every block takes an equal run of them, whatever the lengths are: they are read on the device, so that a
 // captured call follows them. A head costs as much as some tiles more (KV_HEAD_COST). A run that begins or ends inside a sequence's head leaves (m, l, O) in the workspace, at most two of them a
@@ -123,27 +125,30 @@ __device__ __forceinline__ uint64_t kv_request(const AttendArgs &A, uint32_t b, 
     return valid;
 }
 
-// A warp's share of a part: every KV_WARPS-th tile of [t0, t1), 8 query heads; (m, l, O) to shared memory. For a cache of floats the sums on CUDA cores.
-template <class T, class QT, int HD>
+// A warp's share of a part: every KV_WARPS-th tile of [t0, t1), up to NH query heads; (m, l, O) to shared memory. For a cache of floats the sums on CUDA cores, 32 / NH positions at a time:
+// their 32 scores are summed over the lanes together and end in a lane each. What bounds it is instructions: 4 NH of a warp for a position's products and some 20 for the rest (packed fp32), where the
+// bytes of a position of 128 leave an SM 23 cycles; hence the form for 4 heads.
+template <class T, class QT, int HD, int NH>
 __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t h0, uint32_t nh, uint32_t len, uint32_t t0, uint32_t t1,
                                             uint8_t *ring, uint64_t *valid, float *p_sh, float *m_out, float *l_out, float *o_out) {
     using L = KvTile<T, HD>;
-    constexpr int E = HD / 32;
+    constexpr int E = HD / 32, PS = 32 / NH;
+    static_assert(L::TP % PS == 0, "whole steps");
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
     // element i of a lane: a 16-byte piece (or less) of the row, two pieces for rows of 1 KB
     auto elem = [&](int i) { return E * sizeof(T) > 16 ? (uint32_t)(i / 4) * 128u + lane * 4u + (uint32_t)(i % 4) : lane * E + (uint32_t)i; };
-    float2 q[8][E / 2], o[8][E / 2];
+    float2 q[NH][E / 2], o[NH][E / 2];
     const QT *qp = reinterpret_cast<const QT *>(A.q) + (uint64_t)b * A.q_stride + (uint64_t)h0 * HD;
 #pragma unroll
-    for (int h = 0; h < 8; ++h)
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int i = 0; i < E; i += 2) {
             q[h][i / 2] = make_float2(0.f, 0.f);
             if (h < (int)nh) q[h][i / 2] = make_float2(to_f32(qp[h * HD + elem(i)]) * A.scale_log2, to_f32(qp[h * HD + elem(i + 1)]) * A.scale_log2);
             o[h][i / 2] = make_float2(0.f, 0.f);
         }
-    float m = -INFINITY, l = 0.f;                // of head lane / 4; l: this lane's share
+    float m = -INFINITY, l = 0.f;                // of head lane / PS; l: this lane's share
     uint32_t next = t0 + warp;
 #pragma unroll 1
     for (int s = 0; s < KV_STAGES - 1; ++s) {
@@ -173,20 +178,20 @@ __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b,
             }
         };
 #pragma unroll 1
-        for (uint32_t r = 0; r < L::TP; r += 4u) {
-            const uint32_t bits = (uint32_t)(live >> r) & 15u;
+        for (uint32_t r = 0; r < L::TP; r += PS) {
+            const uint32_t bits = (uint32_t)(live >> r) & ((1u << PS) - 1u);
             if (!bits) continue;
-            float s[32];                         // score of head i / 4, position r + i % 4: this lane's part
+            float s[32];                         // score of head i / PS, position r + i % PS: this lane's part
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < PS; ++j) {
                 float2 k[E / 2];
                 row(kt, r + j, k);
 #pragma unroll
-                for (int h = 0; h < 8; ++h) {
+                for (int h = 0; h < NH; ++h) {
                     float2 a = __fmul2_rn(q[h][0], k[0]);
 #pragma unroll
                     for (int i = 1; i < E / 2; ++i) a = __ffma2_rn(q[h][i], k[i], a);
-                    s[h * 4 + j] = a.x + a.y;
+                    s[h * PS + j] = a.x + a.y;
                 }
             }
             // 32 sums over 32 lanes: each exchange halves the values that a lane carries; value i ends in lane i
@@ -200,37 +205,41 @@ __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b,
                         s[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
                     }
             }
-            const float x = (bits >> (lane & 3u)) & 1u ? s[0] : -INFINITY;
-            float mx = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float x = (bits >> (lane % PS)) & 1u ? s[0] : -INFINITY;
+            float mx = x;
+#pragma unroll
+            for (int w = 1; w < PS; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
             const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn, alpha = exp2f(m - base), p = exp2f(x - base);
             const bool moved = __any_sync(0xffffffffu, mn > m);
             m = mn;
             l = l * alpha + p;
             __syncwarp();
             p_sh[lane] = p;
-            if ((lane & 3u) == 0u) p_sh[32u + lane / 4u] = alpha;
+            if (lane % PS == 0u) p_sh[32u + lane / PS] = alpha;
             __syncwarp();
             if (moved) {
 #pragma unroll
-                for (int h = 0; h < 8; ++h) {
+                for (int h = 0; h < NH; ++h) {
                     const float a = p_sh[32 + h];
 #pragma unroll
                     for (int i = 0; i < E / 2; ++i) o[h][i] = __fmul2_rn(o[h][i], make_float2(a, a));
                 }
             }
-            float2 v[4][E / 2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) row(vt, r + j, v[j]);
+            for (int k = 0; k < PS; k += 4) {
+                float2 v[4][E / 2];
 #pragma unroll
-            for (int h = 0; h < 8; ++h) {
-                const float4 p4 = *reinterpret_cast<const float4 *>(p_sh + h * 4);
+                for (int j = 0; j < 4; ++j) row(vt, r + k + j, v[j]);
 #pragma unroll
-                for (int i = 0; i < E / 2; ++i) {
-                    o[h][i] = __ffma2_rn(make_float2(p4.x, p4.x), v[0][i], o[h][i]);
-                    o[h][i] = __ffma2_rn(make_float2(p4.y, p4.y), v[1][i], o[h][i]);
-                    o[h][i] = __ffma2_rn(make_float2(p4.z, p4.z), v[2][i], o[h][i]);
-                    o[h][i] = __ffma2_rn(make_float2(p4.w, p4.w), v[3][i], o[h][i]);
+                for (int h = 0; h < NH; ++h) {
+                    const float4 p4 = *reinterpret_cast<const float4 *>(p_sh + h * PS + k);
+#pragma unroll
+                    for (int i = 0; i < E / 2; ++i) {
+                        o[h][i] = __ffma2_rn(make_float2(p4.x, p4.x), v[0][i], o[h][i]);
+                        o[h][i] = __ffma2_rn(make_float2(p4.y, p4.y), v[1][i], o[h][i]);
+                        o[h][i] = __ffma2_rn(make_float2(p4.z, p4.z), v[2][i], o[h][i]);
+                        o[h][i] = __ffma2_rn(make_float2(p4.w, p4.w), v[3][i], o[h][i]);
+                    }
                 }
             }
         }
@@ -238,12 +247,13 @@ __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b,
         st = st + 1u == KV_STAGES ? 0u : st + 1u;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if ((lane & 3u) == 0u) { m_out[lane / 4u] = m; l_out[lane / 4u] = l; }
+#pragma unroll
+    for (int w = 1; w < PS; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+    if (lane % PS == 0u) { m_out[lane / PS] = m; l_out[lane / PS] = l; }
+    if (NH < 8 && lane < 8u - NH) { m_out[NH + lane] = -INFINITY; l_out[NH + lane] = 0.f; }
     __syncthreads();                             // the rings are read no more
 #pragma unroll
-    for (int h = 0; h < 8; ++h)
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int i = 0; i < E; i += 2) { o_out[h * HD + elem(i)] = o[h][i / 2].x; o_out[h * HD + elem(i + 1)] = o[h][i / 2].y; }
 }
@@ -441,8 +451,9 @@ __device__ __forceinline__ void kv_write_new(const AttendArgs &A, uint32_t b, ui
     }
 }
 
-template <class T, class QT, int HD>
-__global__ void __launch_bounds__(KV_WARPS * 32, 1) k_kv_attend(AttendArgs A) {
+// NH: heads that a group can have (4 only for a cache of floats)
+template <class T, class QT, int HD, int NH>
+__global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend(AttendArgs A) {
     pdl_prologue();
     using L = KvTile<T, HD>;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -499,7 +510,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) k_kv_attend(AttendArgs A) {
             uint8_t *ring = sm + warp * KV_STAGES * L::BYTES;
             float *o_warp = o_sh + warp * 8u * HD;
             if constexpr (sizeof(T) == 4)
-                attend_part_f32<T, QT, HD>(A, b, kvh, h0, nh, len, t0, t1, ring, s_valid[warp], s_p[sizeof(T) == 4 ? warp : 0], s_m[warp], s_l[warp], o_warp);
+                attend_part_f32<T, QT, HD, NH>(A, b, kvh, h0, nh, len, t0, t1, ring, s_valid[warp], s_p[sizeof(T) == 4 ? warp : 0], s_m[warp], s_l[warp], o_warp);
             else
                 attend_part_mma<T, QT, HD>(A, b, kvh, h0, nh, len, t0, t1, ring, s_valid[warp], s_m[warp], s_l[warp], o_warp);
             __syncthreads();
@@ -518,7 +529,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) k_kv_attend(AttendArgs A) {
                 else if (tid < nh && A.lse) A.lse[(uint64_t)b * A.n_q + h0 + tid] = kv_lse(M, lt);
             }
             __syncthreads();
-            for (uint32_t i = tid * 4u; i < 8u * HD; i += KV_WARPS * 128u) {
+            for (uint32_t i = tid * 4u; i < (uint32_t)NH * HD; i += KV_WARPS * 128u) {
                 const uint32_t h = i / HD;
                 float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -600,12 +611,12 @@ __global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
     if (tid == 0u && A.lse) A.lse[(uint64_t)b * A.n_q + head] = kv_lse(M, l);
 }
 
-template <class T, class QT, int HD> static int launch_attend(const AttendArgs &A, uint32_t blocks, cudaStream_t s) {
+template <class T, class QT, int HD, int NH> static int launch_attend(const AttendArgs &A, uint32_t blocks, cudaStream_t s) {
     constexpr size_t smem = (size_t)KV_WARPS * KV_STAGES * KvTile<T, HD>::BYTES;
     static std::atomic<uint64_t> set{0};
-    if (!raise_smem_limit(reinterpret_cast<const void *>(k_kv_attend<T, QT, HD>), smem, set)) return 0;
+    if (!raise_smem_limit(reinterpret_cast<const void *>(k_kv_attend<T, QT, HD, NH>), smem, set)) return 0;
     prof_begin("kv_attend", s);
-    RC_LAUNCH((k_kv_attend<T, QT, HD>), blocks, KV_WARPS * 32, smem, s, A);
+    RC_LAUNCH((k_kv_attend<T, QT, HD, NH>), blocks, KV_WARPS * 32, smem, s, A);
     RC_LAUNCHED();
     prof_end(s);
     prof_begin("kv_attend_join", s);
@@ -615,7 +626,9 @@ template <class T, class QT, int HD> static int launch_attend(const AttendArgs &
     return 1;
 }
 template <class T, class QT> static int launch_attend_hd(const AttendArgs &A, uint32_t hd, uint32_t blocks, cudaStream_t s) {
-    return hd == 256u ? launch_attend<T, QT, 256>(A, blocks, s) : hd == 128u ? launch_attend<T, QT, 128>(A, blocks, s) : launch_attend<T, QT, 64>(A, blocks, s);
+    if constexpr (sizeof(T) == 4)                // half the instructions where K/V heads have at most four query heads
+        if (A.G <= 4u) return hd == 256u ? launch_attend<T, QT, 256, 4>(A, blocks, s) : hd == 128u ? launch_attend<T, QT, 128, 4>(A, blocks, s) : launch_attend<T, QT, 64, 4>(A, blocks, s);
+    return hd == 256u ? launch_attend<T, QT, 256, 8>(A, blocks, s) : hd == 128u ? launch_attend<T, QT, 128, 8>(A, blocks, s) : launch_attend<T, QT, 64, 8>(A, blocks, s);
 }
 
 // the cache's strides in elements (0: dense), or a message
@@ -675,7 +688,7 @@ uint64_t redcuda_kv_attend_workspace(const redcuda_paged_kv *kv, uint32_t n_q) {
     if (!require_device()) return 0;
     const uint32_t sms = sm_count();
     RC_REQUIRE(sms, "kv attend: the device's size is not known");
-    return attend_workspace(sms, kv->head_dim);
+    return attend_workspace(sms * KV_BLOCKS, kv->head_dim);
 }
 
 int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *lens_dev,
@@ -703,7 +716,7 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     if (!require_device()) return 0;
     const uint32_t sms = sm_count();
     RC_REQUIRE(sms, "kv attend: the device's size is not known");
-    RC_REQUIRE(workspace_dev && workspace_bytes >= attend_workspace(sms, hd), "kv attend: a workspace of %llu bytes is needed", (unsigned long long)attend_workspace(sms, hd));
+    RC_REQUIRE(workspace_dev && workspace_bytes >= attend_workspace(sms * KV_BLOCKS, hd), "kv attend: a workspace of %llu bytes is needed", (unsigned long long)attend_workspace(sms * KV_BLOCKS, hd));
     AttendArgs A{};
     A.k = kv->k; A.v = kv->v; A.page_stride = st[0]; A.token_stride = st[1]; A.head_stride = st[2];
     A.table = table_dev; A.table_width = table_width; A.page_size = kv->page_size; A.n_pages = kv->n_pages;
@@ -715,7 +728,7 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     const uint64_t tile = 8192u / (hd * val_size(kv->type)), tiles = ((uint64_t)table_width * kv->page_size + tile - 1u) / tile;
     auto few = [](uint64_t n) { return n < 8192u ? n : 8192u; };      // more than that of one thing is blocks enough
     const uint64_t runs = (few(tiles) * few(n_seqs) * few(A.n_kv * A.gsplit) + KV_MIN_TILES - 1u) / KV_MIN_TILES;
-    const uint32_t blocks = runs < sms ? (uint32_t)runs : sms;
+    const uint32_t blocks = runs < sms * KV_BLOCKS ? (uint32_t)runs : sms * KV_BLOCKS;
     A.meta = (uint32_t *)workspace_dev;
     A.part = (float *)(A.meta + (size_t)blocks * 4u);
     A.part_ml = A.part + (size_t)blocks * 2u * 8u * hd;

@@ -4,9 +4,12 @@
 
 namespace rc {
 
-constexpr int KV_WARPS = 6, KV_STAGES = 2;
+// Warps and stages of a block, blocks of a multiprocessor: twelve stages of 16 KB an SM in every form. Six warps x two stages x one block: two documents of 131072 and some 115000 positions 86 us, 64 ragged
+// sequences 22, 238 of 147 positions 42, 205 of up to 33 36; three x two x two 89, 20, 35, 24 (one block's head begins or ends while the other's tiles flow); two x three x two 90, 21, 36, 25;
+// two x two x three 93, 21, 34, 22.
+constexpr int KV_WARPS = 3, KV_STAGES = 2, KV_BLOCKS = 2;
 constexpr uint32_t KV_HEAD_COST = 12u;           // what a head's begin and end take, in tiles
-constexpr uint32_t KV_MIN_TILES = 4u;            // tiles that a block takes at least
+constexpr uint32_t KV_MIN_TILES = 3u;            // tiles that a block takes at least: one a warp
 
 struct AttendArgs {
     void *k, *v;
