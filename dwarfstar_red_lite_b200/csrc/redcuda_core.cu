@@ -79,7 +79,7 @@ int status_failed() {
     else if (pg) set_error("a position beyond a sequence's page table, or a page id outside the cache");
     else if (sl) set_error("a state slot outside the states, or one that two sequences of a call share");
     else if (sq) set_error("sequence bounds that do not ascend within the rows of the call");
-    else set_error("an expert kernel gave up waiting for a weight copy (bounded wait ran out); its outputs are incomplete");
+    else set_error("a kernel gave up waiting for a copy or a product (bounded wait ran out); its outputs are incomplete");
     return 1;
 }
 

@@ -159,6 +159,7 @@ static int delta_check(const redcuda_delta_dims *d, const char *who, uint32_t ro
 static int delta_pointers(const redcuda_delta_dims *d, const char *who, uint32_t rows, uint32_t n_slots, const DeltaArgs &A) {
     RC_REQUIRE(A.q && A.k && A.v && A.gate && A.beta && A.state && A.out, "%s: null argument", who);
     RC_REQUIRE(aligned16(A.q) && aligned16(A.k) && aligned16(A.v) && aligned16(A.state) && aligned16(A.out), "%s: a pointer is not 16-byte aligned", who);
+    RC_REQUIRE(aligned4(A.gate) && aligned4(A.beta) && aligned4(A.slots) && aligned4(A.cu), "%s: gates, betas or whole numbers are not 4-byte aligned", who);
     const uint32_t size = val_size(d->type);
     const uint64_t key = (uint64_t)d->n_group * d->d_state, val = (uint64_t)d->dt_rank * d->d_state, ob = (uint64_t)rows * val * size, sb = (uint64_t)n_slots * val * d->d_state * 4u;
     const void *in[5] = {A.q, A.k, A.v, A.gate, A.beta};
@@ -208,6 +209,15 @@ int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, ui
     if (!delta_pointers(d, "delta rule", n_tokens, n_slots, A)) return 0;
     const uint64_t need = redcuda_delta_rule_workspace(d, n_tokens, n_seqs);
     RC_REQUIRE(!need || (workspace_dev && workspace_bytes >= need && aligned16(workspace_dev)), "delta rule: a 16-byte aligned workspace of %llu bytes is needed", (unsigned long long)need);
+    if (need) {
+        const uint32_t size = val_size(d->type);
+        const uint64_t val = (uint64_t)d->dt_rank * d->d_state, rows = (uint64_t)n_tokens * d->dt_rank * 4u;
+        RC_REQUIRE(!overlap(workspace_dev, need, out_dev, n_tokens * val * size) && !overlap(workspace_dev, need, state_dev, n_slots * val * d->d_state * 4u) &&
+                   !overlap(workspace_dev, need, q_dev, span_bytes(n_tokens, A.q_stride, (uint64_t)d->n_group * d->d_state, size)) &&
+                   !overlap(workspace_dev, need, k_dev, span_bytes(n_tokens, A.k_stride, (uint64_t)d->n_group * d->d_state, size)) &&
+                   !overlap(workspace_dev, need, v_dev, span_bytes(n_tokens, A.v_stride, val, size)) && !overlap(workspace_dev, need, gate_dev, rows) && !overlap(workspace_dev, need, beta_dev, rows),
+                   "delta rule: the workspace overlaps rows, states or outputs");
+    }
     if (!require_device()) return 0;
     if (!n_tokens) return 1;
     A.status = status_words();

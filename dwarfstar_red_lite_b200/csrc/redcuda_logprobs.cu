@@ -355,6 +355,7 @@ int redcuda_token_logprobs_device(uint32_t type, uint32_t rows, uint32_t vocab, 
     const uint64_t lb = span_bytes(rows, row_stride, vocab, val_size(type)), ob = (uint64_t)rows * 4u;
     RC_REQUIRE(!overlap(logits_dev, lb, logprob_dev, ob) && !overlap(logits_dev, lb, entropy_dev, ob) && !overlap(logits_dev, lb, top_ids_dev, ob * top_n) &&
                !overlap(logits_dev, lb, top_logprobs_dev, ob * top_n), "token logprobs: an output lies inside the logits");
+    RC_REQUIRE(aligned4(tokens_dev) && aligned4(logprob_dev) && aligned4(entropy_dev) && aligned4(top_ids_dev) && aligned4(top_logprobs_dev), "token logprobs: tokens or outputs are not 4-byte aligned");
     if (!require_device()) return 0;
     if (!rows) return 1;
     LogprobArgs A{logits_dev, row_stride, tokens_dev, logprob_dev, entropy_dev, top_logprobs_dev, top_ids_dev, status_words(), vocab, top_n};

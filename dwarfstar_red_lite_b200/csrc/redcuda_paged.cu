@@ -649,6 +649,11 @@ static int kv_check(const redcuda_paged_kv *kv, const char *who, uint64_t (&st)[
     return 1;
 }
 
+// whether some array lies inside the cache
+static bool kv_overlap(const redcuda_paged_kv *kv, const uint64_t (&st)[3], const void *p, uint64_t bytes) {
+    const uint64_t n = ((uint64_t)(kv->n_pages - 1u) * st[0] + (uint64_t)(kv->page_size - 1u) * st[1] + (uint64_t)(kv->n_kv - 1u) * st[2] + kv->head_dim) * val_size(kv->type);
+    return overlap(kv->k, n, p, bytes) || overlap(kv->v, n, p, bytes);
+}
 static uint64_t attend_workspace(uint32_t blocks, uint32_t hd) { return (uint64_t)blocks * (2u * (8u * hd + 16u) * 4u + 16u); }
 
 }  // namespace rc
@@ -670,6 +675,9 @@ int redcuda_kv_append_device(const redcuda_paged_kv *kv, const int32_t *table_de
     if (!row_stride) row_stride = row;
     RC_REQUIRE(row_stride >= row && row_stride * val_size(in_type) % 16u == 0u && row_stride < (1ull << 32), "kv append: row stride %llu", (unsigned long long)row_stride);
     RC_REQUIRE(aligned16(k_dev) && aligned16(v_dev), "kv append: rows are not 16-byte aligned");
+    RC_REQUIRE(aligned4(table_dev) && aligned4(start_dev) && aligned4(cu_seqlens_dev), "kv append: whole numbers are not 4-byte aligned");
+    const uint64_t bytes = span_bytes(n_tokens, row_stride, row, val_size(in_type));
+    RC_REQUIRE(!kv_overlap(kv, st, k_dev, bytes) && !kv_overlap(kv, st, v_dev, bytes), "kv append: the rows lie inside the cache");
     if (!require_device()) return 0;
     if (!n_tokens) return 1;
     AppendArgs A{kv->k, kv->v, st[0], st[1], st[2], table_dev, start_dev, cu_seqlens_dev, k_dev, v_dev, row_stride, table_width, kv->page_size, kv->n_pages, n_seqs, n_tokens, kv->n_kv,
@@ -712,6 +720,12 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     const uint64_t out_bytes = (uint64_t)n_seqs * qrow * qs;
     RC_REQUIRE(!overlap(out_dev, out_bytes, q_dev, span_bytes(n_seqs, q_stride, qrow, qs)) && !overlap(out_dev, out_bytes, k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) &&
                !overlap(out_dev, out_bytes, v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)), "kv attend: the output lies inside the inputs");
+    RC_REQUIRE(aligned4(table_dev) && aligned4(lens_dev) && aligned4(lse_dev), "kv attend: whole numbers or lse are not 4-byte aligned");
+    RC_REQUIRE(!kv_overlap(kv, st, out_dev, out_bytes) && !kv_overlap(kv, st, q_dev, span_bytes(n_seqs, q_stride, qrow, qs)) && !kv_overlap(kv, st, workspace_dev, workspace_bytes) &&
+               !kv_overlap(kv, st, k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) && !kv_overlap(kv, st, v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) &&
+               !kv_overlap(kv, st, lse_dev, (uint64_t)n_seqs * n_q * 4u), "kv attend: rows, output or workspace lie inside the cache");
+    RC_REQUIRE(!overlap(workspace_dev, workspace_bytes, out_dev, out_bytes) && !overlap(workspace_dev, workspace_bytes, lse_dev, (uint64_t)n_seqs * n_q * 4u) &&
+               !overlap(out_dev, out_bytes, lse_dev, (uint64_t)n_seqs * n_q * 4u), "kv attend: output, lse and workspace overlap");
     RC_REQUIRE(!(scale != scale), "kv attend: scale is not a number");
     if (!require_device()) return 0;
     const uint32_t sms = sm_count();

@@ -11,6 +11,7 @@ constexpr uint32_t VT_F32 = 0u, VT_F16 = 1u, VT_BF16 = 30u;       // ggml ids
 inline uint32_t val_size(uint32_t t) { return t == VT_F32 ? 4u : t == VT_F16 || t == VT_BF16 ? 2u : 0u; }
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+inline bool aligned4(const void *p) { return ((uintptr_t)p & 3u) == 0; }
 inline bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
     return a && b && na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }

@@ -313,7 +313,8 @@ int redcuda_delta_step_device(const redcuda_delta_dims *d, uint32_t n_seqs, cons
                               const void *v_dev, const float *gate_dev, const float *beta_dev, float *state_dev, void *out_dev, void *stream);
 
 /* Prompts laid end to end: tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of the n_tokens rows are sequence b's, in order (n_seqs + 1 ascending numbers on
- * the device; a sequence may be empty; rows from cu_seqlens[n_seqs] on are left as they were). Slots as above. workspace_dev:
+ * the device; a sequence may be empty; rows from cu_seqlens[n_seqs] on are left as they were). Bounds that fall or leave the rows are reported and their sequence left out;
+ * of rows that two sequences then claim the results are not defined. A value that is not finite makes what depends on it NaN, from its token on. Slots as above. workspace_dev:
  * redcuda_delta_rule_workspace bytes, 16-byte aligned (0: none is needed); calls that overlap on the GPU need one each. */
 uint64_t redcuda_delta_rule_workspace(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs);
 int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs, const int32_t *cu_seqlens_dev, const int32_t *slots_dev,

@@ -220,6 +220,34 @@ def test_a_nan_stays_in_its_sequence():
     assert bool(state[0].isfinite().all()) and bool(state[2].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("what, value", [("q", math.nan), ("k", math.inf), ("k", math.nan), ("gate", math.nan), ("gate", math.inf), ("beta", -math.inf), ("v", math.inf)])
+@pytest.mark.parametrize("t", [130, 193, 200, 257])
+def test_what_is_not_finite_comes_from_its_token_on(dtype, what, value, t):
+    """The tokens before it, also those of its chunk, and the other sequences are as they were to the bit; a query spoils its own output alone."""
+    x = _inputs(_gen(6), 400, 1, 2, 128, TYPES[dtype][1], 3)
+    cu, dims = [0, 130, 260, 400], rc.DeltaDims(TYPES[dtype][0], 1, 2, 128)
+    clean, want = _rule(x, cu, [0, 1, 2], dims, 3)
+    x[what][(t, 0, 7) if what in ("q", "k") else (t, 1, 5) if what == "v" else (t, 1)] = value
+    out, state = _rule(x, cu, [0, 1, 2], dims, 3)
+    heads = {"q": [0, 1], "k": [0, 1]}.get(what, [1])
+    last = t + 1 if what == "q" else 260
+    for h in (0, 1):
+        rows = slice(5, 6) if what == "v" else slice(None)
+        if h in heads:
+            assert bool(out[t:last, h, rows].isnan().all())
+            assert torch.equal(out[:t, h], clean[:t, h]) and torch.equal(out[last:, h], clean[last:, h])
+        else:
+            assert torch.equal(out[:, h], clean[:, h])
+        for s in range(3):
+            if s == 1 and h in heads and what != "q":
+                assert bool(state[s, h, rows].isnan().all())
+                if what == "v":
+                    assert torch.equal(state[s, h, :5], want[s, h, :5])
+            else:
+                assert torch.equal(state[s, h], want[s, h])
+
+
 def test_capture_and_repeats():
     x = _inputs(_gen(7), 500, 2, 4, 128, torch.bfloat16, 4)
     dims, s = rc.DeltaDims(30, 2, 4, 128), torch.cuda.Stream()

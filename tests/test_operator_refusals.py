@@ -36,7 +36,9 @@ def _attend(kv=None, table=A[2], width=4, n_seqs=3, lens=A[3], n_q=8, q_type=0, 
     (dict(kv=_kv(type=0), q_type=1), "queries of type 1"), (dict(q_stride=500), "row strides 500"), (dict(q_stride=513), "row strides 513"),
     (dict(k_new=A[8], v_new=A[9], new_stride=64), "row strides"), (dict(q=A[4] + 4), "not 16-byte aligned"), (dict(out=A[5] + 2), "not 16-byte aligned"), (dict(work=A[7] + 8), "not 16-byte aligned"),
     (dict(out=A[4] + 16), "lies inside the inputs"), (dict(k_new=A[5] - 16, v_new=A[9]), "lies inside the inputs"), (dict(scale=float("nan")), "not a number"),
-    (dict(width=0x7ffffff0, kv=_kv(page_size=64)), "2^32 positions"),
+    (dict(width=0x7ffffff0, kv=_kv(page_size=64)), "2^32 positions"), (dict(lens=A[3] + 2), "4-byte aligned"), (dict(table=A[2] + 1), "4-byte aligned"), (dict(lse=A[6] + 2), "4-byte aligned"),
+    (dict(out=A[0] + 64), "inside the cache"), (dict(q=A[1] + 64), "inside the cache"), (dict(work=A[0] - 64), "inside the cache"), (dict(k_new=A[1], v_new=A[9]), "inside the cache"),
+    (dict(lse=A[0]), "inside the cache"), (dict(lse=A[5] + 16), "overlap"), (dict(work=A[5] + 16), "overlap"),
 ])
 def test_attend(change, message):
     _refused(lambda: _attend(**change), message)
@@ -50,7 +52,8 @@ def _append(kv=None, table=A[2], width=4, n_seqs=3, start=A[3], n_tokens=5, cu=A
 @pytest.mark.parametrize("change, message", [
     (dict(kv=_kv(type=8)), "cache type 8"), (dict(table=None), "null or empty"), (dict(start=None), "null or empty"), (dict(k=None), "null or empty"), (dict(v=None), "null or empty"),
     (dict(n_seqs=0), "null or empty"), (dict(t=12), "rows of type 12"), (dict(cu=None), "5 rows for 3 sequences"), (dict(stride=100), "row stride 100"), (dict(stride=130), "row stride 130"),
-    (dict(k=A[5] + 4), "not 16-byte aligned"), (dict(n_tokens=0x7fffffff), "too many rows"),
+    (dict(k=A[5] + 4), "not 16-byte aligned"), (dict(n_tokens=0x7fffffff), "too many rows"), (dict(start=A[3] + 2), "4-byte aligned"), (dict(cu=A[4] + 1), "4-byte aligned"),
+    (dict(k=A[0] + 16), "inside the cache"), (dict(v=A[1] + 512), "inside the cache"),
 ])
 def test_append(change, message):
     _refused(lambda: _append(**change), message)
@@ -75,7 +78,7 @@ def _delta(form="rule", dims=None, n_tokens=6, n_seqs=2, cu=A[0], slots=A[1], n_
     (dict(dims=rc.DeltaDims(0, 2, 4, 64, 0, 0, 0, float("nan"))), "not a number"), (dict(n_slots=0), "no states"), (dict(slots=None, n_slots=1), "2 sequences for 1 states"),
     (dict(q=None), "null argument"), (dict(gate=None), "null argument"), (dict(state=None), "null argument"), (dict(out=None), "null argument"), (dict(k=A[3] + 8), "not 16-byte aligned"),
     (dict(state=A[7] + 4), "not 16-byte aligned"), (dict(out=A[4]), "inside the inputs"), (dict(out=A[2] + 16), "inside the inputs"), (dict(state=A[4] + 64), "inside the inputs"),
-    (dict(out=A[7] + 32), "inside the states"), (dict(n_seqs=0), "no sequences"),
+    (dict(out=A[7] + 32), "inside the states"), (dict(n_seqs=0), "no sequences"), (dict(gate=A[5] + 2), "4-byte aligned"), (dict(slots=A[1] + 1), "4-byte aligned"),
 ])
 def test_delta(form, change, message):
     _refused(lambda: _delta(form, **change), message)
@@ -85,6 +88,11 @@ def test_delta_rule_without_bounds_or_workspace():
     _refused(lambda: _delta("rule", cu=None), "no sequences")
     d = rc.DeltaDims(0, 16, 32, 128)
     need = d.workspace(5000, 2)
+    assert need
+    call = lambda work: rc.lib().redcuda_delta_rule_device(C.byref(d), 5000, 2, A[0], A[1], 4, A[2], A[3], A[4], A[5], A[6], A[7], A[11] * 4, work, need, None)  # noqa: E731
+    for inside in (A[2], A[4] + 64, A[5], A[7] + 1024, A[11] * 4):
+        _refused(lambda: call(inside), "the workspace overlaps")
+    _refused(lambda: call(A[9] + 8), "aligned workspace")
     if need:
         _refused(lambda: rc.lib().redcuda_delta_rule_device(C.byref(d), 5000, 2, A[0], A[1], 4, A[2], A[3], A[4], A[5], A[6], A[7], A[11] * 4, A[9], need - 1, None), "workspace of")
 
@@ -97,6 +105,7 @@ def _logprobs(t=0, rows=4, vocab=100, stride=0, x=A[0], tokens=A[1], top=3, lp=A
     (dict(t=2), "logits of type 2"), (dict(x=None), "null or empty"), (dict(vocab=0), "null or empty"), (dict(stride=99), "100 values 99 apart"), (dict(top=33), "33 alternatives"),
     (dict(vocab=2), "3 alternatives of 2"), (dict(ids=None), "alternatives need"), (dict(tlp=None), "alternatives need"), (dict(top=0), "alternatives need"),
     (dict(tokens=None), "of no token"), (dict(x=A[0] + 2), "not aligned"), (dict(t=1, x=A[0] + 1), "not aligned"), (dict(ent=A[0] + 64), "inside the logits"), (dict(ids=A[0]), "inside the logits"),
+    (dict(lp=A[2] + 2), "4-byte aligned"), (dict(tokens=A[1] + 1), "4-byte aligned"),
 ])
 def test_logprobs(change, message):
     _refused(lambda: _logprobs(**change), message)
