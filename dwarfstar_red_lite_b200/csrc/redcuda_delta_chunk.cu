@@ -23,9 +23,9 @@ constexpr uint32_t DC_KT = DC_T * DC_S * 2u;             // a digit of the keys 
 constexpr uint32_t DC_SQ = DC_T * DC_T * 2u;             // a digit of T or P, rows t, k: s
 struct DcMeta {                                  // of a chunk and value head
     float dec[DC_T], kdec[DC_T];                 // exp(G_t), exp(G_last - G_t)
-    float last, f_k, f_q, f_t, f_p;              // exp(G_last); what a digit's unit is worth in K, Q, T, P
+    float last, f_k, f_q, f_t[4], f_p[4];        // exp(G_last); what a digit's unit is worth in K, in Q, in 16 rows each of T and P
     float most_dec;                              // the largest exp(G_t)
-    uint32_t nan_from, bad_q[2], pad[119];       // tokens from which on everything is NaN; tokens whose query is not finite
+    uint32_t nan_from, bad_q[2], pad[113];       // tokens from which on everything is NaN; tokens whose query is not finite
 };
 static_assert(sizeof(DcMeta) == 1024, "copied in whole");
 constexpr uint32_t DC_REC = 4u * DC_SQ + (uint32_t)sizeof(DcMeta);       // T hi, T lo, P hi, P lo, meta
@@ -62,12 +62,15 @@ __device__ __forceinline__ void dc_mma(float (&c)[4], const uint32_t (&a)[4], ui
 }
 
 // ---- what does not depend on the state ----------------------------------------------------------------------------------------------------------
-// A block per chunk and key head: digits of K and Q, K K^T and Q K^T on the tensor cores (their lower triangles), then for each of the key head's value heads (two at a time, half a block
-// each) the decays, the inverse of 1 + A and the digits of T and P. The inverse goes by blocks of 16: those on the diagonal by substitution, a column a lane; the others T_ij = -T_ii sum_k A_ik T_kj
-// in the order of their distance from it, which is as stable as substitution (powers of A are not, where keys are alike).
+// A block per chunk and key head: digits of K and Q (a power of two for the chunk's keys, one for its queries), K K^T and Q K^T on the tensor cores (their lower triangles, 16 rows a warp, which stay in its
+// registers), then for the key head's value heads, two at a time, the decays, P and its digits from the registers, A to shared memory, the inverse of 1 + A and the digits of T. The inverse goes by blocks
+// of 16: those on the diagonal by substitution, a column a lane; the others T_ij = -T_ii sum_k A_ik T_kj, a column of blocks a warp, which is as stable as substitution (powers of A are not, where
+// keys are alike). The digits of T and P have a power of two for 16 rows each, so that no warp waits for another's largest.
+// What bounds it is latency: a dozen short phases between barriers, hence three blocks an SM.
 constexpr uint32_t DC_PITCH = 68u;               // floats of a row of the 64 x 64 matrices in shared memory
 constexpr uint32_t DC_MAT = DC_T * DC_PITCH * 4u;
 __device__ __forceinline__ void dc_half_sync(uint32_t half) { asm volatile("bar.sync %0, 128;" :: "r"(half + 1u) : "memory"); }
+__device__ __forceinline__ float dc_warp_max(float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x))); }      // of numbers that are not negative
 // e^x for x <= 0 (and moderate x above): the error of the argument is |x| 2^-24, of a result e^x
 __device__ __forceinline__ float dc_exp(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896340736f)); return r; }
 // The digits of a 16 x 16 block in the accumulator layout (8 values a lane) as operand A, under the block's own power of two
@@ -77,7 +80,7 @@ __device__ __forceinline__ float dc_block_operand(const float (&x)[2][4], uint32
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[i][e]));
-    dc_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))), up, unit);
+    dc_scale(dc_warp_max(most), up, unit);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         dc_digits(x[i][0] * up, x[i][1] * up, hi[2 * i], lo[2 * i]);
@@ -102,15 +105,12 @@ __device__ __forceinline__ void dc_block_product(float (&c)[2][4], const uint32_
     }
 }
 
-template <class T, int DIG>
-__global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_seqs, uint8_t *ws, uint64_t slots) {
+// WIDE: more than two value heads a key head (the products are then kept for the next two)
+template <class T, int DIG, bool WIDE>
+__global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_seqs, uint8_t *ws, uint64_t slots) {
     pdl_prologue();
-    extern __shared__ __align__(128) uint8_t sm[];
-    float *const s_kk = reinterpret_cast<float *>(sm), *const s_qk = s_kk + DC_T * DC_PITCH;
-    uint8_t *const dig = sm + 2u * DC_MAT;       // the digits; later the halves' matrices A and T
-    __shared__ float s_red[2][8], s_beta[2][DC_T];
-    __shared__ float2 s_max[2][4];
-    __shared__ float s_d[2][4];
+    extern __shared__ __align__(128) uint8_t sm[];           // the digits; then the matrices A and T of two value heads
+    __shared__ float s_red[2][8], s_beta[2][DC_T], s_diag[2][4], s_amax[2][4], s_peak[2];
     __shared__ float2 s_cum[2][DC_T];            // the sums of the gates, each as a float and what it lacks
     __shared__ uint32_t s_bad[2][2];             // tokens whose key or query is not finite
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, kh = blockIdx.y, width = A.rank / A.groups;
@@ -128,14 +128,24 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
     const int64_t chunk = (int64_t)slot - (int64_t)(lo / DC_T) - (int64_t)b;
     if (chunk < 0 || chunk * DC_T >= hi - lo) return;
     const uint32_t t0 = (uint32_t)lo + (uint32_t)chunk * DC_T, n = min((uint32_t)DC_T, (uint32_t)hi - t0);
+    uint8_t *const keys = ws + (slot * A.groups + kh) * dc_keys(DIG), *const recs = ws + slots * A.groups * dc_keys(DIG) + slot * A.rank * DC_REC;
+    const uint32_t dv = warp == 0u ? 0u : warp == 7u ? 1u : 2u;          // the value head of a pair whose decays this warp makes (2: none): the warps with the fewest products
 
-    // rows 8 warp .. 8 warp + 7 of K and Q: a lane has row lane % 8 and the 8-value pieces lane / 8 + 4 i
-    const uint32_t t = warp * 8u + (lane & 7u);
-    float kx[4][8], qx[4][8], mk = 0.f, mq = 0.f;
-    const uint32_t half = tid >> 7, ht = tid & 127u, hw = ht >> 5;       // from the decays on, half a block has a value head
-    float g_raw[2] = {0.f, 0.f}, b_raw[2] = {0.f, 0.f};      // the gates and betas of the half's first value head, tokens 2 lane and 2 lane + 1
-    {
-        constexpr int P = 8 * sizeof(T) / 16;    // loads of eight values
+    float g_raw[2] = {0.f, 0.f}, b_raw[2] = {0.f, 0.f};      // gates and betas of tokens 2 lane and 2 lane + 1
+    auto gates = [&](uint32_t v) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2u; ++i) {
+            g_raw[i] = b_raw[i] = 0.f;
+            if (lane * 2u + i < n) {
+                g_raw[i] = A.gate[(uint64_t)(t0 + lane * 2u + i) * A.rank + kh * width + v];
+                b_raw[i] = A.beta[(uint64_t)(t0 + lane * 2u + i) * A.rank + kh * width + v];
+            }
+        }
+    };
+    float f_k, f_q;
+    {   // rows 8 warp .. 8 warp + 7 of K and Q: a lane has row lane % 8 and the 8-value pieces lane / 8 + 4 i
+        constexpr int P = 8 * sizeof(T) / 16, N = 16 / sizeof(T);      // loads of eight values, values of a load
+        const uint32_t t = warp * 8u + (lane & 7u);
         uint4 rk[4][P], rq[4][P];
         const T *const k = reinterpret_cast<const T *>(A.k) + (uint64_t)(t0 + min(t, n - 1u)) * A.k_stride + kh * DC_S + (lane >> 3) * 8u;
         const T *const q = reinterpret_cast<const T *>(A.q) + (uint64_t)(t0 + min(t, n - 1u)) * A.q_stride + kh * DC_S + (lane >> 3) * 8u;
@@ -143,79 +153,79 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < P; ++e) { rk[i][e] = reinterpret_cast<const uint4 *>(k + i * 32)[e]; rq[i][e] = reinterpret_cast<const uint4 *>(q + i * 32)[e]; }
-        if (hw == 0u && half < width)
+        if (dv < width) gates(dv);
+        if (tid < 4u) s_bad[tid >> 1][tid & 1u] = 0u;
+        __syncthreads();
+        // a row's largest; a row behind the last token or with a number that is not finite is taken out
+        auto values = [](uint4 w, float (&x)[N]) {
+            const T *const p = reinterpret_cast<const T *>(&w);
 #pragma unroll
-            for (uint32_t i = 0; i < 2u; ++i)
-                if (lane * 2u + i < n) {
-                    g_raw[i] = A.gate[(uint64_t)(t0 + lane * 2u + i) * A.rank + kh * width + half];
-                    b_raw[i] = A.beta[(uint64_t)(t0 + lane * 2u + i) * A.rank + kh * width + half];
-                }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const T *const pk = reinterpret_cast<const T *>(rk[i]), *const pq = reinterpret_cast<const T *>(rq[i]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { kx[i][e] = t < n ? to_f32(pk[e]) : 0.f; qx[i][e] = t < n ? to_f32(pq[e]) : 0.f; }
-        }
-    }
-    if (tid < 4u) s_bad[tid >> 1][tid & 1u] = 0u;
-    __syncthreads();
-    bool fk = true, fq = true;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { fk &= fabsf(kx[i][e]) < INFINITY; fq &= fabsf(qx[i][e]) < INFINITY; mk = fmaxf(mk, fabsf(kx[i][e])); mq = fmaxf(mq, fabsf(qx[i][e])); }
-    const uint32_t row_lanes = 0x01010101u << (lane & 7u), wk = __ballot_sync(0xffffffffu, !fk) & row_lanes, wq = __ballot_sync(0xffffffffu, !fq) & row_lanes;
-    if (wk) {                                    // a row that is not finite is taken out
-        mk = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) kx[i >> 3][i & 7] = 0.f;
-        if (lane < 8u) atomicOr(&s_bad[0][t >> 5], 1u << (t & 31u));
-    }
-    if (wq) {
-        mq = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) qx[i >> 3][i & 7] = 0.f;
-        if (lane < 8u) atomicOr(&s_bad[1][t >> 5], 1u << (t & 31u));
-    }
-    for (int w = 16; w; w >>= 1) { mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, w)); mq = fmaxf(mq, __shfl_xor_sync(0xffffffffu, mq, w)); }
-    if (lane == 0u) { s_red[0][warp] = mk; s_red[1][warp] = mq; }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { mk = fmaxf(mk, s_red[0][i]); mq = fmaxf(mq, s_red[1][i]); }
-    float up_k, f_k, up_q, f_q;
-    dc_scale(mk, up_k, f_k);
-    dc_scale(mq, up_q, f_q);
-    uint8_t *const keys = ws + (slot * A.groups + kh) * dc_keys(DIG);
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) {
-        auto put = [&](const float (&x)[8], float up, uint32_t row) {
-            const uint32_t at = dc_kq_at(row, (lane >> 3) + 4u * i);
-            uint4 h, l;
-            dc_digits(x[0] * up, x[1] * up, h.x, l.x); dc_digits(x[2] * up, x[3] * up, h.y, l.y);
-            dc_digits(x[4] * up, x[5] * up, h.z, l.z); dc_digits(x[6] * up, x[7] * up, h.w, l.w);
-            *reinterpret_cast<uint4 *>(dig + at) = h;
-            *reinterpret_cast<uint4 *>(keys + at) = h;
-            if (DIG == 2) { *reinterpret_cast<uint4 *>(dig + DC_KQ + at) = l; *reinterpret_cast<uint4 *>(keys + DC_KQ + at) = l; }
+            for (int e = 0; e < N; ++e) x[e] = to_f32(p[e]);
         };
-        put(kx[i], up_k, t);
-        put(qx[i], up_q, DC_T + t);
+        auto most_of = [&](uint4 (&r)[4][P], uint32_t (&bad)[2]) {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    float x[N];
+                    values(r[i][e], x);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(x[j])));
+                }
+            const bool out = __ballot_sync(0xffffffffu, !(most < INFINITY)) & (0x01010101u << (lane & 7u));
+            if (out && t < n && lane < 8u) atomicOr(&bad[t >> 5], 1u << (t & 31u));
+            if (out || t >= n) {
+                most = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < P; ++e) r[i][e] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            return dc_warp_max(most);
+        };
+        float mk = most_of(rk, s_bad[0]), mq = most_of(rq, s_bad[1]);
+        if (lane == 0u) { s_red[0][warp] = mk; s_red[1][warp] = mq; }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { mk = fmaxf(mk, s_red[0][i]); mq = fmaxf(mq, s_red[1][i]); }
+        float up_k, up_q;
+        dc_scale(mk, up_k, f_k);
+        dc_scale(mq, up_q, f_q);
+        auto put = [&](const uint4 (&r)[P], float up, uint32_t at) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                float x[N];
+                values(r[e], x);
+#pragma unroll
+                for (int j = 0; j < N; j += 2) dc_digits(x[j] * up, x[j + 1] * up, h[(e * N + j) / 2], l[(e * N + j) / 2]);
+            }
+            *reinterpret_cast<uint4 *>(sm + at) = *reinterpret_cast<const uint4 *>(h);
+            *reinterpret_cast<uint4 *>(keys + at) = *reinterpret_cast<const uint4 *>(h);
+            if (DIG == 2) { *reinterpret_cast<uint4 *>(sm + DC_KQ + at) = *reinterpret_cast<const uint4 *>(l); *reinterpret_cast<uint4 *>(keys + DC_KQ + at) = *reinterpret_cast<const uint4 *>(l); }
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            put(rk[i], up_k, dc_kq_at(t, (lane >> 3) + 4u * i));
+            put(rq[i], up_q, dc_kq_at(DC_T + t, (lane >> 3) + 4u * i));
+        }
+        __syncthreads();
     }
-    __syncthreads();
     // the keys transposed: 8 x 8 blocks turned by ldmatrix; warp: eight tokens, four blocks of eight columns at a time
 #pragma unroll
     for (uint32_t d = 0; d < (uint32_t)DIG; ++d)
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
             uint32_t x[4];
-            dc_ldsm_t(x, dc_smem(dig) + d * DC_KQ + dc_kq_at(warp * 8u + (lane & 7u), i * 4u + (lane >> 3)));
+            dc_ldsm_t(x, dc_smem(sm) + d * DC_KQ + dc_kq_at(warp * 8u + (lane & 7u), i * 4u + (lane >> 3)));
 #pragma unroll
             for (uint32_t j = 0; j < 4u; ++j)
                 *reinterpret_cast<uint32_t *>(keys + DIG * DC_KQ + d * DC_KT + dc_kq_at((i * 4u + j) * 8u + (lane >> 2), warp) + (lane & 3u) * 4u) = x[j];
         }
     // The decays of a value head, by one warp: tokens 2 lane and 2 lane + 1. The sums of the gates are kept as a float and what it lacks: differences of long sums are wanted to 2^-24 of themselves.
     auto decays = [&](uint32_t v) {
-        const uint32_t h = kh * width + v;
-        DcMeta *const meta = reinterpret_cast<DcMeta *>(ws + slots * A.groups * dc_keys(DIG) + (slot * A.rank + h) * DC_REC + 4u * DC_SQ);
+        DcMeta *const meta = reinterpret_cast<DcMeta *>(recs + (uint64_t)(kh * width + v) * DC_REC + 4u * DC_SQ);
         auto add = [](float2 x, float2 y) {      // (x.x + x.y) + (y.x + y.y)
             const float s = x.x + y.x, z = s - x.x, e = ((x.x - (s - z)) + (y.x - z)) + (x.y + y.y), r = s + e;
             return make_float2(r, e - (r - s));
@@ -226,14 +236,9 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t t = lane * 2u + i;
-            float gv = g_raw[i], bv = b_raw[i];
-            if (v >= 2u) {
-                gv = bv = 0.f;
-                if (t < n) { gv = A.gate[(uint64_t)(t0 + t) * A.rank + h]; bv = A.beta[(uint64_t)(t0 + t) * A.rank + h]; }
-            }
-            bad[i] = !(gv < INFINITY) || !(fabsf(bv) < INFINITY) || ((s_bad[0][t >> 5] >> (t & 31u)) & 1u);
-            gv = gv < -200.f ? -200.f : gv;      // exp is 0 from -104 on; -infinity cuts the past off
-            g[i] = make_float2(bad[i] ? 0.f : gv, 0.f); bt[i] = bad[i] ? 0.f : bv;
+            bad[i] = !(g_raw[i] < INFINITY) || !(fabsf(b_raw[i]) < INFINITY) || ((s_bad[0][t >> 5] >> (t & 31u)) & 1u);
+            g[i] = make_float2(bad[i] ? 0.f : g_raw[i] < -200.f ? -200.f : g_raw[i], 0.f);      // exp is 0 from -104 on; -infinity cuts the past off
+            bt[i] = bad[i] ? 0.f : b_raw[i];
         }
         g[1] = add(g[0], g[1]);
         float2 sum = g[1];
@@ -255,137 +260,144 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
         }
         *reinterpret_cast<float2 *>(&meta->dec[lane * 2u]) = make_float2(dec[0], dec[1]);
         *reinterpret_cast<float2 *>(&meta->kdec[lane * 2u]) = make_float2(kdec[0], kdec[1]);
-        const float most_dec = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(dec[0], dec[1]))));
+        const float most_dec = dc_warp_max(fmaxf(dec[0], dec[1]));
+        // the largest exp(G_t - G_s), s <= t: 1 unless a gate is positive
+        float low = fminf(G[0].x, G[1].x);
+        for (int w = 1; w < 32; w <<= 1) { const float x = __shfl_up_sync(0xffffffffu, low, w); if (lane >= (uint32_t)w) low = fminf(low, x); }
+        float ahead = __shfl_up_sync(0xffffffffu, low, 1);
+        if (lane == 0u) ahead = INFINITY;
+        const float rise = fmaxf(fmaxf(G[0].x - fminf(ahead, G[0].x), G[1].x - low), 0.f), peak = expf(dc_warp_max(rise));
         if (lane == 0u) {
+            s_peak[v & 1u] = peak;
             meta->last = expf(last.x + last.y); meta->f_k = f_k; meta->f_q = f_q; meta->most_dec = most_dec;
             meta->nan_from = min(first0, first1); meta->bad_q[0] = s_bad[1][0]; meta->bad_q[1] = s_bad[1][1];
         }
     };
-    {   // warps 0-3: K K^T, 4-7: Q K^T; 16 rows each, the columns up to the diagonal
-        const uint32_t mt = warp & 3u, which = warp >> 2, a_at = dc_smem(dig), b_at = a_at;
-        const uint32_t ar = which * DC_T + mt * 16u + (lane & 15u), ac = lane >> 4, br = (lane & 7u) + (lane >> 4) * 8u, bc = (lane >> 3) & 1u;
-        float c[4][2][4];
+    if (dv < width) decays(dv);
+    // warps 0-3: K K^T, rows 16 warp on; 4-7: Q K^T, rows 16 (7 - warp) on, so that every scheduler has as much; the columns up to the diagonal
+    const uint32_t which = warp >> 2, mt = which ? 7u - warp : warp, g = lane >> 2, c2 = (lane & 3u) * 2u;
+    float c[4][2][4];
+    {
+        const uint32_t at = dc_smem(sm), ar = which * DC_T + mt * 16u + (lane & 15u), ac = lane >> 4, br = (lane & 7u) + (lane >> 4) * 8u, bc = (lane >> 3) & 1u;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[i][j][e] = 0.f;
-#pragma unroll 4
+#pragma unroll 2
         for (uint32_t s = 0; s < 8u; ++s) {
             uint32_t ah[4], al[4];
-            dc_ldsm(ah, a_at + dc_kq_at(ar, 2u * s + ac));
-            if (DIG == 2) dc_ldsm(al, a_at + DC_KQ + dc_kq_at(ar, 2u * s + ac));
+            dc_ldsm(ah, at + dc_kq_at(ar, 2u * s + ac));
+            if (DIG == 2) dc_ldsm(al, at + DC_KQ + dc_kq_at(ar, 2u * s + ac));
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i)
                 if (i <= mt) {
                     uint32_t x[4];
-                    dc_ldsm(x, b_at + dc_kq_at(i * 16u + br, 2u * s + bc));
+                    dc_ldsm(x, at + dc_kq_at(i * 16u + br, 2u * s + bc));
                     dc_mma(c[i][0], ah, x[0], x[1]); dc_mma(c[i][1], ah, x[2], x[3]);
                     if (DIG == 2) {
                         dc_mma(c[i][0], al, x[0], x[1]); dc_mma(c[i][1], al, x[2], x[3]);
-                        dc_ldsm(x, b_at + DC_KQ + dc_kq_at(i * 16u + br, 2u * s + bc));
+                        dc_ldsm(x, at + DC_KQ + dc_kq_at(i * 16u + br, 2u * s + bc));
                         dc_mma(c[i][0], ah, x[0], x[1]); dc_mma(c[i][1], ah, x[2], x[3]);
                     }
                 }
         }
-        float *const to = which ? s_qk : s_kk;
-        const float f = which ? f_q : f_k;
-        const uint32_t g = lane >> 2, c2 = (lane & 3u) * 2u;
+        const float f = (which ? f_q : f_k) * f_k;
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i)
-            if (i <= mt)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (uint32_t j = 0; j < 2u; ++j) {
-                    float *p = to + (mt * 16u + g) * DC_PITCH + i * 16u + j * 8u + c2;
-                    *reinterpret_cast<float2 *>(p) = make_float2(c[i][j][0] * f * f_k, c[i][j][1] * f * f_k);
-                    *reinterpret_cast<float2 *>(p + 8u * DC_PITCH) = make_float2(c[i][j][2] * f * f_k, c[i][j][3] * f * f_k);
-                }
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[i][j][e] *= f;
     }
-    if (hw == 0u && half < width) decays(half);      // the warps with the fewest products
-    __syncthreads();
-    float *const s_a = reinterpret_cast<float *>(dig + half * 2u * DC_MAT), *const s_t = s_a + DC_T * DC_PITCH;
-    float2 *const s_m = s_max[half];
-    for (uint32_t v = half; v < width; v += 2u) {
-        const uint32_t h = kh * width + v;
-        uint8_t *const rec = ws + slots * A.groups * dc_keys(DIG) + (slot * A.rank + h) * DC_REC;
-        DcMeta *const meta = reinterpret_cast<DcMeta *>(rec + 4u * DC_SQ);
-        if (v >= 2u && hw == 0u) decays(v);      // of the first two: ahead of the barrier above
-        dc_half_sync(half);
-        // A below the diagonal; P and its digits: pieces of eight columns, four a thread, whose tokens run along the lanes
-        float p[4][8], most = 0.f, most_a = 0.f;
+    const uint32_t half = warp >> 2, hw = warp & 3u;         // for the inverse, half a block has a value head
+    float *const s_a = reinterpret_cast<float *>(sm + half * 2u * DC_MAT), *const s_t = s_a + DC_T * DC_PITCH;
+    float most_c = 0.f;                          // of the warp's products
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t t = ht & 63u, s0 = (2u * i + (ht >> 6)) * 8u;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[i][j] = 0.f;
-            if (s0 > (t | 31u)) continue;        // the whole warp's tokens lie before the piece
-            const float bt = s_beta[half][t];
-            const float2 Gt = s_cum[half][t];
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                const float4 qk = *reinterpret_cast<const float4 *>(s_qk + t * DC_PITCH + s0 + j), kk = *reinterpret_cast<const float4 *>(s_kk + t * DC_PITCH + s0 + j);
-                const float qv[4] = {qk.x, qk.y, qk.z, qk.w}, kv[4] = {kk.x, kk.y, kk.z, kk.w};
-                float a[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t s = s0 + j + e;
-                    const float2 Gs = s_cum[half][s];
-                    const float ratio = dc_exp((Gt.x - Gs.x) + (Gt.y - Gs.y));
-                    p[i][j + e] = s <= t ? qv[e] * ratio : 0.f;
-                    a[e] = s < t ? bt * kv[e] * ratio : 0.f;
-                    most = fmaxf(most, fabsf(p[i][j + e])); most_a = fmaxf(most_a, fabsf(a[e]));
-                }
-                *reinterpret_cast<float4 *>(s_a + t * DC_PITCH + s0 + j) = make_float4(a[0], a[1], a[2], a[3]);
-            }
+            for (int e = 0; e < 4; ++e) most_c = fmaxf(most_c, fabsf(c[i][j][e]));
+    most_c = dc_warp_max(most_c);
+    uint32_t v0 = 0u;
+    do {
+        if (WIDE && v0) {
+            __syncthreads();                     // the matrices and decays of the last two have been read
+            if (v0 + dv < width && dv < 2u) { gates(v0 + dv); decays(v0 + dv); }
         }
-        for (int w = 16; w; w >>= 1) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w)); most_a = fmaxf(most_a, __shfl_xor_sync(0xffffffffu, most_a, w)); }
-        if (lane == 0u) s_m[hw] = make_float2(most, most_a);
-        dc_half_sync(half);
+        __syncthreads();                         // the digits have been read; the decays are there
+#pragma unroll 1
+        for (uint32_t v = v0; v < v0 + 2u && v < width; ++v) {
+            const uint32_t o = v & 1u, t = mt * 16u + g;     // rows t and t + 8
+            const float2 G0 = s_cum[o][t], G1 = s_cum[o][t + 8u];
+            const float b0 = which ? 1.f : s_beta[o][t], b1 = which ? 1.f : s_beta[o][t + 8u];
+            uint8_t *const rec = recs + (uint64_t)(kh * width + v) * DC_REC;
+            float *const s_to = reinterpret_cast<float *>(sm + o * 2u * DC_MAT) + t * DC_PITCH + c2;
+            float up, unit, most = 0.f;
+            dc_scale(fminf(most_c * s_peak[o], 3e38f), up, unit);        // of P, from its bound
+            if (which && lane == 0u) reinterpret_cast<DcMeta *>(rec + 4u * DC_SQ)->f_p[mt] = unit;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { most = fmaxf(most, s_m[i].x); most_a = fmaxf(most_a, s_m[i].y); }
-        float up, unit, up_a, unit_a;
-        dc_scale(most, up, unit);
-        dc_scale(most_a, up_a, unit_a);
-        if (ht == 0u) meta->f_p = unit;
-        auto put = [&](const float (&x)[8], float f, uint32_t t, uint32_t piece, uint8_t *to) {
-            uint4 h, l;
-            dc_digits(x[0] * f, x[1] * f, h.x, l.x); dc_digits(x[2] * f, x[3] * f, h.y, l.y);
-            dc_digits(x[4] * f, x[5] * f, h.z, l.z); dc_digits(x[6] * f, x[7] * f, h.w, l.w);
-            *reinterpret_cast<uint4 *>(to + dc_sq_at(t, piece)) = h;
-            *reinterpret_cast<uint4 *>(to + DC_SQ + dc_sq_at(t, piece)) = l;
-        };
+            for (uint32_t i = 0; i < 4u; ++i)
+                if (i <= mt)
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) put(p[i], up, ht & 63u, 2u * i + (ht >> 6), rec + 2u * DC_SQ);
+                    for (uint32_t j = 0; j < 2u; ++j) {
+                        float y[4];
+#pragma unroll
+                        for (uint32_t e = 0; e < 2u; ++e) {
+                            const uint32_t s = i * 16u + j * 8u + c2 + e;
+                            const float2 Gs = s_cum[o][s];
+                            const float x0 = b0 * c[i][j][e] * dc_exp((G0.x - Gs.x) + (G0.y - Gs.y)), x1 = b1 * c[i][j][e + 2] * dc_exp((G1.x - Gs.x) + (G1.y - Gs.y));
+                            y[e] = s < t + which ? x0 : 0.f;             // s < t for A, s <= t for P
+                            y[e + 2] = s < t + 8u + which ? x1 : 0.f;
+                        }
+                        if (which) {             // P
+#pragma unroll
+                            for (uint32_t r = 0; r < 2u; ++r) {
+                                uint32_t h, l;
+                                dc_digits(y[2u * r] * up, y[2u * r + 1u] * up, h, l);
+                                uint8_t *const to = rec + 2u * DC_SQ + dc_sq_at(t + 8u * r, i * 2u + j) + c2 * 2u;
+                                *reinterpret_cast<uint32_t *>(to) = h;
+                                *reinterpret_cast<uint32_t *>(to + DC_SQ) = l;
+                            }
+                        } else {
+                            *reinterpret_cast<float2 *>(s_to + i * 16u + j * 8u) = make_float2(y[0], y[1]);
+                            *reinterpret_cast<float2 *>(s_to + 8u * DC_PITCH + i * 16u + j * 8u) = make_float2(y[2], y[3]);
+                            most = fmaxf(fmaxf(fmaxf(most, fabsf(y[0])), fmaxf(fabsf(y[1]), fabsf(y[2]))), fabsf(y[3]));
+                        }
+                    }
+            most = dc_warp_max(most);
+            if (!which && lane == 0u) s_amax[o][mt] = most;
+        }
+        __syncthreads();
+        if (v0 + half >= width) { v0 += 2u; continue; }
+        uint8_t *const rec = recs + (uint64_t)(kh * width + v0 + half) * DC_REC;
         // the diagonal blocks of the inverse: warp hw has block hw, lane c column c
         {
-            const uint32_t o = hw * 16u, c = lane & 15u;
-            float x[16];
+            const uint32_t o = hw * 16u, col = lane & 15u;
+            float x[16], most_t = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float e = (uint32_t)r == c ? 1.f : 0.f;
+                float e = (uint32_t)r == col ? 1.f : 0.f;
 #pragma unroll
                 for (int k = 0; k < r; ++k) e = fmaf(-s_a[(o + r) * DC_PITCH + o + k], x[k], e);
                 x[r] = e;
+                most_t = fmaxf(most_t, fabsf(e));
             }
-            float most_t = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) most_t = fmaxf(most_t, fabsf(x[r]));
             if (lane < 16u)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s_t[(o + r) * DC_PITCH + o + c] = x[r];
-            most_t = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_t)));
-            if (lane == 0u) s_d[half][hw] = most_t;
+                for (int r = 0; r < 16; ++r) s_t[(o + r) * DC_PITCH + o + col] = x[r];
+            most_t = dc_warp_max(most_t);
+            if (lane == 0u) s_diag[half][hw] = most_t;
         }
         dc_half_sync(half);
         // The others, a column of blocks a warp: X_i = T_ij^T = -(sum_{k < i} X_k A_ik^T) T_ii^T. Transposed, an accumulator is the next product's operand A and rows of A and T_ii are operand B.
         {
-            float up_t, unit_t;
-            float diag = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) diag = fmaxf(diag, s_d[half][i]);
-            dc_scale(diag, up_t, unit_t);
-            const uint32_t j = hw, g = lane >> 2, c2 = (lane & 3u) * 2u;
+            float up_t, unit_t, up_a, unit_a;
+            dc_scale(fmaxf(fmaxf(s_diag[half][0], s_diag[half][1]), fmaxf(s_diag[half][2], s_diag[half][3])), up_t, unit_t);
+            dc_scale(fmaxf(fmaxf(s_amax[half][0], s_amax[half][1]), fmaxf(s_amax[half][2], s_amax[half][3])), up_a, unit_a);
+            const uint32_t j = hw;
             uint32_t xh[3][4], xl[3][4];
             float f[3], x[2][4];
 #pragma unroll
@@ -432,32 +444,36 @@ __global__ void __launch_bounds__(256, 2) k_delta_prep(DeltaArgs A, uint32_t n_s
             }
         }
         dc_half_sync(half);
-        most = 0.f;
+        // T with its columns' betas: warp hw has 16 rows, a lane every other piece of eight columns of one
+        {
+            const uint32_t t = hw * 16u + (lane & 15u), p0 = lane >> 4;
+            float y[4][8], most = 0.f, up, unit;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t t = ht & 63u, s0 = (2u * i + (ht >> 6)) * 8u;
+            for (uint32_t i = 0; i < 4u; ++i)
+                if (i <= hw)
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                const float4 y = *reinterpret_cast<const float4 *>(s_t + t * DC_PITCH + s0 + j);
-                const float v4[4] = {y.x, y.y, y.z, y.w};
+                    for (uint32_t e = 0; e < 8u; e += 4u) {
+                        const uint32_t s = (p0 + 2u * i) * 8u + e;
+                        const float4 x = *reinterpret_cast<const float4 *>(s_t + t * DC_PITCH + s), bt = *reinterpret_cast<const float4 *>(&s_beta[half][s]);
+                        y[i][e] = s <= t ? x.x * bt.x : 0.f; y[i][e + 1] = s + 1u <= t ? x.y * bt.y : 0.f;
+                        y[i][e + 2] = s + 2u <= t ? x.z * bt.z : 0.f; y[i][e + 3] = s + 3u <= t ? x.w * bt.w : 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t s = s0 + j + e;
-                    p[i][j + e] = s <= t ? v4[e] * s_beta[half][s] : 0.f;
-                    most = fmaxf(most, fabsf(p[i][j + e]));
+                        for (uint32_t a = 0; a < 4u; ++a) most = fmaxf(most, fabsf(y[i][e + a]));
+                    }
+            dc_scale(dc_warp_max(most), up, unit);
+            if (lane == 0u) reinterpret_cast<DcMeta *>(rec + 4u * DC_SQ)->f_t[hw] = unit;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i)
+                if (i <= hw) {
+                    uint4 h, l;
+                    dc_digits(y[i][0] * up, y[i][1] * up, h.x, l.x); dc_digits(y[i][2] * up, y[i][3] * up, h.y, l.y);
+                    dc_digits(y[i][4] * up, y[i][5] * up, h.z, l.z); dc_digits(y[i][6] * up, y[i][7] * up, h.w, l.w);
+                    *reinterpret_cast<uint4 *>(rec + dc_sq_at(t, p0 + 2u * i)) = h;
+                    *reinterpret_cast<uint4 *>(rec + DC_SQ + dc_sq_at(t, p0 + 2u * i)) = l;
                 }
-            }
         }
-        for (int w = 16; w; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
-        if (lane == 0u) s_d[half][hw] = most;
-        dc_half_sync(half);
-        most = fmaxf(fmaxf(s_d[half][0], s_d[half][1]), fmaxf(s_d[half][2], s_d[half][3]));
-        dc_scale(most, up, unit);
-        if (ht == 0u) meta->f_t = unit;
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) put(p[i], up, ht & 63u, 2u * i + (ht >> 6), rec);
-        dc_half_sync(half);
-    }
+        v0 += 2u;
+    } while (WIDE && v0 < width);
 }
 
 // ---- the states through their chunks -------------------------------------------------------------------------------------------------------------
@@ -783,10 +799,10 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             load32(x, DT_M2 + hf * 32u);
             float f4, most_d = 0.f, most_dk = 0.f;
             {
-                const float f = unit * M.f_t;
+                const float f[2] = {unit * M.f_t[2u * hf], unit * M.f_t[2u * hf + 1u]};
 #pragma unroll
                 for (uint32_t i = 0; i < 32u; ++i) {
-                    x[i] *= f; r[i] = x[i] * M.kdec[hf * 32u + i];
+                    x[i] *= f[i >> 4]; r[i] = x[i] * M.kdec[hf * 32u + i];
                     most_d = fmaxf(most_d, fabsf(x[i])); most_dk = fmaxf(most_dk, fabsf(r[i]));
                 }
                 s_ex[3][hf][j] = most_d;
@@ -799,7 +815,6 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
                 dc_scale(most_d, up, unit);
                 dc_put32(x, up, mine + DT_D + hf * 16u, mine + DT_D + 32u + hf * 16u);
                 dc_hand_over(bar(DB_D));
-                unit *= M.f_p;                   // of M3's result
                 f4 *= M.f_k;                     // of M4's
             }
             const float last = M.last;
@@ -822,9 +837,9 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             load32(x, DT_M3 + hf * 32u);
             const uint32_t bad_q = M.bad_q[hf];
-            unit *= A.scale;
+            const float f3[2] = {unit * A.scale * M.f_p[2u * hf], unit * A.scale * M.f_p[2u * hf + 1u]};
 #pragma unroll
-            for (uint32_t i = 0; i < 32u; ++i) x[i] = fmaf(x[i], unit, A.scale * o[i]);
+            for (uint32_t i = 0; i < 32u; ++i) x[i] = fmaf(x[i], f3[i >> 4], A.scale * o[i]);
             if (bad_q || from < (uint32_t)DC_T)
 #pragma unroll
                 for (uint32_t i = 0; i < 32u; ++i) if (((bad_q >> i) & 1u) || hf * 32u + i >= from) x[i] = NAN;
@@ -866,13 +881,18 @@ template <class T, int DIG> static int launch_chunk(DeltaArgs A, uint32_t n_seqs
 }
 template <class T, int DIG> static int launch_chunks(const DeltaArgs &A, uint32_t n_seqs, uint8_t *ws, cudaStream_t s) {
     const uint64_t slots = dc_slots(A.n_tokens, n_seqs);
-    constexpr uint32_t region = 4u * DC_MAT > DIG * DC_KQ ? 4u * DC_MAT : DIG * DC_KQ;
-    constexpr size_t smem = 2u * DC_MAT + region;
-    static std::atomic<uint64_t> set{0};
-    if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_prep<T, DIG>), smem, set)) return 0;
+    constexpr size_t smem = 4u * DC_MAT > DIG * DC_KQ ? 4u * DC_MAT : DIG * DC_KQ;
     RC_REQUIRE(slots <= 0x7fffffffu && A.groups <= 65535u, "delta rule: too many chunks");
     prof_begin("delta_prep", s);
-    RC_LAUNCH((k_delta_prep<T, DIG>), dim3((uint32_t)slots, A.groups), 256, smem, s, A, n_seqs, ws, slots);
+    if (A.rank > 2u * A.groups) {
+        static std::atomic<uint64_t> set{0};
+        if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_prep<T, DIG, true>), smem, set)) return 0;
+        RC_LAUNCH((k_delta_prep<T, DIG, true>), dim3((uint32_t)slots, A.groups), 256, smem, s, A, n_seqs, ws, slots);
+    } else {
+        static std::atomic<uint64_t> set{0};
+        if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_prep<T, DIG, false>), smem, set)) return 0;
+        RC_LAUNCH((k_delta_prep<T, DIG, false>), dim3((uint32_t)slots, A.groups), 256, smem, s, A, n_seqs, ws, slots);
+    }
     RC_LAUNCHED();
     prof_end(s);
     prof_begin("delta_chunk", s);
