@@ -105,13 +105,15 @@ template <class T> __device__ __forceinline__ float lp_most(uint4 w) {
     }
 }
 
-// What bounds it is the row's bytes, if a value takes no more than the seven instructions it has here (of which one is an exponential, a
-// sixteenth of the fp32 rate). The alternatives therefore cost one comparison a lane and round of LP_UNROLL pieces: a warp keeps its 32 largest keys, one a
+// What bounds it is the row's bytes for 32-bit logits (592 rows of 151936: 56 us, 6.4 TB/s) and instructions for 16-bit ones (seven a value, one of them an exponential at a
+// sixteenth of the fp32 rate: 777 rows 50 us, 4.8 TB/s). A round's loads are on their way while the last one's values are added up; four blocks an SM for 32 bits, three for 16, which spill with four
+// (777 rows 65 us).
+// The alternatives cost one comparison a lane and round of LP_UNROLL pieces where there are none: a warp keeps its 32 largest keys, one a
 // lane, and looks at single values only where the largest of a lane's round reaches what is known to be among the row's n largest. That is the n-th of the warp's own,
 // or the least of the warps' ceil(n / LP_WARPS)-th largest, which every warp publishes (n values are at least that large; a stale one is a lower bound too), or in a warp's first
-// round the n-th of its lanes' largest.
+// round the n-th of its lanes' largest. 777 rows of BF16 with 5, 20 alternatives: 74, 87 us.
 template <class T>
-__global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs A) {
+__global__ void __launch_bounds__(LP_WARPS * 32, sizeof(T) == 4 ? 4 : 3) k_token_logprobs(LogprobArgs A) {
     pdl_prologue();
     constexpr int VEC = 16 / sizeof(T), U = LP_UNROLL;
     constexpr float LOG2E = 1.44269504088896340736f;
@@ -159,17 +161,24 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
         m = to;
     };
     bool fresh = true;
-    for (uint32_t p = p0 + warp * (32u * U); p < p1; p += LP_WARPS * 32u * U) {
+    uint4 ahead[U];                              // the next round's pieces
+    auto load = [&](uint32_t p) {
         const uint4 *const at = reinterpret_cast<const uint4 *>(x + head) + p + lane;
-        uint4 w[U];
         if (p + 32u * U <= p1) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) w[u] = at[u * 32];
+            for (int u = 0; u < U; ++u) ahead[u] = at[u * 32];
         } else {
             const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;       // -infinity
 #pragma unroll
-            for (int u = 0; u < U; ++u) w[u] = p + u * 32u + lane < p1 ? at[u * 32] : make_uint4(low, low, low, low);
+            for (int u = 0; u < U; ++u) ahead[u] = p + u * 32u + lane < p1 ? at[u * 32] : make_uint4(low, low, low, low);
         }
+    };
+    load(p0 + warp * (32u * U));
+    for (uint32_t p = p0 + warp * (32u * U); p < p1; p += LP_WARPS * 32u * U) {
+        uint4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = ahead[u];
+        load(p + LP_WARPS * 32u * U);
         float top[U], most = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) { top[u] = lp_most<T>(w[u]); most = fmaxf(most, top[u]); }
@@ -314,6 +323,8 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(LogprobArgs
 template <class T> static int launch_logprobs(const LogprobArgs &A, uint32_t rows, cudaStream_t s) {
     const uint32_t sms = sm_count();
     uint32_t parts = 1u;
+    // Blocks of a row: until there are two for every SM. Twice as many change nothing for up to 36 rows (24 us for 36 of 152064 F16 logits), 145 rows of F32 take 35 -> 41 us; eight times
+    // as many 777 rows of BF16 101 -> 140: a block's end costs some 4 us.
     while (parts < (uint32_t)LP_CLUSTER && (uint64_t)rows * parts < 2u * sms && A.vocab / parts > 4096u) parts *= 2u;
     prof_begin("token_logprobs", s);
     for (uint64_t r = 0; r < rows; r += 1u << 24) {

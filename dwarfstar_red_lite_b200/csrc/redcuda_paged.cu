@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend(AttendAr
 template <class QT, int HD>
 __global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
     pdl_prologue();
-    constexpr uint32_t COLS = HD / 4, ROWS = 256u / COLS, AHEAD = 4u;
+    constexpr uint32_t COLS = HD / 4, ROWS = 256u / COLS, AHEAD = 8u;
     extern __shared__ float s_w[];               // a weight for every part
     __shared__ float s_max[8], s_sum[8];
     __shared__ __align__(16) float s_o[ROWS][HD];
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
 #pragma unroll
     for (uint32_t i = 0; i < AHEAD; ++i)
         if (row + i * ROWS <= n) add(s_w[row + i * ROWS], x[i]);
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t p = row + AHEAD * ROWS; p <= n; p += ROWS) add(s_w[p], part(p));
     *reinterpret_cast<float4 *>(&s_o[row][col * 4u]) = o;
     __syncthreads();
