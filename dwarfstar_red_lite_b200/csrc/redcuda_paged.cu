@@ -3,14 +3,18 @@
 //   k_kv_append     a warp per token: its K and V rows, converted, to the page that the table names
 //   k_kv_attend     decode attention over the sequences' whole lengths (below)
 //   k_kv_attend_join  sums the parts of sequences that several blocks worked on
+//   k_kv_attend_cluster  the same for few heads of moderate length, in one launch
 #include "redcuda_paged.cuh"
 #include "redcuda_stage.cuh"
 #include "../../include/redcuda.h"
 
+#include <cooperative_groups.h>
 #include <math.h>
 #include <type_traits>
 
 namespace rc {
+
+namespace cg = cooperative_groups;
 
 struct AppendArgs {
     void *k, *v;
@@ -611,10 +615,93 @@ __global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
     if (tid == 0u && A.lse) A.lse[(uint64_t)b * A.n_q + head] = kv_lse(M, l);
 }
 
+// ---- few heads of moderate length: one launch -----------------------------------------------------------------------------------------
+// A cluster of eight blocks has a head, an eighth of its tiles each; their parts meet in shared memory, block r sums up query head r. What bounds it is the chain of reads; its figures stand at the rule (KV_CLUSTER_HEADS).
+template <class T, class QT, int HD, int NH>
+__global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend_cluster(AttendArgs A) {
+    pdl_prologue();
+    using L = KvTile<T, HD>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint64_t s_valid[KV_WARPS][KV_STAGES];
+    __shared__ __align__(16) float s_p[sizeof(T) == 4 ? KV_WARPS : 1][40], s_m[KV_WARPS][8], s_l[KV_WARPS][8], s_part[2][8];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, rank = cluster.block_rank(), HG = A.n_kv * A.gsplit, b = blockIdx.x / KV_CLUSTER / HG, hg = blockIdx.x / KV_CLUSTER % HG;
+    const uint32_t kvh = hg / A.gsplit, g0 = (hg % A.gsplit) * 8u, h0 = kvh * A.G + g0, nh = min(8u, A.G - g0);
+    const uint32_t len = kv_len(A, b), nt = (len + L::TP - 1u) / L::TP, t0 = nt * rank / KV_CLUSTER, t1 = nt * (rank + 1u) / KV_CLUSTER;
+    QT *const out = reinterpret_cast<QT *>(A.out) + ((uint64_t)b * A.n_q + h0) * HD;
+    if (A.status && tid == 0u && rank == 0u && A.lens[b] > 0 && (uint32_t)A.lens[b] != len) A.status[ST_PAGE_RANGE] = 1u;
+    if (len == 0u) {                             // nothing to attend to, for the whole cluster
+        if (rank < nh) for (uint32_t i = tid; i < (uint32_t)HD; i += KV_WARPS * 32u) out[rank * HD + i] = from_f32<QT>(0.f);
+        if (rank < nh && A.lse && tid == 0u) A.lse[(uint64_t)b * A.n_q + h0 + rank] = -INFINITY;
+        return;
+    }
+    if (A.k_new && rank == KV_CLUSTER - 1u && len == (uint32_t)A.lens[b]) kv_write_new<T, QT, HD>(A, b, kvh, len - 1u);       // the last block has the last tile
+    __syncthreads();
+    float *o_sh = reinterpret_cast<float *>(sm);
+    uint8_t *ring = sm + warp * KV_STAGES * L::BYTES;
+    if constexpr (sizeof(T) == 4)
+        attend_part_f32<T, QT, HD, NH>(A, b, kvh, h0, nh, len, t0, t1, ring, s_valid[warp], s_p[sizeof(T) == 4 ? warp : 0], s_m[warp], s_l[warp], o_sh + warp * 8u * HD);
+    else
+        attend_part_mma<T, QT, HD>(A, b, kvh, h0, nh, len, t0, t1, ring, s_valid[warp], s_m[warp], s_l[warp], o_sh + warp * 8u * HD);
+    __syncthreads();
+    if (tid < 8u) {
+        float M = s_m[0][tid], lt = 0.f;
+#pragma unroll
+        for (uint32_t j = 1; j < KV_WARPS; ++j) M = fmaxf(M, s_m[j][tid]);
+        const float z = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (uint32_t j = 0; j < KV_WARPS; ++j) { const float w = exp2f(s_m[j][tid] - z); lt += w * s_l[j][tid]; s_m[j][tid] = w; }
+        s_part[0][tid] = M; s_part[1][tid] = lt;
+    }
+    __syncthreads();
+    for (uint32_t i = tid * 4u; i < (uint32_t)NH * HD; i += KV_WARPS * 128u) {
+        const uint32_t h = i / HD;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t j = 0; j < KV_WARPS; ++j) {
+            const float4 y = *reinterpret_cast<const float4 *>(o_sh + j * 8u * HD + i);
+            const float w = s_m[j][h];
+            x.x += w * y.x; x.y += w * y.y; x.z += w * y.z; x.w += w * y.w;
+        }
+        *reinterpret_cast<float4 *>(o_sh + i) = x;           // over the first warp's, which this thread alone reads
+    }
+    cluster.sync();
+    if (rank < nh) {
+        float M = -INFINITY, lt = 0.f, w[KV_CLUSTER];
+#pragma unroll
+        for (uint32_t r = 0; r < KV_CLUSTER; ++r) { w[r] = cluster.map_shared_rank(s_part[0], r)[rank]; M = fmaxf(M, w[r]); }
+        const float z = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (uint32_t r = 0; r < KV_CLUSTER; ++r) { w[r] = exp2f(w[r] - z); lt += w[r] * cluster.map_shared_rank(s_part[1], r)[rank]; }
+        for (uint32_t i = tid * 4u; i < (uint32_t)HD; i += KV_WARPS * 128u) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t r = 0; r < KV_CLUSTER; ++r) {
+                const float4 y = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(o_sh, r) + rank * HD + i);
+                x[0] += w[r] * y.x; x[1] += w[r] * y.y; x[2] += w[r] * y.z; x[3] += w[r] * y.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = lt == 0.f ? 0.f : x[e] / lt;
+            store_vals<4>(out + rank * HD + i, x);
+        }
+        if (A.lse && tid == 0u) A.lse[(uint64_t)b * A.n_q + h0 + rank] = kv_lse(M, lt);
+    }
+    cluster.sync();                              // the others have read this block's shared memory
+}
+
 template <class T, class QT, int HD, int NH> static int launch_attend(const AttendArgs &A, uint32_t blocks, cudaStream_t s) {
     constexpr size_t smem = (size_t)KV_WARPS * KV_STAGES * KvTile<T, HD>::BYTES;
     static std::atomic<uint64_t> set{0};
     if (!raise_smem_limit(reinterpret_cast<const void *>(k_kv_attend<T, QT, HD, NH>), smem, set)) return 0;
+    if (A.clusters) {
+        static std::atomic<uint64_t> set_cluster{0};
+        if (!raise_smem_limit(reinterpret_cast<const void *>(k_kv_attend_cluster<T, QT, HD, NH>), smem, set_cluster)) return 0;
+        prof_begin("kv_attend", s);
+        RC_LAUNCH_CLUSTER(KV_CLUSTER, (k_kv_attend_cluster<T, QT, HD, NH>), A.clusters * KV_CLUSTER, KV_WARPS * 32, smem, s, A);
+        RC_LAUNCHED();
+        prof_end(s);
+        return 1;
+    }
     prof_begin("kv_attend", s);
     RC_LAUNCH((k_kv_attend<T, QT, HD, NH>), blocks, KV_WARPS * 32, smem, s, A);
     RC_LAUNCHED();
@@ -743,6 +830,10 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     auto few = [](uint64_t n) { return n < 8192u ? n : 8192u; };      // more than that of one thing is blocks enough
     const uint64_t runs = (few(tiles) * few(n_seqs) * few(A.n_kv * A.gsplit) + KV_MIN_TILES - 1u) / KV_MIN_TILES;
     const uint32_t blocks = runs < sms * KV_BLOCKS ? (uint32_t)runs : sms * KV_BLOCKS;
+    // one launch for few heads of moderate length
+    const uint64_t heads = (uint64_t)n_seqs * A.n_kv * A.gsplit;
+    const uint64_t most_tiles = (uint64_t)KV_CLUSTER * KV_WARPS * (kv->type == VT_F32 ? KV_CLUSTER_TILES_F32 : KV_CLUSTER_TILES);
+    A.clusters = heads <= KV_CLUSTER_HEADS && heads * KV_CLUSTER <= (uint64_t)sms * KV_BLOCKS && tiles <= most_tiles ? (uint32_t)heads : 0u;
     A.meta = (uint32_t *)workspace_dev;
     A.part = (float *)(A.meta + (size_t)blocks * 4u);
     A.part_ml = A.part + (size_t)blocks * 2u * 8u * hd;

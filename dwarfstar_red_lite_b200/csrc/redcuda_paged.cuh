@@ -11,6 +11,11 @@ constexpr int KV_WARPS = 3, KV_STAGES = 2, KV_BLOCKS = 2;
 constexpr uint32_t KV_HEAD_COST = 12u;           // what a head's begin and end take, in tiles
 constexpr uint32_t KV_MIN_TILES = 3u;            // tiles that a block takes at least: one a warp
 
+// A cluster of blocks a head: how many blocks, for how many heads at most, and up to how many tiles a warp can have (by the page table's width) for 16-bit caches and caches of floats. us, dealt out -> in clusters:
+// F16, 2 K/V heads of 256: 1 sequence of 50 positions 10.5 -> 7.8, of 613 11.1 -> 9.3, of 1500 12.5 -> 11.7; 4 of 613 12.9 -> 9.9; 9 of 613 14.2 -> 11.0; 18 of 300 15.1 -> 15.8. BF16, 8 of 128: 1 of 613 9.7 -> 6.0,
+// 4 of 613 10.8 -> 6.8. F32, 2 of 256: 1 of 200 12.4 -> 9.9, of 613 11.6 -> 13.6; 4 of 100 12.8 -> 7.8.
+constexpr uint32_t KV_CLUSTER = 8u, KV_CLUSTER_HEADS = 32u, KV_CLUSTER_TILES = 4u, KV_CLUSTER_TILES_F32 = 2u;
+
 struct AttendArgs {
     void *k, *v;
     uint64_t page_stride, token_stride, head_stride;     // in elements
@@ -21,6 +26,7 @@ struct AttendArgs {
     float *lse, *part, *part_ml;
     uint32_t *meta, *status;
     uint32_t table_width, page_size, n_pages, n_seqs, n_kv, n_q, G, gsplit;     // G: query heads of a K/V head, in gsplit groups of 8
+    uint32_t clusters;                                   // heads, where each has a cluster of blocks; 0: the form that deals tiles out
     float scale_log2;
 };
 

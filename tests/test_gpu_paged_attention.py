@@ -130,9 +130,25 @@ def test_splits(qt, cache, lens):
 
 
 @pytest.mark.parametrize("qt, cache", PAIRS)
-def test_new_rows(qt, cache):
+@pytest.mark.parametrize("n_q, n_kv, hd", [(16, 2, 256), (8, 8, 64), (5, 1, 128), (12, 1, 64)])
+def test_few_heads(qt, cache, n_q, n_kv, hd):
+    """A sequence or a few of every length up to some hundred, in the form for few heads and, by a wide page table, in the other: the same within the tolerance."""
+    g = _gen(n_q)
+    for lens in ([1], [7], [16], [0], [23], [130], [257], [600], [3, 0, 190], [64, 65, 63]):
+        c = Cache(g, cache, n_kv, hd, 16, lens)
+        q = _q(g, len(lens), n_q, hd, qt)
+        _check(c, q, lens, n_q, *_attend(c, q, lens, n_q, qt))
+        wide = torch.full((len(lens), 4000), -1, dtype=torch.int32, device="cuda")
+        wide[:, :c.width] = c.table
+        c.table, c.width = wide, 4000
+        _check(c, q, lens, n_q, *_attend(c, q, lens, n_q, qt))
+    rc.device_status()
+
+
+@pytest.mark.parametrize("qt, cache", PAIRS)
+@pytest.mark.parametrize("lens", [[1, 16, 17, 0, 700, 33, 64], [1, 16, 17, 0, 300, 33, 64], [33], [4000, 2]])
+def test_new_rows(qt, cache, lens):
     """The new rows are written to the last position and attended to; nothing else of the cache changes."""
-    lens = [1, 16, 17, 0, 700, 33, 64]
     g = _gen(3)
     c = Cache(g, cache, 2, 256, 16, lens)
     dt = TYPES[qt][1]
