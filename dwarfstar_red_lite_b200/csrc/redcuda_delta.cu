@@ -1,8 +1,8 @@
 // The gated delta rule by itself, for a batch of sequences with states in slots (the recurrence of native/redlite_native_engine_cpu.c:198-216):
 //     S <- exp(g) S;   d = beta (v - S k);   S <- S + d k^T;   out = scale S q
 //
-//   k_delta_step  one token of each sequence
-//   k_delta_scan  whole sequences laid end to end, a token at a time
+//   k_delta_scan  one token of each sequence (STEP), or whole sequences laid end to end, a token at a time
+//   k_delta_prep, k_delta_chunk (redcuda_delta_chunk.cu)  whole sequences in chunks on the tensor cores
 #include "redcuda_delta.cuh"
 #include "redcuda_stage.cuh"
 #include "../../include/redcuda.h"
@@ -43,6 +43,8 @@ __device__ __forceinline__ float row_sums(float (&x)[N], uint32_t p) {
 //     S k = a (m . k),  S q = a (m . q) + d (k . q),  a = exp(g),
 // so that both products of a row are summed over its lanes in one exchange.
 // STEP: one token per sequence, token b; otherwise the tokens cu[b] .. cu[b + 1] - 1.
+// What bounds the step is the state, read once and written once: 96 sequences of 32 heads x 128 x 128 (403 MB) take 62 us, 6.5 TB/s; one sequence 2.3 us, a launch. Blocks of 32 rows, so that one
+// sequence is 128 of them. What bounds the scan is the chain of a token (two products, an exchange, the correction): some 0.29 us a token for F32 rows, 0.42 for 16 bits.
 template <class T, int S, bool STEP>
 __global__ void __launch_bounds__(DELTA_WARPS * 32) k_delta_scan(DeltaArgs A) {
     pdl_prologue();
@@ -132,9 +134,10 @@ template <bool STEP> static int launch_scan_t(const DeltaArgs &A, uint32_t type,
     return type == VT_F32 ? launch_scan_s<float, STEP>(A, S, n_seqs, s) : type == VT_F16 ? launch_scan_s<__half, STEP>(A, S, n_seqs, s) : launch_scan_s<__nv_bfloat16, STEP>(A, S, n_seqs, s);
 }
 
-// In chunks on the tensor cores, or a token at a time: a chunk costs the same whatever it holds, and the first one of a call 20 us. us with 32 heads, a token at a time -> in chunks, F32 (BF16):
-// 1 sequence of 32 tokens 12 -> 27 (16 -> 23), of 64 21 -> 30 (30 -> 24), of 128 40 -> 33 (58 -> 28); 16 of 16 43 -> 76 (49 -> 67), of 32 79 -> 79 (92 -> 68), of 64 161 -> 86 (177 -> 71); 64 of 32 316 -> 304 (371 -> 264).
-static bool delta_in_chunks(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs) { return d->d_state == 128u && n_tokens >= 32u * (uint64_t)n_seqs + 32u; }
+// In chunks on the tensor cores, or a token at a time: a chunk costs nearly the same whatever it holds, and the first one of a call 20 us. us with 32 heads, a token at a time -> in chunks, F32 (BF16):
+// 1 sequence of 32 tokens 12 -> 24 (16 -> 20), of 64 21 -> 26 (30 -> 21), of 128 39 -> 30 (58 -> 26); 4 of 32 30 -> 33 (35 -> 26); 16 of 16 42 -> 71 (49 -> 58), of 32 79 -> 75 (91 -> 61);
+// 64 of 16 172 -> 244 (198 -> 221), of 32 316 -> 258 (371 -> 227). The crossing lies at some 25 tokens a sequence and 50 more for F32, 18 and 20 for 16 bits; one rule between them.
+static bool delta_in_chunks(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs) { return d->d_state == 128u && n_tokens >= 24u * (uint64_t)n_seqs + 32u; }
 
 // What a call's arguments have to be; fills the strides. rows: tokens of q, k, v and out
 static int delta_check(const redcuda_delta_dims *d, const char *who, uint32_t rows, uint32_t n_seqs, uint32_t n_slots, DeltaArgs &A) {

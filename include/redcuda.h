@@ -276,7 +276,7 @@ typedef struct {
 /* Writes the K/V rows [n_kv][head_dim] (in_type; converted, rounded to nearest even) of n_tokens tokens to the cache. Rows cu_seqlens[b] up to
  * cu_seqlens[b + 1] - 1 are positions start[b], start[b] + 1, ... of sequence b; cu_seqlens NULL: one row per sequence, row b being position
  * start[b] of sequence b. A sequence with a negative start is left out, as are rows from cu_seqlens[n_seqs] on. row_stride: elements between
- * the rows of two tokens, 0 = n_kv * head_dim. */
+ * the rows of two tokens, 0 = n_kv * head_dim. Where two sequences of a call write the same position of a page that both have, what it then holds is not defined. */
 int redcuda_kv_append_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *start_dev,
                              uint32_t n_tokens, const int32_t *cu_seqlens_dev, uint32_t in_type, const void *k_dev, const void *v_dev, uint64_t row_stride,
                              void *stream);
@@ -314,7 +314,8 @@ int redcuda_delta_step_device(const redcuda_delta_dims *d, uint32_t n_seqs, cons
 
 /* Prompts laid end to end: tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of the n_tokens rows are sequence b's, in order (n_seqs + 1 ascending numbers on
  * the device; a sequence may be empty; rows from cu_seqlens[n_seqs] on are left as they were). Bounds that fall or leave the rows are reported and their sequence left out;
- * of rows that two sequences then claim the results are not defined. A value that is not finite makes what depends on it NaN, from its token on. Slots as above. workspace_dev:
+ * of rows that two sequences then claim the results are not defined. A value that is not finite makes what depends on it NaN, from its token on. In longer calls
+ * (those that need a workspace) the keys of 64 tokens share an exponent, as do their queries: one 2^17 smaller than the largest beside it keeps 22 bits, smaller ones fewer. Slots as above. workspace_dev:
  * redcuda_delta_rule_workspace bytes, 16-byte aligned (0: none is needed); calls that overlap on the GPU need one each. */
 uint64_t redcuda_delta_rule_workspace(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs);
 int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs, const int32_t *cu_seqlens_dev, const int32_t *slots_dev,

@@ -144,3 +144,68 @@ def test_prompts_then_captured_steps(kv):
                 assert abs(float(y[int(got[i]["ids"][b, j])] - best.values[j])) < 2 * tol
         assert float((sv.state[int(sv.slots[b])].double() - m).abs().max()) < 1e-4
     del graph
+
+
+def test_two_streams_at_once():
+    """Two streams that each run all operators on arrays and workspaces of their own, at the same time: every answer is the one that it is alone, to the bit."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def setup(kv16, lens, prompt, rows):
+        n, width = len(lens), -(-max(lens) // PAGE)
+        dt = torch.bfloat16 if kv16 else torch.float32
+        d = dict(n=n, width=width, rows=rows, k=rnd(n * width, PAGE, N_KV, HD).to(dt), v=rnd(n * width, PAGE, N_KV, HD).to(dt), type=30 if kv16 else 0,
+                 table=torch.randperm(n * width, generator=g, device="cuda").int().view(n, width), lens=ints(lens), q=rnd(n, N_Q, HD).to(dt), att=torch.empty(n, N_Q, HD, device="cuda", dtype=dt))
+        d["kv"] = rc.PagedKv(d["type"], N_KV, HD, PAGE, n * width, d["k"].data_ptr(), d["v"].data_ptr())
+        d["work"] = torch.empty(d["kv"].attend_workspace(N_Q), dtype=torch.uint8, device="cuda")
+        d["dims"] = rc.DeltaDims(d["type"], GROUPS, RANK, S)
+        unit = lambda x: (x / x.norm(dim=-1, keepdim=True)).to(dt)  # noqa: E731
+        T = sum(prompt)
+        d["T"], d["cu"], d["m"] = T, ints(np.cumsum([0] + prompt).tolist()), len(prompt)
+        d["dn"] = [unit(rnd(T, GROUPS, S)), unit(rnd(T, GROUPS, S)), rnd(T, RANK, S).to(dt), -rnd(T, RANK).abs(), torch.sigmoid(rnd(T, RANK))]
+        d["state0"], d["dout"] = rnd(len(prompt), RANK, S, S), torch.empty(T, RANK, S, device="cuda", dtype=dt)
+        d["state"] = d["state0"].clone()
+        d["dwork"] = torch.empty(d["dims"].workspace(T, d["m"]), dtype=torch.uint8, device="cuda")
+        d["x"], d["tok"] = rnd(rows, 20001).to(dt), ints(list(range(rows)))
+        d["lp"], d["ids"], d["top"] = torch.empty(2, rows, device="cuda"), torch.empty(rows, 4, dtype=torch.int32, device="cuda"), torch.empty(rows, 4, device="cuda")
+        return d
+
+    def run(d, s):
+        d["kv"].attend_device(d["table"].data_ptr(), d["width"], d["n"], d["lens"].data_ptr(), N_Q, d["type"], d["q"].data_ptr(), d["att"].data_ptr(), d["work"].data_ptr(), d["work"].numel(), s)
+        rc.delta_rule_device(d["dims"], d["T"], d["m"], d["cu"].data_ptr(), 0, d["m"], *[a.data_ptr() for a in d["dn"]], d["state"].data_ptr(), d["dout"].data_ptr(), d["dwork"].data_ptr(),
+                             d["dwork"].numel(), s)
+        rc.token_logprobs_device(d["type"], d["rows"], 20001, 0, d["x"].data_ptr(), d["tok"].data_ptr(), 4, d["lp"][0].data_ptr(), d["lp"][1].data_ptr(), d["ids"].data_ptr(), d["top"].data_ptr(), s)
+
+    got = lambda d: [d[n].clone() for n in ("att", "dout", "state", "lp", "ids", "top")]  # noqa: E731
+    both = [setup(True, [700, 3, 1900, 0, 64] * 9, [200, 70, 0, 333], 3), setup(False, [90, 17], [500, 1], 150)]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    alone = []
+    for d, s in zip(both, streams):
+        run(d, s.cuda_stream)
+        torch.cuda.synchronize()
+        alone.append(got(d))
+        assert all(bool(a.float().isfinite().all()) for a in alone[-1])
+    for _ in range(20):
+        for d in both:
+            d["state"].copy_(d["state0"])
+            for n in ("att", "dout", "lp", "ids", "top"):
+                d[n].fill_(7)
+        torch.cuda.synchronize()
+        for _ in range(3):                                # the second and third run go on from the states of the one before: only the outputs of the attention are the same
+            for d, s in zip(both, streams):
+                run(d, s.cuda_stream)
+        torch.cuda.synchronize()
+        for d, want in zip(both, alone):
+            now = got(d)
+            assert all(torch.equal(now[i], want[i]) for i in (0, 3, 4, 5))
+        for d in both:
+            d["state"].copy_(d["state0"])
+        torch.cuda.synchronize()
+        for d, s in zip(both, streams):
+            run(d, s.cuda_stream)
+        torch.cuda.synchronize()
+        for d, want in zip(both, alone):
+            assert all(torch.equal(a, b) for a, b in zip(got(d), want))
+    rc.device_status()

@@ -299,3 +299,51 @@ def test_host_form(dtype):
     _close(x, [0, 30, 90], [2, 0], torch.from_numpy(out).cuda(), torch.from_numpy(state).cuda(), 1 / 8)
     with pytest.raises(rc.RedcudaError, match="slot"):
         rc.delta_rule(h["q"], h["k"], h["v"], h["gate"], h["beta"], state, [0, 30, 90], [2, 2])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_keys_and_queries_of_many_sizes(dtype):
+    """Tokens whose keys and queries are up to 2^12 apart, some of them zero: an output is as good as its own query is large."""
+    x = _inputs(_gen(10), 300, 2, 4, 128, TYPES[dtype][1], 1)
+    size = torch.exp2(-torch.randint(0, 13, (2, 300), generator=_gen(11), device="cuda").float())
+    size[:, [0, 70, 71, 299]] = 0.0
+    x["q"], x["k"] = [(x[n].float() * size[i][:, None, None]).to(x[n].dtype) for i, n in enumerate("qk")]        # powers of two: exact but for what F16 rounds below 2^-14
+    out, state = _rule(x, [0, 300], [0], rc.DeltaDims(TYPES[dtype][0], 2, 4, 128), 1)
+    assert bool((out[size[0] == 0] == 0).all())
+    rows = size[0] > 0
+    want, last, most = _reference(x, [0, 300], [0], 1 / math.sqrt(128))
+    unit = 8 * math.sqrt(316) * 2.0 ** -22 * (most + float(x["v"].double().abs().max()))
+    length = x["q"].double().norm(dim=-1).amax(-1)
+    tol = unit / math.sqrt(128) * length[:, None, None] + torch.finfo(out.dtype).eps / 2 * want.abs() + 2.0 ** -25 * (out.dtype == torch.float16)      # half a step of F16's smallest numbers
+    assert bool(((out.double() - want).abs() <= tol)[rows].all()), float(((out.double() - want).abs() / tol)[rows].max())
+    assert float((state.double() - last).abs().max()) <= unit
+
+
+@pytest.mark.parametrize("B", [65535, 65536, 70001])
+def test_very_many_sequences(B):
+    """More sequences than a grid has rows of blocks, a token each: the step and the rule, with some of them padded."""
+    x = _inputs(_gen(B), B, 1, 1, 32, torch.float32, B)
+    slots = torch.arange(B - 1, -1, -1, dtype=torch.int32, device="cuda")
+    slots[5], slots[B - 2] = -1, -1
+    state, out, dims = x["state"].clone(), torch.full_like(x["v"], 7.0), rc.DeltaDims(0, 1, 1, 32)
+    again, other = x["state"].clone(), torch.full_like(x["v"], 7.0)
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    rows = [x[n].data_ptr() for n in ("q", "k", "v", "gate", "beta")]
+    torch.cuda.synchronize()
+    s = torch.cuda.current_stream().cuda_stream
+    rc.delta_step_device(dims, B, slots.data_ptr(), B, *rows, state.data_ptr(), out.data_ptr(), s)
+    rc.delta_rule_device(dims, B, B, cu.data_ptr(), slots.data_ptr(), B, *rows, again.data_ptr(), other.data_ptr(), 0, 0, s)
+    torch.cuda.synchronize()
+    rc.device_status()
+    live = slots >= 0
+    k, q, v = (x[n][:, 0].double() for n in ("k", "q", "v"))
+    m = x["state"][slots.clamp(min=0).long(), 0].double() * torch.exp(x["gate"].double())[:, :, None]
+    m = m + ((v - (m @ k[:, :, None])[:, :, 0]) * x["beta"].double())[:, :, None] * k[:, None]
+    unit = 8 * math.sqrt(17) * 2.0 ** -22 * (float(m.norm(dim=-1).max()) + float(v.abs().max()))
+    want = (m @ q[:, :, None])[:, :, 0] / math.sqrt(32)
+    for st, o in ((state, out), (again, other)):
+        assert float((o[:, 0].double() - want)[live].abs().max()) <= unit and bool((o[~live] == 7.0).all())
+        assert float((st[slots[live].long(), 0].double() - m[live]).abs().max()) <= unit
+        unused = torch.ones(B, dtype=torch.bool, device="cuda")
+        unused[slots[live].long()] = False
+        assert torch.equal(st[unused], x["state"][unused])

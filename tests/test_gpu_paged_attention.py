@@ -352,3 +352,16 @@ def test_append_finds_every_sequence(n_seqs):
         want[b, :n] = np.arange(t, t + n)
         t += n
     assert np.array_equal(k[:, :, 0, 0].cpu().numpy(), want) and np.array_equal(v[:, :, 0, 63].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("qt, cache", PAIRS)
+def test_queries_and_rows_of_zeros(qt, cache):
+    """Queries of zeros weigh every position alike; keys and values of zeros; queries near the smallest numbers."""
+    c = Cache(_gen(14), cache, 2, 128, 16, [200, 33, 5])
+    q = _q(_gen(15), 3, 8, 128, qt)
+    q[0], q[1, 3] = 0.0, 0.0
+    q[2] = (q[2].float() * 2.0 ** -20).to(q.dtype)
+    c.k[int(c.table[1, 0])] = 0.0
+    c.v[int(c.table[1, 1])] = 0.0
+    out, lse = _attend(c, q, [200, 33, 5], 8, qt)
+    _check(c, q, [200, 33, 5], 8, out, lse)
