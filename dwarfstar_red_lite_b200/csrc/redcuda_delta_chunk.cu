@@ -483,9 +483,10 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_s
 //     M1  [S k | S q] = S [K | Q]^T      M2  D = R T^T      M4  D' K (the state's)      M3  D P^T (the outputs')
 // between them the threads make R of M1's result, D and D' = D exp(G_last - G) of M2's, the new S of M4's, the outputs of M1's and M3's. Of four further warps one issues the products and fetches their
 // operands (a tile again as soon as the product that reads it is done), one fetches the values, two store the outputs. What bounds it is the chain M1, R, M2, D', M4, S: each link waits for the one before, so what is
-// not a link (the outputs, the digits of D, the largest of S) comes behind the hand-over of one. The scales of R and S come from bounds, which need no exchange between a row's two threads: up to 2^13
+// not a link (the outputs, the digits of D, the largest of S) comes behind the hand-over of one, and M4, S and M1 go by halves of the state's columns, one of the row's two threads behind the other
+// (a prompt of 2000 tokens 182 -> 177 us with the preparation, twelve prompts 434 -> 424; M1's keys ahead of its queries 195 and 434: products of 64 columns take as long as those of 128). The scales of R and S come from bounds, which need no exchange between a row's two threads: up to 2^13
 // too large costs nothing, as two fp16 digits reach from 2^16 down to 2^-24.
-// A chunk takes some 4 us: a prompt of 2000 tokens 141 us (32 blocks), twelve prompts of 16384 tokens together 261 (384 blocks on 148 SMs; tensor cores 26 to 36 % busy).
+// A chunk takes some 4 us: a prompt of 2000 tokens 136 us (32 blocks), twelve prompts of 16384 tokens together 251 (384 blocks on 148 SMs; tensor cores 26 to 36 % busy).
 // The adder of the tensor cores truncates, so lower digits go first and M1's sums are kept in two halves of 64 columns each, which are added in fp32.
 constexpr uint32_t DC_THREADS = 384u, DC_ROW_WARPS = 8u, DC_CONTROL = 8u, DC_LOADER = 9u, DC_STORER = 10u;        // 10 and 11 store
 // registers: 384 threads are launched with 168 each, of which the four further warps keep 72 and the threads of the rows have 216 (256 x 216 + 128 x 72 = 384 x 168)
@@ -493,7 +494,7 @@ constexpr uint32_t DC_REGS_ROWS = 216u, DC_REGS_CONTROL = 72u;
 static_assert(256u * DC_REGS_ROWS + 128u * DC_REGS_CONTROL <= 384u * 168u, "a split above the launch's registers waits forever");
 constexpr uint32_t DC_SPIN_LIMIT = 1u << 26;     // polls of some twenty cycles: more than half a second, far beyond any real wait
 enum : uint32_t { DT_S = 0, DT_M1 = 128, DT_D = 128, DT_DK = 192, DT_M4 = 256, DT_R = 384, DT_M3 = 384, DT_M2 = 448 };      // columns of tensor memory; M1: two accumulators of 128
-enum : uint32_t { DB_KQ, DB_T, DB_PK, DB_META0, DB_META1, DB_V, DB_M1, DB_M2, DB_M3, DB_M4, DB_OFREE, DB_R, DB_DK, DB_D, DB_S, DB_VFREE, DB_OUT, DB_END, DB_PAIR, DB_COUNT = DB_PAIR + 4 };
+enum : uint32_t { DB_KQ, DB_T, DB_PK, DB_META0, DB_META1, DB_V, DB_M1, DB_M2, DB_M3, DB_M4, DB_M4B, DB_OFREE, DB_R, DB_DK, DB_D, DB_VFREE, DB_OUT, DB_END, DB_S, DB_SB, DB_PAIR, DB_COUNT = DB_PAIR + 4 };
 constexpr uint32_t DC_SROW = DC_S * 4u + 16u;    // a row of the state on its way through shared memory, 16 bytes further apart than it is long: a quarter warp's rows lie in different banks
 constexpr uint32_t dc_smem_bytes(int dig, uint32_t size) { return dc_keys(dig) + 4u * DC_SQ + 2u * (uint32_t)sizeof(DcMeta) + 2u * DC_T * DC_S * size; }
 static_assert(dc_smem_bytes(1, 2u) >= 114u * 1024u && dc_smem_bytes(2, 4u) < 220u * 1024u, "one block an SM: it takes all of the tensor memory");
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
     auto bar = [&](uint32_t i) { return dc_smem(&s_bar[i]); };
     if (tid == 0u) {
         fail = 0u;
-        for (uint32_t i = 0; i < DB_COUNT; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar(i)), "r"(i >= DB_PAIR || i == DB_OFREE ? 2u : i >= DB_R ? DC_ROW_WARPS : i == DB_V ? 32u : 1u));
+        for (uint32_t i = 0; i < DB_COUNT; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar(i)), "r"(i >= DB_PAIR || i == DB_OFREE ? 2u : i >= DB_S ? DC_ROW_WARPS / 2u : i >= DB_R ? DC_ROW_WARPS : i == DB_V ? 32u : 1u));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -613,19 +614,19 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
                 if (lane == 0u) { expect(DB_META0 + (c & 1u), sizeof(DcMeta)); copy(DB_META0 + (c & 1u), s_meta + (c & 1u) * sizeof(DcMeta), rec + c * rec_step + 4u * DC_SQ, sizeof(DcMeta)); }
             };
             get_kq(0u);
-            if (wait(DB_S, 0u)) { get_meta(0u); get_t(0u); get_pk(0u); }         // over the state, which has been read
+            if (wait(DB_S, 0u) && wait(DB_SB, 0u)) { get_meta(0u); get_t(0u); get_pk(0u); }         // over the state, which has been read
             const uint64_t desc = tc_smem_desc(0u, 2048u, 128u), desc_sq = tc_smem_desc(0u, 1024u, 128u);
             const uint32_t high = (uint32_t)(desc >> 32), wide = (uint32_t)desc, slim = (uint32_t)desc_sq;       // the upper words are alike
             const uint32_t b_kq = wide | (dc_smem(s_kq) >> 4), b_kt = wide | (dc_smem(s_kt) >> 4), b_t = slim | (dc_smem(s_tt) >> 4), b_p = slim | (dc_smem(s_pp) >> 4);
-            // 128 columns of results += A B^T over 64 of k, lower digits first. a_lo: columns from A's upper to its lower digits, b_lo: 16-byte units from B's
-            auto square = [&](uint32_t d, uint32_t a, uint32_t a_lo, uint32_t bd, uint32_t b_lo) {
+            // n columns of results += A B^T over 64 of k, lower digits first. a_lo: columns from A's upper to its lower digits, b_lo: 16-byte units from B's
+            auto square = [&](uint32_t n, uint32_t d, uint32_t a, uint32_t a_lo, uint32_t bd, uint32_t b_lo) {
 #pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + a_lo + 8u * k, bd + k * 256u, high, tc_idesc(128u), k ? 1u : 0u);
+                for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + a_lo + 8u * k, bd + k * 256u, high, tc_idesc(n), k ? 1u : 0u);
                 if (DIG == 2)
 #pragma unroll
-                    for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + 8u * k, bd + b_lo + k * 256u, high, tc_idesc(128u), 1u);
+                    for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + 8u * k, bd + b_lo + k * 256u, high, tc_idesc(n), 1u);
 #pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + 8u * k, bd + k * 256u, high, tc_idesc(128u), 1u);
+                for (uint32_t k = 0; k < 4u; ++k) dc_mma_ts(leader, tmem + d, tmem + a + 8u * k, bd + k * 256u, high, tc_idesc(n), 1u);
             };
             // the same with a lower triangle of 64: a step of 16 of k meets the rows from its own on
             auto triangle = [&](uint32_t d, uint32_t a, uint32_t bd) {
@@ -641,8 +642,10 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
                 const bool more = c + 1u < chunks;
                 if (!wait(DB_KQ, c) || !wait(DB_S, c) || (c && !wait(DB_M3, c - 1u))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                square(DT_M1, DT_S, 64u, b_kq, DC_KQ >> 4);
-                square(DT_M1 + 128u, DT_S + 32u, 64u, b_kq + 4u * 256u, DC_KQ >> 4);
+                square(128u, DT_M1, DT_S, 64u, b_kq, DC_KQ >> 4);
+                if (!wait(DB_SB, c)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                square(128u, DT_M1 + 128u, DT_S + 32u, 64u, b_kq + 4u * 256u, DC_KQ >> 4);
                 tc_commit_if(leader, bar(DB_M1));
                 if (c) get_pk(c);
                 if (!wait(DB_M1, c)) break;
@@ -656,8 +659,10 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
                 if (more) get_t(c + 1u);
                 if (!wait(DB_PK, c) || !wait(DB_DK, c)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                square(DT_M4, DT_DK, 32u, b_kt, DC_KT >> 4);
+                square(64u, DT_M4, DT_DK, 32u, b_kt, DC_KT >> 4);
                 tc_commit_if(leader, bar(DB_M4));
+                square(64u, DT_M4 + 64u, DT_DK, 32u, b_kt + 64u, DC_KT >> 4);
+                tc_commit_if(leader, bar(DB_M4B));
                 if (!wait(DB_D, c)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 triangle(DT_M3, DT_D, b_p);
@@ -672,7 +677,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
 #pragma unroll 1
             for (uint32_t c = 0; c < chunks; ++c) {
                 const uint32_t n = min((uint32_t)DC_T, (uint32_t)(hi - lo) - c * DC_T) * PIECES;
-                if (c ? !wait(DB_VFREE, c - 1u) : !wait(DB_S, 0u)) break;      // ahead of the first chunk the state is there
+                if (c ? !wait(DB_VFREE, c - 1u) : !(wait(DB_S, 0u) && wait(DB_SB, 0u))) break;      // ahead of the first chunk the state is there
 #pragma unroll 4
                 for (uint32_t i = lane; i < n; i += 32u)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dc_smem(s_v) + i * 16u), "l"(v + (uint64_t)(c * DC_T + i / PIECES) * A.v_stride + i % PIECES * (16u / sizeof(T))) : "memory");
@@ -721,7 +726,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
             dc_scale(bound, up, unit_s);
             dc_put32(s, up, mine + DT_S + hf * 32u, mine + DT_S + 64u + hf * 32u);
             dc_put32(s + 32, up, mine + DT_S + hf * 32u + 16u, mine + DT_S + 64u + hf * 32u + 16u);
-            dc_hand_over(bar(DB_S));
+            dc_hand_over(bar(DB_S + hf));
         };
         // a warp reads a row at a time and has it from shared memory a row a lane
 #pragma unroll
@@ -820,7 +825,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
                 f4 *= M.f_k;                     // of M4's
             }
             const float last = M.last;
-            if (!(ok = wait(DB_M4, c))) break;
+            if (!(ok = wait(DB_M4 + hf, c))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int i = 0; i < 64; i += 32) {
