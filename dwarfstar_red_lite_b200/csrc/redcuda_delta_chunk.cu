@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_s
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < P; ++e) { rk[i][e] = reinterpret_cast<const uint4 *>(k + i * 32)[e]; rq[i][e] = reinterpret_cast<const uint4 *>(q + i * 32)[e]; }
-        if (dv < width) gates(dv);
+        if (dv < min(width, 2u)) gates(dv);
         if (tid < 4u) s_bad[tid >> 1][tid & 1u] = 0u;
         __syncthreads();
         // a row's largest; a row behind the last token or with a number that is not finite is taken out
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_s
             meta->nan_from = min(first0, first1); meta->bad_q[0] = s_bad[1][0]; meta->bad_q[1] = s_bad[1][1];
         }
     };
-    if (dv < width) decays(dv);
+    if (dv < min(width, 2u)) decays(dv);
     // warps 0-3: K K^T, rows 16 warp on; 4-7: Q K^T, rows 16 (7 - warp) on, so that every scheduler has as much; the columns up to the diagonal
     const uint32_t which = warp >> 2, mt = which ? 7u - warp : warp, g = lane >> 2, c2 = (lane & 3u) * 2u;
     float c[4][2][4];

@@ -347,3 +347,12 @@ def test_very_many_sequences(B):
         unused = torch.ones(B, dtype=torch.bool, device="cuda")
         unused[slots[live].long()] = False
         assert torch.equal(st[unused], x["state"][unused])
+
+
+@pytest.mark.parametrize("groups, rank", [(1, 4), (4, 4), (20, 40), (8, 48)])       # few states: several blocks each; many: one each
+@pytest.mark.parametrize("gate, keys", [("none", "same"), ("strong", "random"), ("cut", "near"), ("mixed", "same")])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gates_and_keys_of_few_and_many_heads(groups, rank, gate, keys, dtype):
+    cu = [0, 333]
+    x = _inputs(_gen(rank), 333, groups, rank, 128, TYPES[dtype][1], 1, gate, keys)
+    _close(x, cu, [0], *_rule(x, cu, [0], rc.DeltaDims(TYPES[dtype][0], groups, rank, 128), 1), 1 / math.sqrt(128))
