@@ -356,3 +356,70 @@ def test_gates_and_keys_of_few_and_many_heads(groups, rank, gate, keys, dtype):
     cu = [0, 333]
     x = _inputs(_gen(rank), 333, groups, rank, 128, TYPES[dtype][1], 1, gate, keys)
     _close(x, cu, [0], *_rule(x, cu, [0], rc.DeltaDims(TYPES[dtype][0], groups, rank, 128), 1), 1 / math.sqrt(128))
+
+
+@pytest.mark.parametrize("T", [256, 319, 320, 321, 1000])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_one_sequence(T, dtype):
+    """Rows ahead of the sequence and behind it are left as they were."""
+    x = _inputs(_gen(T), T + 90, 2, 6, 128, TYPES[dtype][1], 3)
+    _close(x, [70, 70 + T], [1], *_rule(x, [70, 70 + T], [1], rc.DeltaDims(TYPES[dtype][0], 2, 6, 128), 3), 1 / math.sqrt(128))
+
+
+@pytest.mark.parametrize("groups, rank", [(1, 2), (20, 40)])
+@pytest.mark.parametrize("what, value", [("q", math.nan), ("k", math.inf), ("gate", math.nan), ("beta", -math.inf), ("v", math.inf), ("v", math.nan)])
+@pytest.mark.parametrize("t", [0, 63, 200, 257, 399])
+def test_what_is_not_finite_in_one_sequence(groups, rank, what, value, t):
+    """As above, where the one sequence's states are worked on by several blocks each, or by one."""
+    x = _inputs(_gen(6), 400, groups, rank, 128, torch.float32, 1)
+    cu, dims = [0, 400], rc.DeltaDims(0, groups, rank, 128)
+    clean, want = _rule(x, cu, [0], dims, 1)
+    x[what][(t, 0, 7) if what in ("q", "k") else (t, 1, 37) if what == "v" else (t, 1)] = value
+    out, state = _rule(x, cu, [0], dims, 1)
+    last = t + 1 if what == "q" else 400
+    for h in range(rank):
+        if h in ([0, 1] if what in ("q", "k") else [1]):
+            rows = slice(37, 38) if what == "v" else slice(None)
+            assert bool(out[t:last, h, rows].isnan().all())
+            assert torch.equal(out[:t - t % 64, h], clean[:t - t % 64, h]) if what == "q" else torch.equal(out[:t, h], clean[:t, h])
+            if what == "q":
+                # A chunk's queries share an exponent, which the largest of them sets: without that one the others' lower digits may be rounded at another place. Either output is within its
+                # tolerance of the exact one, so they differ by twice that at most; what follows the chunk is the same.
+                end = min(400, t - t % 64 + 64)
+                unit = 8 * math.sqrt(416) * 2.0 ** -22 * (float(want.norm(dim=-1).max()) + float(x["v"].abs().max())) / math.sqrt(128)
+                near = [i for i in range(t - t % 64, end) if i != t]
+                assert float((out[near, h] - clean[near, h]).abs().max()) <= 2 * unit and torch.equal(out[end:, h], clean[end:, h])
+            else:
+                assert torch.equal(out[last:, h], clean[last:, h])
+            if what != "q":
+                assert bool(state[0, h, rows].isnan().all())
+            if what == "v":
+                others = [i for i in range(128) if i != 37]
+                assert torch.equal(state[0, h][others], want[0, h][others]) and torch.equal(out[:, h][:, others], clean[:, h][:, others])
+        else:
+            assert torch.equal(out[:, h], clean[:, h]) and torch.equal(state[0, h], want[0, h])
+
+
+@pytest.mark.parametrize("groups, rank", [(1, 2), (20, 40)])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_a_state_that_is_not_finite(groups, rank, value):
+    """A row of the state with an infinity or a NaN is no number from the first token on; the other rows are as they were."""
+    x = _inputs(_gen(16), 400, groups, rank, 128, torch.float32, 1)
+    dims, others = rc.DeltaDims(0, groups, rank, 128), [i for i in range(128) if i != 70]
+    clean, want = _rule(x, [0, 400], [0], dims, 1)
+    x["state"][0, 1, 70, 3] = value
+    out, state = _rule(x, [0, 400], [0], dims, 1)
+    assert bool(out[:, 1, 70].isnan().all()) and bool(state[0, 1, 70].isnan().all())
+    assert torch.equal(out[:, 1][:, others], clean[:, 1][:, others]) and torch.equal(state[0, 1][others], want[0, 1][others])
+    assert torch.equal(out[:, 0], clean[:, 0]) and torch.equal(state[0, 0], want[0, 0])
+
+
+@pytest.mark.parametrize("groups, rank", [(1, 2), (20, 40)])
+def test_rows_of_many_sizes(groups, rank):
+    """Rows of values, and of the state, up to 2^12 apart: each as good as it is large."""
+    x = _inputs(_gen(17), 300, groups, rank, 128, torch.float32, 1)
+    size = torch.exp2(-torch.randint(0, 13, (rank, 128), generator=_gen(18), device="cuda").float())
+    x["v"], x["state"] = x["v"] * size, x["state"] * size[:, :, None]
+    out, state = _rule(x, [0, 300], [0], rc.DeltaDims(0, groups, rank, 128), 1)
+    y = dict(x, v=x["v"] / size, state=x["state"] / size[:, :, None])                  # the rows by themselves, which are independent: powers of two are exact
+    _close(y, [0, 300], [0], out / size, state / size[:, :, None], 1 / math.sqrt(128))
