@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
 // Lanes 0 to 63 of M1 and M2 become R and D, lanes 64 to 127 of M1 and M3 the outputs; warps 0, 1, 4 and 5 make the former, 2, 3, 6 and 7 the latter, all of them the state (16 rows a thread). The operands A come
 // as k_delta_prep left them, T and P by two warps of their own, row block by row block as far as the triangles reach. R, D, D' and S are operands B in shared memory, which the threads write as [row / 8][k][8 rows]. Their digits have
 // one exponent for the block's 32 rows: a row 2^17 smaller than the largest keeps its 22 bits. Bounds, truncation and what is not finite as above.
-// What bounds it is the same chain with shorter links, some 4800 cycles a chunk: M1 1160, R 890, M2 640, D' 690, M4 820, S 600; a product takes some 65 cycles, whatever its columns, as it reads 4 KB of A.
+// What bounds it is the same chain with shorter links, some 4800 cycles a chunk (a prompt of 2000 tokens 95 us, 128 blocks): M1 1160, R 890, M2 640, D' 690, M4 820, S 600; a product takes some 65 cycles, whatever its columns, as it reads 4 KB of A.
 constexpr int DN_ROWS = 32;
 constexpr uint32_t DN_CONTROL = 8u, DN_TP = 9u, DN_THREADS = 352u;             // 9: T, 10: P
 enum : uint32_t { NT_M1 = 0, NT_M2 = 128, NT_M3 = 192, NT_M4 = 256, NT_COLS = 512 };     // each 32 columns for the upper digits' products and 32 for those with a lower digit; M1 twice
