@@ -121,7 +121,6 @@ __global__ void __launch_bounds__(LP_WARPS * 32, sizeof(T) == 4 ? 4 : 3) k_token
     const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank(), row = blockIdx.x / parts;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, n = A.top_n;
     __shared__ uint64_t s_keys[LP_WARPS][32], s_best[LP_CLUSTER][32];
-    __shared__ uint16_t s_cand[LP_WARPS][32 * U * VEC];
     __shared__ LpSums s_sums[LP_WARPS], s_parts[LP_CLUSTER];
     __shared__ __align__(16) float s_floor[LP_WARPS];
     const T *x = reinterpret_cast<const T *>(A.x) + (uint64_t)row * A.row_stride;
@@ -160,6 +159,10 @@ __global__ void __launch_bounds__(LP_WARPS * 32, sizeof(T) == 4 ? 4 : 3) k_token
         s2.x *= f; s2.y *= f;
         m = to;
     };
+    // the token and its logit are asked for long before they are wanted: read at the end, one after the other, they would take a microsecond of every row
+    const bool asks = A.logprob && part == 0u && tid == 0u;
+    int32_t token = -1;
+    if (asks) asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(token) : "l"(A.tokens + row));
     bool fresh = true;
     uint4 ahead[U];                              // the next round's pieces
     auto load = [&](uint32_t p) {
@@ -217,28 +220,26 @@ __global__ void __launch_bounds__(LP_WARPS * 32, sizeof(T) == 4 ? 4 : 3) k_token
         }
         // what equals the n-th of earlier rounds has a larger index
         if (!__any_sync(0xffffffffu, most >= bar && (least == 0ull || most > lp_value(least)))) continue;
-        // the places of the values that reach the bar, then the values themselves, 32 at a time
-        uint32_t count = 0u;
-        __syncwarp();
+        // a lane's values that reach the bar, as bits, which are then offered one a lane at a time
+        static_assert(U * VEC <= 32, "a bit each");
+        uint32_t places = 0u;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (!__any_sync(0xffffffffu, top[u] >= bar)) continue;
             float v[VEC];
             if constexpr (sizeof(T) == 4) lp_unpack(w[u], v); else lp_unpack<T>(w[u], v);
-            const bool have = p + u * 32u + lane < p1;
+            if (p + u * 32u + lane < p1)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const bool in = have && v[i] >= bar;
-                const uint32_t who = __ballot_sync(0xffffffffu, in);
-                if (in) s_cand[warp][count + __popc(who & ((1u << lane) - 1u))] = (uint16_t)((u * 32u + lane) * VEC + i);
-                count += __popc(who);
-            }
+                for (int i = 0; i < VEC; ++i) places |= v[i] >= bar ? 1u << (u * VEC + i) : 0u;
         }
-        __syncwarp();
 #pragma unroll 1
-        for (uint32_t k = lane; k - lane < count; k += 32u) {
+        while (__any_sync(0xffffffffu, places)) {
             uint64_t key = 0ull;
-            if (k < count) { const uint32_t i = head + p * VEC + s_cand[warp][k]; key = lp_key(to_f32(x[i]), i); }
+            if (places) {
+                const uint32_t j = (uint32_t)__ffs((int)places) - 1u, i = head + (p + j / VEC * 32u + lane) * VEC + j % VEC;
+                places &= places - 1u;
+                key = lp_key(to_f32(x[i]), i);
+            }
             offer(key);
         }
         if (least) bar = fmaxf(bar, lp_value(least));
@@ -254,6 +255,9 @@ __global__ void __launch_bounds__(LP_WARPS * 32, sizeof(T) == 4 ? 4 : 3) k_token
         u2.x += e * d;
         if (n) offer(have && v == v ? lp_key(v, i) : 0ull);
     }
+    const bool known = token >= 0 && (uint32_t)token < A.vocab;
+    T logit = from_f32<T>(0.f);
+    if (asks && known) logit = x[token];
     LpSums S{m, s2.x + s2.y, u2.x + u2.y};
 #pragma unroll
     for (int w = 16; w; w >>= 1) {
@@ -306,10 +310,9 @@ __global__ void __launch_bounds__(LP_WARPS * 32, sizeof(T) == 4 ? 4 : 3) k_token
     const bool nan = !(S.s == S.s), none = !nan && S.m == -INFINITY;
     if (lane == 0u) {
         if (A.logprob) {
-            const int32_t t = A.tokens[row];
             float lp = NAN;
-            if (t >= 0 && (uint32_t)t < A.vocab) lp = nan ? NAN : none ? -INFINITY : (to_f32(x[t]) - S.m) - ls;
-            else if (t != -1 && A.status) A.status[ST_TOKEN_RANGE] = 1u;
+            if (known) lp = nan ? NAN : none ? -INFINITY : (to_f32(logit) - S.m) - ls;
+            else if (token != -1 && A.status) A.status[ST_TOKEN_RANGE] = 1u;
             A.logprob[row] = lp;
         }
         if (A.entropy) A.entropy[row] = nan ? NAN : none ? 0.f : fmaxf(ls - S.u / S.s, 0.f);
