@@ -111,7 +111,7 @@ template <class T> __device__ __forceinline__ float lp_most(uint4 w) {
 // The alternatives cost one comparison a lane and round of LP_UNROLL pieces where there are none: a warp keeps its 32 largest keys, one a
 // lane, and looks at single values only where the largest of a lane's round reaches what is known to be among the row's n largest. That is the n-th of the warp's own,
 // or the least of the warps' ceil(n / LP_WARPS)-th largest, which every warp publishes (n values are at least that large; a stale one is a lower bound too), or in a warp's first
-// round the n-th of its lanes' largest. 777 rows of BF16 with 5, 20 alternatives: 74, 87 us.
+// round the n-th of its lanes' largest. 777 rows of BF16 with 5, 20 alternatives: 69, 82 us (the n-th of what the warps publish instead of the least, found anew with every list: 69, 93).
 template <class T>
 __global__ void __launch_bounds__(LP_WARPS * 32, sizeof(T) == 4 ? 4 : 3) k_token_logprobs(LogprobArgs A) {
     pdl_prologue();
