@@ -159,16 +159,16 @@ static int delta_check(const redcuda_delta_dims *d, const char *who, uint32_t ro
     A.n_tokens = rows; A.n_slots = n_slots; A.groups = d->n_group; A.rank = d->dt_rank;
     return 1;
 }
-static int delta_pointers(const redcuda_delta_dims *d, const char *who, uint32_t rows, uint32_t n_slots, const DeltaArgs &A) {
+static int delta_pointers(const redcuda_delta_dims *d, const char *who, uint32_t rows, uint32_t n_seqs, uint32_t n_slots, const DeltaArgs &A) {
     RC_REQUIRE(A.q && A.k && A.v && A.gate && A.beta && A.state && A.out, "%s: null argument", who);
     RC_REQUIRE(aligned16(A.q) && aligned16(A.k) && aligned16(A.v) && aligned16(A.state) && aligned16(A.out), "%s: a pointer is not 16-byte aligned", who);
     RC_REQUIRE(aligned4(A.gate) && aligned4(A.beta) && aligned4(A.slots) && aligned4(A.cu), "%s: gates, betas or whole numbers are not 4-byte aligned", who);
     const uint32_t size = val_size(d->type);
     const uint64_t key = (uint64_t)d->n_group * d->d_state, val = (uint64_t)d->dt_rank * d->d_state, ob = (uint64_t)rows * val * size, sb = (uint64_t)n_slots * val * d->d_state * 4u;
-    const void *in[5] = {A.q, A.k, A.v, A.gate, A.beta};
-    const uint64_t bytes[5] = {span_bytes(rows, A.q_stride, key, size), span_bytes(rows, A.k_stride, key, size), span_bytes(rows, A.v_stride, val, size), (uint64_t)rows * d->dt_rank * 4u,
-                               (uint64_t)rows * d->dt_rank * 4u};
-    for (int i = 0; i < 5; ++i) RC_REQUIRE(!overlap(A.out, ob, in[i], bytes[i]) && !overlap(A.state, sb, in[i], bytes[i]), "%s: the output or the states lie inside the inputs", who);
+    const void *in[7] = {A.q, A.k, A.v, A.gate, A.beta, A.cu, A.slots};
+    const uint64_t bytes[7] = {span_bytes(rows, A.q_stride, key, size), span_bytes(rows, A.k_stride, key, size), span_bytes(rows, A.v_stride, val, size), (uint64_t)rows * d->dt_rank * 4u,
+                               (uint64_t)rows * d->dt_rank * 4u, (n_seqs + 1ull) * 4u, (uint64_t)n_seqs * 4u};
+    for (int i = 0; i < 7; ++i) RC_REQUIRE(!overlap(A.out, ob, in[i], bytes[i]) && !overlap(A.state, sb, in[i], bytes[i]), "%s: the output or the states lie inside the inputs", who);
     RC_REQUIRE(!overlap(A.out, ob, A.state, sb), "%s: the output lies inside the states", who);
     return 1;
 }
@@ -186,7 +186,7 @@ int redcuda_delta_step_device(const redcuda_delta_dims *d, uint32_t n_seqs, cons
     A.q = q_dev; A.k = k_dev; A.v = v_dev; A.gate = gate_dev; A.beta = beta_dev; A.state = state_dev; A.out = out_dev; A.slots = slots_dev;
     RC_REQUIRE(n_seqs, "delta step: no sequences");
     RC_REQUIRE(slots_dev || n_seqs <= n_slots, "delta step: %u sequences for %u states", n_seqs, n_slots);
-    if (!delta_pointers(d, "delta step", n_seqs, n_slots, A) || !require_device()) return 0;
+    if (!delta_pointers(d, "delta step", n_seqs, n_seqs, n_slots, A) || !require_device()) return 0;
     A.status = status_words();
     cudaStream_t s = (cudaStream_t)stream;
     prof_begin("delta_step", s);
@@ -209,7 +209,7 @@ int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, ui
     A.q = q_dev; A.k = k_dev; A.v = v_dev; A.gate = gate_dev; A.beta = beta_dev; A.state = state_dev; A.out = out_dev; A.slots = slots_dev; A.cu = cu_seqlens_dev;
     RC_REQUIRE(n_seqs && cu_seqlens_dev, "delta rule: no sequences");
     RC_REQUIRE(slots_dev || n_seqs <= n_slots, "delta rule: %u sequences for %u states", n_seqs, n_slots);
-    if (!delta_pointers(d, "delta rule", n_tokens, n_slots, A)) return 0;
+    if (!delta_pointers(d, "delta rule", n_tokens, n_seqs, n_slots, A)) return 0;
     const uint64_t need = redcuda_delta_rule_workspace(d, n_tokens, n_seqs);
     RC_REQUIRE(!need || (workspace_dev && workspace_bytes >= need && aligned16(workspace_dev)), "delta rule: a 16-byte aligned workspace of %llu bytes is needed", (unsigned long long)need);
     if (need) {
@@ -218,8 +218,9 @@ int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, ui
         RC_REQUIRE(!overlap(workspace_dev, need, out_dev, n_tokens * val * size) && !overlap(workspace_dev, need, state_dev, n_slots * val * d->d_state * 4u) &&
                    !overlap(workspace_dev, need, q_dev, span_bytes(n_tokens, A.q_stride, (uint64_t)d->n_group * d->d_state, size)) &&
                    !overlap(workspace_dev, need, k_dev, span_bytes(n_tokens, A.k_stride, (uint64_t)d->n_group * d->d_state, size)) &&
-                   !overlap(workspace_dev, need, v_dev, span_bytes(n_tokens, A.v_stride, val, size)) && !overlap(workspace_dev, need, gate_dev, rows) && !overlap(workspace_dev, need, beta_dev, rows),
-                   "delta rule: the workspace overlaps rows, states or outputs");
+                   !overlap(workspace_dev, need, v_dev, span_bytes(n_tokens, A.v_stride, val, size)) && !overlap(workspace_dev, need, gate_dev, rows) && !overlap(workspace_dev, need, beta_dev, rows) &&
+                   !overlap(workspace_dev, need, cu_seqlens_dev, (n_seqs + 1ull) * 4u) && !overlap(workspace_dev, need, slots_dev, (uint64_t)n_seqs * 4u),
+                   "delta rule: the workspace overlaps rows, states, outputs, bounds or slots");
     }
     if (!require_device()) return 0;
     if (!n_tokens) return 1;

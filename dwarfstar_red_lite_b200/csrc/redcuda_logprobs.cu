@@ -367,8 +367,8 @@ int redcuda_token_logprobs_device(uint32_t type, uint32_t rows, uint32_t vocab, 
                                   float *logprob_dev, float *entropy_dev, int32_t *top_ids_dev, float *top_logprobs_dev, void *stream) {
     if (!logprobs_check(type, rows, vocab, row_stride, logits_dev, tokens_dev, top_n, logprob_dev, top_ids_dev, top_logprobs_dev)) return 0;
     const uint64_t lb = span_bytes(rows, row_stride, vocab, val_size(type)), ob = (uint64_t)rows * 4u;
-    RC_REQUIRE(!overlap(logits_dev, lb, logprob_dev, ob) && !overlap(logits_dev, lb, entropy_dev, ob) && !overlap(logits_dev, lb, top_ids_dev, ob * top_n) &&
-               !overlap(logits_dev, lb, top_logprobs_dev, ob * top_n), "token logprobs: an output lies inside the logits");
+    const Span written[4] = {{logprob_dev, ob}, {entropy_dev, ob}, {top_ids_dev, ob * top_n}, {top_logprobs_dev, ob * top_n}}, read[2] = {{logits_dev, lb}, {tokens_dev, ob}};
+    RC_REQUIRE(!spans_overlap(written, read), "token logprobs: an output lies inside the logits, the tokens or another output");
     RC_REQUIRE(aligned4(tokens_dev) && aligned4(logprob_dev) && aligned4(entropy_dev) && aligned4(top_ids_dev) && aligned4(top_logprobs_dev), "token logprobs: tokens or outputs are not 4-byte aligned");
     if (!require_device()) return 0;
     if (!rows) return 1;

@@ -765,6 +765,8 @@ int redcuda_kv_append_device(const redcuda_paged_kv *kv, const int32_t *table_de
     RC_REQUIRE(aligned4(table_dev) && aligned4(start_dev) && aligned4(cu_seqlens_dev), "kv append: whole numbers are not 4-byte aligned");
     const uint64_t bytes = span_bytes(n_tokens, row_stride, row, val_size(in_type));
     RC_REQUIRE(!kv_overlap(kv, st, k_dev, bytes) && !kv_overlap(kv, st, v_dev, bytes), "kv append: the rows lie inside the cache");
+    RC_REQUIRE(!kv_overlap(kv, st, table_dev, (uint64_t)n_seqs * table_width * 4u) && !kv_overlap(kv, st, start_dev, (uint64_t)n_seqs * 4u) && !kv_overlap(kv, st, cu_seqlens_dev, (n_seqs + 1ull) * 4u),
+               "kv append: the page table, starts or bounds lie inside the cache");
     if (!require_device()) return 0;
     if (!n_tokens) return 1;
     AppendArgs A{kv->k, kv->v, st[0], st[1], st[2], table_dev, start_dev, cu_seqlens_dev, k_dev, v_dev, row_stride, table_width, kv->page_size, kv->n_pages, n_seqs, n_tokens, kv->n_kv,
@@ -811,8 +813,11 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     RC_REQUIRE(!kv_overlap(kv, st, out_dev, out_bytes) && !kv_overlap(kv, st, q_dev, span_bytes(n_seqs, q_stride, qrow, qs)) && !kv_overlap(kv, st, workspace_dev, workspace_bytes) &&
                !kv_overlap(kv, st, k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) && !kv_overlap(kv, st, v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) &&
                !kv_overlap(kv, st, lse_dev, (uint64_t)n_seqs * n_q * 4u), "kv attend: rows, output or workspace lie inside the cache");
-    RC_REQUIRE(!overlap(workspace_dev, workspace_bytes, out_dev, out_bytes) && !overlap(workspace_dev, workspace_bytes, lse_dev, (uint64_t)n_seqs * n_q * 4u) &&
-               !overlap(out_dev, out_bytes, lse_dev, (uint64_t)n_seqs * n_q * 4u), "kv attend: output, lse and workspace overlap");
+    const Span written[3] = {{out_dev, out_bytes}, {lse_dev, (uint64_t)n_seqs * n_q * 4u}, {workspace_dev, workspace_bytes}};
+    const Span read[5] = {{q_dev, span_bytes(n_seqs, q_stride, qrow, qs)}, {k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)}, {v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)},
+                          {table_dev, (uint64_t)n_seqs * table_width * 4u}, {lens_dev, (uint64_t)n_seqs * 4u}};
+    RC_REQUIRE(!spans_overlap(written, read), "kv attend: output, lse or workspace overlap one another or the inputs");
+    RC_REQUIRE(!kv_overlap(kv, st, table_dev, read[3].n) && !kv_overlap(kv, st, lens_dev, read[4].n), "kv attend: the page table or the lengths lie inside the cache");
     RC_REQUIRE(!(scale != scale), "kv attend: scale is not a number");
     if (!require_device()) return 0;
     const uint32_t sms = sm_count();

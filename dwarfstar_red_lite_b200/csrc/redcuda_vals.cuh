@@ -15,6 +15,15 @@ inline bool aligned4(const void *p) { return ((uintptr_t)p & 3u) == 0; }
 inline bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
     return a && b && na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
+struct Span { const void *p; uint64_t n; };
+// whether an array that is written lies in one that is read or in another that is written
+template <int W, int R> inline bool spans_overlap(const Span (&written)[W], const Span (&read)[R]) {
+    for (int i = 0; i < W; ++i) {
+        for (int j = 0; j < R; ++j) if (overlap(written[i].p, written[i].n, read[j].p, read[j].n)) return true;
+        for (int j = 0; j < i; ++j) if (overlap(written[i].p, written[i].n, written[j].p, written[j].n)) return true;
+    }
+    return false;
+}
 // bytes of `rows` rows of n elements that lie `stride` elements apart
 inline uint64_t span_bytes(uint64_t rows, uint64_t stride, uint64_t n, uint32_t size) { return rows ? ((rows - 1u) * stride + n) * size : 0u; }
 // streaming multiprocessors of the current device (0: unknown)

@@ -128,3 +128,30 @@ def test_python_forms_check_shapes():
         rc.delta_rule(z((3, 2, 64)), z((3, 2, 64)), z((3, 4, 64), np.float32), z((3, 4)), z((3, 4)), z((1, 4, 64, 64)))
     with pytest.raises(ValueError):
         rc.token_logprobs(z((3, 10), np.float32), tokens=[1, 2])
+
+
+@pytest.mark.parametrize("change, message", [(dict(work=A[4] + 16), "overlap"), (dict(work=A[2]), "overlap"), (dict(work=A[3]), "overlap"), (dict(out=A[3]), "overlap"), (dict(lse=A[4] + 64), "overlap"),
+                                             (dict(lse=A[2] + 4), "overlap"), (dict(k_new=A[8], v_new=A[7] + 64), "overlap"), (dict(table=A[0] + 64), "inside the cache"),
+                                             (dict(lens=A[1] + 64), "inside the cache")])
+def test_attend_arrays_over_one_another(change, message):
+    _refused(lambda: _attend(**change), message)
+
+
+@pytest.mark.parametrize("change", [dict(table=A[0] + 64), dict(start=A[1]), dict(cu=A[0])])
+def test_append_arrays_inside_the_cache(change):
+    _refused(lambda: _append(**change), "inside the cache")
+
+
+def test_delta_arrays_over_bounds_and_slots():
+    for form in ("rule", "step"):
+        _refused(lambda: _delta(form, out=A[1]), "inside the inputs")
+        _refused(lambda: _delta(form, slots=A[7] + 64), "inside the inputs")
+    _refused(lambda: _delta("rule", cu=A[8]), "inside the inputs")
+    d = rc.DeltaDims(0, 16, 32, 128)
+    for work in (A[0], A[1]):
+        _refused(lambda: rc.lib().redcuda_delta_rule_device(C.byref(d), 5000, 2, A[0], A[1], 4, A[2], A[3], A[4], A[5], A[6], A[7], A[11] * 4, work, d.workspace(5000, 2), None), "the workspace overlaps")
+
+
+@pytest.mark.parametrize("change", [dict(lp=A[1]), dict(ids=A[1] + 8), dict(ent=A[2] + 4), dict(tlp=A[4] + 16), dict(ids=A[2])])
+def test_logprob_outputs_over_one_another(change):
+    _refused(lambda: _logprobs(**change), "lies inside")
