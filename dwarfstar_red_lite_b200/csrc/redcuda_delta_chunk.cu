@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_s
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[i][j][e] *= f;
     }
-    const uint32_t half = warp >> 2, hw = warp & 3u;         // for the inverse, half a block has a value head
+    const uint32_t half = warp >> 2, hw = half ? 3u - (warp & 3u) : warp;         // for the inverse, half a block has a value head; the first block columns have the most to do, so the second half counts backwards: a scheduler has warps w and w + 4
     float *const s_a = reinterpret_cast<float *>(sm + half * 2u * DC_MAT), *const s_t = s_a + DC_T * DC_PITCH;
     float most_c = 0.f;                          // of the warp's products
 #pragma unroll
