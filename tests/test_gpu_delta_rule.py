@@ -423,3 +423,59 @@ def test_rows_of_many_sizes(groups, rank):
     out, state = _rule(x, [0, 300], [0], rc.DeltaDims(0, groups, rank, 128), 1)
     y = dict(x, v=x["v"] / size, state=x["state"] / size[:, :, None])                  # the rows by themselves, which are independent: powers of two are exact
     _close(y, [0, 300], [0], out / size, state / size[:, :, None], 1 / math.sqrt(128))
+
+
+def test_capture_of_few_long_sequences():
+    """As test_capture_and_repeats, with rows enough for the form that has several blocks a state: replayed with other bounds, padded sequences, and sequences shorter than a chunk."""
+    x = _inputs(_gen(19), 700, 2, 4, 128, torch.float16, 4)
+    dims, s = rc.DeltaDims(1, 2, 4, 128), torch.cuda.Stream()
+    state, out = x["state"].clone(), torch.zeros_like(x["v"])
+    cu, slots = torch.tensor([0, 0, 0], dtype=torch.int32, device="cuda"), torch.tensor([2, 0], dtype=torch.int32, device="cuda")
+    work = torch.full((dims.workspace(700, 2),), 0xff, dtype=torch.uint8, device="cuda")
+    call = lambda: rc.delta_rule_device(dims, 700, 2, cu.data_ptr(), slots.data_ptr(), 4, *[x[n].data_ptr() for n in ("q", "k", "v", "gate", "beta")], state.data_ptr(), out.data_ptr(),  # noqa: E731
+                                        work.data_ptr(), work.numel(), s.cuda_stream)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            call()
+        for bounds, who in (([0, 700, 700], [2, 0]), ([0, 0, 700], [1, 3]), ([0, 65, 129], [3, 1]), ([5, 6, 690], [0, 2]), ([0, 350, 700], [-1, 2]), ([0, 0, 0], [2, 0])):
+            cu.copy_(torch.tensor(bounds, dtype=torch.int32))
+            slots.copy_(torch.tensor(who, dtype=torch.int32))
+            state.copy_(x["state"])
+            out.fill_(7.0)
+            graph.replay()
+            s.synchronize()
+            got = out.clone(), state.clone()
+            _close(x, bounds, who, *got, 1 / math.sqrt(128))
+            state.copy_(x["state"])
+            call()
+            s.synchronize()
+            assert torch.equal(out, got[0]) and torch.equal(state, got[1])
+    del graph
+    rc.device_status()
+
+
+@pytest.mark.parametrize("cu, fine", [([0, 600, 400, 800], [True, False, True]), ([0, 100, 999, 800], [True, False, False]), ([-5, 100, 500, 800], [False, True, True])])
+def test_bounds_that_cannot_be_of_few_long_sequences(cu, fine):
+    x = _inputs(_gen(20), 800, 1, 2, 128, torch.float32, 3)
+    out, state = _rule(x, cu, [0, 1, 2], rc.DeltaDims(0, 1, 2, 128), 3)
+    with pytest.raises(rc.RedcudaError, match="bounds"):
+        rc.device_status()
+    for b in range(3):
+        if not fine[b]:
+            assert torch.equal(state[b], x["state"][b])
+        elif not any(fine[o] and o != b and cu[o] < cu[b + 1] and cu[b] < cu[o + 1] for o in range(3)):         # of rows that two sequences claim nothing is said
+            y = {n: (a[cu[b]:cu[b + 1]] if n != "state" else a[b:b + 1]) for n, a in x.items()}
+            T = cu[b + 1] - cu[b]
+            _, want, most = _reference(y, [0, T], [0], 1 / math.sqrt(128))
+            assert float((state[b].double() - want[0]).abs().max()) <= 8 * math.sqrt(T + 16) * 2.0 ** -22 * (most + float(y["v"].abs().max()))
+
+
+def test_slots_that_cannot_be_of_few_long_sequences():
+    x = _inputs(_gen(22), 1100, 1, 2, 128, torch.bfloat16, 3)
+    slots, cu = [1, 3, 1, -2], [0, 500, 700, 900, 1100]
+    out, state = _rule(x, cu, slots, rc.DeltaDims(30, 1, 2, 128), 3)
+    with pytest.raises(rc.RedcudaError, match="slot"):
+        rc.device_status()
+    _close(x, cu, [1, -1, -1, -1], out, state, 1 / math.sqrt(128))
