@@ -78,7 +78,7 @@ template <class C> static int launch_append_rows(const AppendArgs &A, uint32_t i
 //
 // What bounds it is the cache's bytes (504 MB of two long documents: 89 us, 5.6 TB/s; 77 us at the measured copy rate) and, for short sequences, the beginning and end of each head (some 3 us
 // a block: lengths, page table, queries, rows, each a read that waits for the one before).
-// The work is cut by bytes: a tile is 16 KB of K and V of one K/V head, all tiles of all (sequence, K/V head, group of 8 query heads) are
+// The work is cut by bytes: a tile is 16 KB (8 of some caches of floats) of K and V of one K/V head, all tiles of all (sequence, K/V head, group of 8 query heads) are
 // counted through in that order, and every block takes an equal run of them, whatever the lengths are: they are read on the device, so that a
 // captured call follows them. A head costs as much as some tiles more (KV_HEAD_COST). A run that begins or ends inside a sequence's head leaves (m, l, O) in the workspace, at most two of them a
 // block, for k_kv_attend_join; what a block has whole it writes itself. A warp has a ring of tiles of its own, so that the warps of a block meet only where a head ends.
@@ -94,7 +94,7 @@ __device__ __forceinline__ uint32_t kv_len(const AttendArgs &A, uint32_t b) {
 
 // What a head counts in the deal: its tiles, and as many more as its begin and end take (KV_HEAD_COST). Those come first: a run that ends among them leaves
 // the whole head to the next block.
-template <uint32_t TP> __device__ __forceinline__ uint32_t kv_cost(uint32_t len) { return len ? (len + TP - 1u) / TP + KV_HEAD_COST : 0u; }
+template <class L> __device__ __forceinline__ uint32_t kv_cost(uint32_t len) { return len ? (len + L::TP - 1u) / L::TP + KV_HEAD_COST : 0u; }
 
 // One tile of a warp's ring: its rows requested, rows beyond the end or without a page as zeros. Returns the rows that count, as bits.
 template <class T, int HD>
@@ -457,7 +457,7 @@ __device__ __forceinline__ void kv_write_new(const AttendArgs &A, uint32_t b, ui
 
 // NH: heads that a group can have (4 only for a cache of floats)
 template <class T, class QT, int HD, int NH>
-__global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend(AttendArgs A) {
+__global__ void __launch_bounds__(KV_WARPS * 32, kv_blocks(sizeof(T), HD)) k_kv_attend(AttendArgs A) {
     pdl_prologue();
     using L = KvTile<T, HD>;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend(AttendAr
     // how many tiles there are, and the sequence in which this block's run begins
     const uint32_t per = (A.n_seqs + KV_WARPS * 32u - 1u) / (KV_WARPS * 32u), b_lo = min(A.n_seqs, tid * per), b_hi = min(A.n_seqs, b_lo + per);
     uint64_t mine = 0;
-    for (uint32_t b = b_lo; b < b_hi; ++b) mine += kv_cost<L::TP>(kv_len(A, b));
+    for (uint32_t b = b_lo; b < b_hi; ++b) mine += kv_cost<L>(kv_len(A, b));
     uint64_t incl = mine;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) { const uint64_t x = __shfl_up_sync(0xffffffffu, incl, w); if (lane >= (uint32_t)w) incl += x; }
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend(AttendAr
     uint64_t base = (incl - mine) * HG;
     if (u0 < u1 && base <= u0 && u0 < incl * HG) {
         uint32_t b = b_lo;
-        for (;; ++b) { const uint64_t n = (uint64_t)kv_cost<L::TP>(kv_len(A, b)) * HG; if (u0 < base + n) break; base += n; }
+        for (;; ++b) { const uint64_t n = (uint64_t)kv_cost<L>(kv_len(A, b)) * HG; if (u0 < base + n) break; base += n; }
         s_b = b; s_base = base;
     }
     for (uint32_t b = blockIdx.x; b < A.n_seqs; b += gridDim.x) {
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend(AttendAr
         base = s_base;
         uint64_t u = u0;
         while (u < u1) {
-            const uint32_t len = kv_len(A, b), nt = (len + L::TP - 1u) / L::TP, cost = kv_cost<L::TP>(len);
+            const uint32_t len = kv_len(A, b), nt = (len + L::TP - 1u) / L::TP, cost = kv_cost<L>(len);
             if (u >= base + (uint64_t)cost * HG) { base += (uint64_t)cost * HG; ++b; continue; }
             const uint32_t hg = (uint32_t)((u - base) / cost);
             const uint64_t end = base + (uint64_t)(hg + 1u) * cost;             // of this head; its tiles are the last nt units before it
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
 // ---- few heads of moderate length: one launch -----------------------------------------------------------------------------------------
 // A cluster of eight blocks has a head, an eighth of its tiles each; their parts meet in shared memory, block r sums up query head r. What bounds it is the chain of reads; its figures stand at the rule (KV_CLUSTER_HEADS).
 template <class T, class QT, int HD, int NH>
-__global__ void __launch_bounds__(KV_WARPS * 32, KV_BLOCKS) k_kv_attend_cluster(AttendArgs A) {
+__global__ void __launch_bounds__(KV_WARPS * 32, kv_blocks(sizeof(T), HD)) k_kv_attend_cluster(AttendArgs A) {
     pdl_prologue();
     using L = KvTile<T, HD>;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -785,7 +785,7 @@ uint64_t redcuda_kv_attend_workspace(const redcuda_paged_kv *kv, uint32_t n_q) {
     if (!require_device()) return 0;
     const uint32_t sms = sm_count();
     RC_REQUIRE(sms, "kv attend: the device's size is not known");
-    return attend_workspace(sms * KV_BLOCKS, kv->head_dim);
+    return attend_workspace(sms * kv_blocks(val_size(kv->type), kv->head_dim), kv->head_dim);
 }
 
 int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *lens_dev,
@@ -822,7 +822,8 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     if (!require_device()) return 0;
     const uint32_t sms = sm_count();
     RC_REQUIRE(sms, "kv attend: the device's size is not known");
-    RC_REQUIRE(workspace_dev && workspace_bytes >= attend_workspace(sms * KV_BLOCKS, hd), "kv attend: a workspace of %llu bytes is needed", (unsigned long long)attend_workspace(sms * KV_BLOCKS, hd));
+    const uint32_t most_blocks = sms * kv_blocks(val_size(kv->type), hd);
+    RC_REQUIRE(workspace_dev && workspace_bytes >= attend_workspace(most_blocks, hd), "kv attend: a workspace of %llu bytes is needed", (unsigned long long)attend_workspace(most_blocks, hd));
     AttendArgs A{};
     A.k = kv->k; A.v = kv->v; A.page_stride = st[0]; A.token_stride = st[1]; A.head_stride = st[2];
     A.table = table_dev; A.table_width = table_width; A.page_size = kv->page_size; A.n_pages = kv->n_pages;
@@ -831,13 +832,13 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
     A.scale_log2 = (float)((scale == 0.f ? 1.0 / sqrt((double)hd) : (double)scale) * 1.4426950408889634074);
     A.out = out_dev; A.lse = lse_dev; A.status = status_words();
     // no more blocks than there can be runs of tiles
-    const uint64_t tile = 8192u / (hd * val_size(kv->type)), tiles = ((uint64_t)table_width * kv->page_size + tile - 1u) / tile;
+    const uint64_t half = kv_half(val_size(kv->type), hd), tile = half / (hd * val_size(kv->type)), tiles = ((uint64_t)table_width * kv->page_size + tile - 1u) / tile;
     auto few = [](uint64_t n) { return n < 8192u ? n : 8192u; };      // more than that of one thing is blocks enough
     const uint64_t runs = (few(tiles) * few(n_seqs) * few(A.n_kv * A.gsplit) + KV_MIN_TILES - 1u) / KV_MIN_TILES;
-    const uint32_t blocks = runs < sms * KV_BLOCKS ? (uint32_t)runs : sms * KV_BLOCKS;
+    const uint32_t blocks = runs < most_blocks ? (uint32_t)runs : most_blocks;
     // one launch for few heads of moderate length
     const uint64_t heads = (uint64_t)n_seqs * A.n_kv * A.gsplit;
-    const uint64_t most_tiles = (uint64_t)KV_CLUSTER * KV_WARPS * (kv->type == VT_F32 ? KV_CLUSTER_TILES_F32 : KV_CLUSTER_TILES);
+    const uint64_t most_tiles = (uint64_t)KV_CLUSTER * KV_WARPS * (kv->type == VT_F32 ? KV_CLUSTER_TILES_F32 * (8192u / half) : KV_CLUSTER_TILES);
     A.clusters = heads <= KV_CLUSTER_HEADS && heads * KV_CLUSTER <= (uint64_t)sms * KV_BLOCKS && tiles <= most_tiles ? (uint32_t)heads : 0u;
     A.meta = (uint32_t *)workspace_dev;
     A.part = (float *)(A.meta + (size_t)blocks * 4u);

@@ -7,6 +7,8 @@ namespace rc {
 // Warps and stages of a block, blocks of a multiprocessor: twelve stages of 16 KB an SM in every form. Six warps x two stages x one block: two documents of 131072 and some 115000 positions 86 us, 64 ragged
 // sequences 22, 238 of 147 positions 42, 205 of up to 33 36; three x two x two 89, 20, 35, 24 (one block's head begins or ends while the other's tiles flow); two x three x two 90, 21, 36, 25;
 // two x two x three 93, 21, 34, 22.
+// Caches of floats with heads of up to 128 wait for their arithmetic, not for bytes, and have the registers for twelve warps an SM: tiles of 8 KB and twice the blocks. us, 16 KB x two blocks -> 8 KB x four: heads of 128, 32 over 8, 24 sequences
+// of 500 to 1999 positions 48.8 -> 45.7, 64 of up to 2048 42.8 -> 32.5, 200 of up to 40 31 -> 23, 4 of 30000 to 60000 242 -> 234; 64 over 8 76 -> 60; heads of 64, 8 over 8 37.9 -> 29.5.
 constexpr int KV_WARPS = 3, KV_STAGES = 2, KV_BLOCKS = 2;
 constexpr uint32_t KV_HEAD_COST = 12u;           // what a head's begin and end take, in tiles
 constexpr uint32_t KV_MIN_TILES = 3u;            // tiles that a block takes at least: one a warp
@@ -30,10 +32,12 @@ struct AttendArgs {
     float scale_log2;
 };
 
-// A tile: 8 KB of K rows, then 8 KB of V rows, the 16-byte pieces of a row turned by its number so that eight rows' pieces of one column lie in
+// A tile: 8 KB (or 4) of K rows, then as much of V rows, the 16-byte pieces of a row turned by its number so that eight rows' pieces of one column lie in
 // different banks.
+constexpr uint32_t kv_half(uint32_t size, uint32_t hd) { return size == 4u && hd <= 128u ? 4096u : 8192u; }
+constexpr uint32_t kv_blocks(uint32_t size, uint32_t hd) { return KV_BLOCKS * (8192u / kv_half(size, hd)); }
 template <class T, int HD> struct KvTile {
-    static constexpr uint32_t ROW = HD * sizeof(T), TP = 8192u / ROW, CPR = ROW / 16u, BYTES = 2u * 8192u;
+    static constexpr uint32_t HALF = kv_half(sizeof(T), HD), ROW = HD * sizeof(T), TP = HALF / ROW, CPR = ROW / 16u, BYTES = 2u * HALF;
     static constexpr int TPL = TP > 32u ? 2 : 1;         // rows that a lane looks up
     static_assert(TP * CPR % 32u == 0u && TP >= 8u && TP <= 64u && CPR >= 8u, "tile");
     static __device__ __forceinline__ uint32_t swizzle(uint32_t row, uint32_t c) { return c ^ (row & 7u); }
