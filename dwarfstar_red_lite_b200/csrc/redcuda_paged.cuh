@@ -9,6 +9,7 @@ namespace rc {
 // two x two x three 93, 21, 34, 22.
 // Caches of floats with heads of up to 128 wait for their arithmetic, not for bytes, and have the registers for twelve warps an SM: tiles of 8 KB and twice the blocks. us, 16 KB x two blocks -> 8 KB x four: heads of 128, 32 over 8, 24 sequences
 // of 500 to 1999 positions 48.8 -> 45.7, 64 of up to 2048 42.8 -> 32.5, 200 of up to 40 31 -> 23, 4 of 30000 to 60000 242 -> 234; 64 over 8 76 -> 60; heads of 64, 8 over 8 37.9 -> 29.5.
+// 16-bit caches with heads of 128 lose by the same what they gain: 200 of up to 40 28 -> 22, 64 of up to 2048 24.2 -> 22.6, 1 of 8000 12.8 -> 14.8, 24 of 500 to 1999 26.5 -> 28.1.
 constexpr int KV_WARPS = 3, KV_STAGES = 2, KV_BLOCKS = 2;
 constexpr uint32_t KV_HEAD_COST = 12u;           // what a head's begin and end take, in tiles
 constexpr uint32_t KV_MIN_TILES = 3u;            // tiles that a block takes at least: one a warp
