@@ -67,7 +67,7 @@ __device__ __forceinline__ void dc_mma(float (&c)[4], const uint32_t (&a)[4], ui
 // of 16: those on the diagonal by substitution, a column a lane; the others T_ij = -T_ii sum_k A_ik T_kj, a column of blocks a warp, which is as stable as substitution (powers of A are not, where
 // keys are alike). The digits of T and P have a power of two for 16 rows each, so that no warp waits for another's largest.
 // What bounds it is latency: a dozen short phases between barriers, hence three blocks an SM. 16 key heads with 2 value heads each: a prompt of 2000 tokens in F32 (512 blocks) 45 us, twelve prompts
-// of 16384 tokens together in BF16 (some 4200 blocks) 180 us. One exponent for a chunk's keys and one for its queries: a key 2^17 smaller than the largest still has its 22 bits, a smaller one loses some.
+// of 16384 tokens together in BF16 (some 4200 blocks) 178 us. One exponent for a chunk's keys and one for its queries: a key 2^17 smaller than the largest still has its 22 bits, a smaller one loses some.
 constexpr uint32_t DC_PITCH = 68u;               // floats of a row of the 64 x 64 matrices in shared memory
 constexpr uint32_t DC_MAT = DC_T * DC_PITCH * 4u;
 __device__ __forceinline__ void dc_half_sync(uint32_t half) { asm volatile("bar.sync %0, 128;" :: "r"(half + 1u) : "memory"); }
