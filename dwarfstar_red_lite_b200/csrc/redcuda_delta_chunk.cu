@@ -31,8 +31,61 @@ static_assert(sizeof(DcMeta) == 1024, "copied in whole");
 constexpr uint32_t DC_REC = 4u * DC_SQ + (uint32_t)sizeof(DcMeta);       // T hi, T lo, P hi, P lo, meta
 __host__ __device__ constexpr uint32_t dc_keys(int dig) { return (uint32_t)dig * (DC_KQ + DC_KT); }      // KQ hi (, lo), KT hi (, lo)
 
-// Chunks are numbered so that a sequence finds its own without the lengths of the others: chunk c of sequence b is number cu[b] / 64 + b + c.
+// A call's chunks are numbered through, sequence by sequence. Bounds that cannot be count no chunk, so that the others' numbers are theirs alone whatever those are. Sequences that have no rows in common
+// have n_tokens / 64 + n_seqs chunks at most; one whose chunks lie beyond that (others claim the same rows) is left out.
+// The number of each sequence's first chunk stands in the workspace (the plan), for the kernels that take the states through: k_delta_plan writes it, or for up to DC_NEAR sequences the first block of
+// k_delta_prep, whose warps then count for themselves, a sequence a lane.
+constexpr uint32_t DC_NEAR = 32u;
 static uint64_t dc_slots(uint32_t n_tokens, uint32_t n_seqs) { return (uint64_t)n_tokens / DC_T + n_seqs; }
+__device__ __forceinline__ uint32_t dc_chunks(int32_t lo, int32_t hi, uint32_t n_tokens) {
+    return lo < 0 || hi < lo || (uint32_t)hi > n_tokens ? 0u : ((uint32_t)(hi - lo) + DC_T - 1u) / DC_T;
+}
+__device__ __forceinline__ uint32_t dc_warp_sum_to(uint32_t x) {             // of the lanes up to this one
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, x, w); if (lane >= (uint32_t)w) x += y; }
+    return x;
+}
+// the sequence that chunk number `slot` belongs to and which of its chunks that is, or false: none (for a whole warp)
+__device__ __forceinline__ bool dc_find(const DeltaArgs &A, uint32_t n_seqs, uint32_t *plan, uint32_t slot, uint32_t &b, uint32_t &chunk) {
+    const uint32_t lane = threadIdx.x & 31u;
+    if (n_seqs <= DC_NEAR) {
+        const uint32_t n = lane < n_seqs ? dc_chunks(A.cu[lane], A.cu[lane + 1u], A.n_tokens) : 0u, end = dc_warp_sum_to(n), m = __ballot_sync(0xffffffffu, slot < end);
+        if (slot == 0u && blockIdx.y == 0u && threadIdx.x < n_seqs) plan[threadIdx.x] = end - n;
+        if (!m) return false;
+        b = (uint32_t)__ffs((int)m) - 1u;
+        chunk = slot - __shfl_sync(0xffffffffu, end - n, (int)b);
+        return true;
+    }
+    uint32_t cnt = n_seqs;                       // the last sequence whose first chunk is no later: one that has chunks, unless slot is behind the last
+    b = 0u;
+    while (cnt > 1u) {
+        const uint32_t step = (cnt + 31u) / 32u, i = lane * step, m = __ballot_sync(0xffffffffu, i < cnt && plan[b + i] <= slot), at = (31u - (uint32_t)__clz((int)m)) * step;
+        cnt = min(step, cnt - at); b += at;
+    }
+    chunk = slot - plan[b];
+    return chunk < dc_chunks(A.cu[b], A.cu[b + 1u], A.n_tokens);
+}
+
+// One block: the first chunks' numbers of more than DC_NEAR sequences. A thread has a run of them; 60000 sequences take no thousandth of their call.
+__global__ void __launch_bounds__(1024) k_delta_plan(DeltaArgs A, uint32_t n_seqs, uint32_t *plan) {
+    pdl_prologue();
+    __shared__ uint64_t s_sum[32];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, per = (n_seqs + 1023u) / 1024u, b0 = min(n_seqs, tid * per), b1 = min(n_seqs, b0 + per);
+    uint64_t mine = 0u;
+    for (uint32_t b = b0; b < b1; ++b) mine += dc_chunks(A.cu[b], A.cu[b + 1u], A.n_tokens);
+    uint64_t at = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) { const uint64_t y = __shfl_up_sync(0xffffffffu, at, w); if (lane >= (uint32_t)w) at += y; }
+    if (lane == 31u) s_sum[tid >> 5] = at;
+    __syncthreads();
+    for (uint32_t w = 0; w < tid >> 5; ++w) at += s_sum[w];
+    at -= mine;
+    for (uint32_t b = b0; b < b1; ++b) {
+        plan[b] = (uint32_t)min(at, (uint64_t)0xffffffffu);
+        at += dc_chunks(A.cu[b], A.cu[b + 1u], A.n_tokens);
+    }
+}
 
 __device__ __forceinline__ uint32_t dc_kq_at(uint32_t row, uint32_t piece) { return piece * 2048u + row * 16u; }       // of KQ, and of KT
 __device__ __forceinline__ uint32_t dc_sq_at(uint32_t row, uint32_t piece) { return piece * 1024u + row * 16u; }
@@ -108,7 +161,7 @@ __device__ __forceinline__ void dc_block_product(float (&c)[2][4], const uint32_
 
 // WIDE: more than two value heads a key head (the products are then kept for the next two)
 template <class T, int DIG, bool WIDE>
-__global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_seqs, uint8_t *ws, uint64_t slots) {
+__global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_seqs, uint8_t *ws, uint64_t slots, uint32_t *plan) {
     pdl_prologue();
     extern __shared__ __align__(128) uint8_t sm[];           // the digits; then the matrices A and T of two value heads
     __shared__ float s_red[2][8], s_beta[2][DC_T], s_diag[2][4], s_amax[2][4], s_peak[2];
@@ -116,19 +169,10 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_s
     __shared__ uint32_t s_bad[2][2];             // tokens whose key or query is not finite
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, kh = blockIdx.y, width = A.rank / A.groups;
     const uint64_t slot = blockIdx.x;
-    // the sequence: the last b with cu[b] / 64 + b <= slot
-    uint32_t b = 0u, cnt = n_seqs;
-    while (cnt > 1u) {
-        const uint32_t step = (cnt + 31u) / 32u, i = lane * step;
-        const bool le = i < cnt && (int64_t)(A.cu[b + i] / DC_T) + (int64_t)(b + i) <= (int64_t)slot;
-        const uint32_t m = __ballot_sync(0xffffffffu, le), at = (m ? 31u - (uint32_t)__clz((int)m) : 0u) * step;
-        cnt = min(step, cnt - at); b += at;
-    }
+    uint32_t b, chunk;
+    if (!dc_find(A, n_seqs, plan, blockIdx.x, b, chunk)) return;
     const int32_t lo = A.cu[b], hi = A.cu[b + 1u];
-    if (lo < 0 || hi < lo || (uint32_t)hi > A.n_tokens) return;          // reported by k_delta_chunk
-    const int64_t chunk = (int64_t)slot - (int64_t)(lo / DC_T) - (int64_t)b;
-    if (chunk < 0 || chunk * DC_T >= hi - lo) return;
-    const uint32_t t0 = (uint32_t)lo + (uint32_t)chunk * DC_T, n = min((uint32_t)DC_T, (uint32_t)hi - t0);
+    const uint32_t t0 = (uint32_t)lo + chunk * DC_T, n = min((uint32_t)DC_T, (uint32_t)hi - t0);
     uint8_t *const keys = ws + (slot * A.groups + kh) * dc_keys(DIG), *const recs = ws + slots * A.groups * dc_keys(DIG) + slot * A.rank * DC_REC;
     const uint32_t dv = warp == 0u ? 0u : warp == 7u ? 1u : 2u;          // the value head of a pair whose decays this warp makes (2: none): the warps with the fewest products
 
@@ -537,7 +581,7 @@ __device__ __forceinline__ void dc_put32(const float *x, float f, uint32_t hi, u
 }
 
 template <class T, int DIG>
-__global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots) {
+__global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, const uint32_t *plan) {
     pdl_prologue();
     constexpr uint32_t KEYS = dc_keys(DIG), VROW = DC_S * sizeof(T);
     extern __shared__ __align__(128) uint8_t sm[];
@@ -564,7 +608,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
     const int32_t state_slot = delta_slot(A.slots, A.n_slots, b, A.status);
     if (state_slot < 0 || lo == hi) return;
     const uint32_t chunks = ((uint32_t)(hi - lo) + DC_T - 1u) / DC_T;
-    const uint64_t slot0 = (uint64_t)(lo / DC_T) + b;
+    if (plan[b] + (uint64_t)chunks > slots) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
     uint8_t *const s_kq = sm, *const s_kt = sm + DIG * DC_KQ, *const s_tt = sm + KEYS, *const s_pp = s_tt + 2u * DC_SQ, *const s_meta = s_tt + 4u * DC_SQ;
     T *const s_v = reinterpret_cast<T *>(s_meta + 2u * sizeof(DcMeta)), *const s_out = s_v + DC_T * DC_S;          // [token][row]
     auto bar = [&](uint32_t i) { return dc_smem(&s_bar[i]); };
@@ -592,6 +636,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(DC_REGS_CONTROL));
         if (warp == DC_CONTROL) {
             const uint32_t leader = tc_elect();
+            const uint64_t slot0 = plan[b];          // here: the warps of the rows have no register for it
             const uint8_t *key = ws + (slot0 * A.groups + kh) * KEYS, *rec = ws + slots * A.groups * KEYS + (slot0 * A.rank + h) * DC_REC;      // the next chunk's, as each is asked for
             const uint64_t key_step = (uint64_t)A.groups * KEYS, rec_step = (uint64_t)A.rank * DC_REC;
             auto get_kq = [&](uint32_t c) { if (lane == 0u) { expect(DB_KQ, DIG * DC_KQ); copy(DB_KQ, s_kq, key + c * key_step, DIG * DC_KQ); } };
@@ -906,7 +951,7 @@ __device__ __forceinline__ float dn_most(const float (&x)[16]) {
 }
 
 template <class T, int DIG>
-__global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A, const uint8_t *ws, uint64_t slots) {
+__global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A, const uint8_t *ws, uint64_t slots, const uint32_t *plan) {
     pdl_prologue();
     constexpr uint32_t KEYS = dc_keys(DIG), SPLIT = DC_S / DN_ROWS;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -921,7 +966,8 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A,
     const int32_t state_slot = delta_slot(A.slots, A.n_slots, b, A.status);
     if (state_slot < 0 || lo == hi) return;
     const uint32_t chunks = ((uint32_t)(hi - lo) + DC_T - 1u) / DC_T;
-    const uint64_t slot0 = (uint64_t)(lo / DC_T) + b;
+    const uint64_t slot0 = plan[b];
+    if (slot0 + chunks > slots) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
     uint8_t *const s_kq = sm, *const s_kt = sm + DIG * DC_KQ, *const s_tp = sm + KEYS, *const s_s = s_tp + 2u * DN_SQ, *const s_r = s_s + 2u * DN_STILE, *const s_d = s_r + 2u * DN_TILE, *const s_dk = s_d + 2u * DN_TILE,
                   *const s_meta = s_dk + 2u * DN_TILE;
     const uint8_t *const key = ws + (slot0 * A.groups + kh) * KEYS, *const rec = ws + slots * A.groups * KEYS + (slot0 * A.rank + h) * DC_REC;
@@ -1207,17 +1253,18 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A,
     if (warp == DN_CONTROL) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((uint32_t)NT_COLS) : "memory");
 }
 
+static uint64_t dc_records(int dig, uint32_t groups, uint32_t rank, uint64_t slots) { return slots * ((uint64_t)groups * dc_keys(dig) + (uint64_t)rank * DC_REC); }
 uint64_t delta_chunk_workspace(uint32_t type, uint32_t groups, uint32_t rank, uint32_t n_tokens, uint32_t n_seqs) {
-    return dc_slots(n_tokens, n_seqs) * ((uint64_t)groups * dc_keys(type == VT_F32 ? 2 : 1) + (uint64_t)rank * DC_REC);
+    return dc_records(type == VT_F32 ? 2 : 1, groups, rank, dc_slots(n_tokens, n_seqs)) + n_seqs * 4ull;
 }
 
-template <class T, int DIG> static int launch_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, cudaStream_t s) {
+template <class T, int DIG> static int launch_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, const uint32_t *plan, cudaStream_t s) {
     // Four blocks a state where that gives no multiprocessor two, and sequences of four chunks on the average: 32 heads, 1 sequence of 64 tokens 25.6 -> 27.5 us in F32 (21.5 -> 21.0 in BF16), of 128 30 -> 34 (24 -> 27), of 256
     // 40 -> 41 (33 -> 32), of 500 56 -> 52 (49 -> 43), of 2000 172 -> 136 (156 -> 131), of 8000 606 -> 519 (561 -> 482), each with the preparation. In two turns four blocks would take 5.5 us a chunk, one takes 4.
     if ((uint64_t)A.rank * n_seqs * (DC_S / DN_ROWS) <= sm_count() && A.n_tokens >= 256u * (uint64_t)n_seqs) {
         static std::atomic<uint64_t> set_rows{0};
         if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_chunk_rows<T, DIG>), dn_smem_bytes(DIG), set_rows)) return 0;
-        RC_LAUNCH((k_delta_chunk_rows<T, DIG>), dim3(A.rank * (DC_S / DN_ROWS), n_seqs), DN_THREADS, dn_smem_bytes(DIG), s, A, ws, slots);
+        RC_LAUNCH((k_delta_chunk_rows<T, DIG>), dim3(A.rank * (DC_S / DN_ROWS), n_seqs), DN_THREADS, dn_smem_bytes(DIG), s, A, ws, slots, plan);
         RC_LAUNCHED();
         return 1;
     }
@@ -1225,7 +1272,7 @@ template <class T, int DIG> static int launch_chunk(DeltaArgs A, uint32_t n_seqs
     if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_chunk<T, DIG>), dc_smem_bytes(DIG, sizeof(T)), set)) return 0;
     for (uint32_t b = 0; b < n_seqs; b += 65535u) {
         A.first_seq = b;
-        RC_LAUNCH((k_delta_chunk<T, DIG>), dim3(A.rank, n_seqs - b < 65535u ? n_seqs - b : 65535u), DC_THREADS, dc_smem_bytes(DIG, sizeof(T)), s, A, n_seqs, ws, slots);
+        RC_LAUNCH((k_delta_chunk<T, DIG>), dim3(A.rank, n_seqs - b < 65535u ? n_seqs - b : 65535u), DC_THREADS, dc_smem_bytes(DIG, sizeof(T)), s, A, n_seqs, ws, slots, plan);
         RC_LAUNCHED();
     }
     return 1;
@@ -1234,20 +1281,25 @@ template <class T, int DIG> static int launch_chunks(const DeltaArgs &A, uint32_
     const uint64_t slots = dc_slots(A.n_tokens, n_seqs);
     constexpr size_t smem = 4u * DC_MAT > DIG * DC_KQ ? 4u * DC_MAT : DIG * DC_KQ;
     RC_REQUIRE(slots <= 0x7fffffffu && A.groups <= 65535u, "delta rule: too many chunks");
+    uint32_t *const plan = (uint32_t *)(ws + dc_records(DIG, A.groups, A.rank, slots));
     prof_begin("delta_prep", s);
+    if (n_seqs > DC_NEAR) {
+        RC_LAUNCH(k_delta_plan, 1, 1024, 0, s, A, n_seqs, plan);
+        RC_LAUNCHED();
+    }
     if (A.rank > 2u * A.groups) {
         static std::atomic<uint64_t> set{0};
         if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_prep<T, DIG, true>), smem, set)) return 0;
-        RC_LAUNCH((k_delta_prep<T, DIG, true>), dim3((uint32_t)slots, A.groups), 256, smem, s, A, n_seqs, ws, slots);
+        RC_LAUNCH((k_delta_prep<T, DIG, true>), dim3((uint32_t)slots, A.groups), 256, smem, s, A, n_seqs, ws, slots, plan);
     } else {
         static std::atomic<uint64_t> set{0};
         if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_prep<T, DIG, false>), smem, set)) return 0;
-        RC_LAUNCH((k_delta_prep<T, DIG, false>), dim3((uint32_t)slots, A.groups), 256, smem, s, A, n_seqs, ws, slots);
+        RC_LAUNCH((k_delta_prep<T, DIG, false>), dim3((uint32_t)slots, A.groups), 256, smem, s, A, n_seqs, ws, slots, plan);
     }
     RC_LAUNCHED();
     prof_end(s);
     prof_begin("delta_chunk", s);
-    const int ok = launch_chunk<T, DIG>(A, n_seqs, ws, slots, s);
+    const int ok = launch_chunk<T, DIG>(A, n_seqs, ws, slots, plan, s);
     prof_end(s);
     return ok;
 }

@@ -314,7 +314,7 @@ int redcuda_delta_step_device(const redcuda_delta_dims *d, uint32_t n_seqs, cons
 
 /* Prompts laid end to end: tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of the n_tokens rows are sequence b's, in order (n_seqs + 1 ascending numbers on
  * the device; a sequence may be empty; rows from cu_seqlens[n_seqs] on are left as they were). Bounds that fall or leave the rows are reported and their sequence left out;
- * of sequences that then claim the same rows, outputs and states are not defined. A value that is not finite makes what depends on it NaN, from its token on. In longer calls
+ * of sequences that then claim the same rows, outputs and states are not defined (where they claim more than the workspace has room for, sequences behind them are reported and left out too). A value that is not finite makes what depends on it NaN, from its token on. In longer calls
  * (those that need a workspace) the keys of 64 tokens share an exponent in the products, as do their queries and 32 rows of values or of the
  * state: one 2^17 smaller than the largest beside it keeps 22 bits, smaller ones fewer. Slots as above. workspace_dev:
  * redcuda_delta_rule_workspace bytes, 16-byte aligned (0: none is needed); calls that overlap on the GPU need one each. */
