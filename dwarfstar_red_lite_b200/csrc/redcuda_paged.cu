@@ -32,14 +32,15 @@ __global__ void __launch_bounds__(128) k_kv_append(AppendArgs A) {
     pdl_prologue();
     constexpr int VEC = 16 / sizeof(C), PART = 16 / sizeof(R) < VEC ? 16 / sizeof(R) : VEC;
     const uint32_t lane = threadIdx.x & 31u, t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (A.cu && A.status)                        // a thread looks at every so many-th sequence's bounds
+        for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < A.n_seqs; i += (uint64_t)gridDim.x * blockDim.x)       // up to 2^36 threads
+            if (!seq_bounds(A.cu, (uint32_t)i, A.n_tokens)) A.status[ST_SEQ_BOUNDS] = 1u;
     if (t >= A.n_tokens) return;
     uint32_t b = t, at = 0u;
     if (A.cu) {
-        b = find_seq(A.cu, A.n_seqs, t);
-        if (b >= A.n_seqs) return;               // behind the last sequence
-        const int32_t lo = A.cu[b], hi = A.cu[b + 1u];
-        if (lo < 0 || (int32_t)t < lo || (int32_t)t >= hi) { if (A.status && lane == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
-        at = t - (uint32_t)lo;
+        b = find_seq(A.cu, A.n_seqs, t, A.n_tokens);
+        if (b >= A.n_seqs) return;               // of no sequence
+        at = t - (uint32_t)A.cu[b];
     }
     const int32_t s = A.start[b];
     if (s < 0) return;

@@ -71,22 +71,27 @@ template <int N, class T> __device__ __forceinline__ void store_vals(T *p, const
     *reinterpret_cast<Pack<T, N> *>(p) = a;
 }
 
-// The sequence that row t belongs to: the last b with cu[b] <= t, found by a whole warp, 32 entries a step; n_seqs or more: behind the last one,
-// ~0u: ahead of the first. Only ascending bounds are searched right; others give some b, which the caller holds against cu[b] and cu[b + 1].
-__device__ __forceinline__ uint32_t find_seq(const int32_t *cu, uint32_t n_seqs, uint32_t t) {
+// whether the bounds of sequence b ascend within n rows
+__device__ __forceinline__ bool seq_bounds(const int32_t *cu, uint32_t b, uint32_t n) {
+    const int32_t lo = cu[b], hi = cu[b + 1u];
+    return lo >= 0 && hi >= lo && (uint32_t)hi <= n;
+}
+// The sequence with right bounds that row t of n belongs to, found by a whole warp; n_seqs: none. Ascending bounds are searched 32 at a step. Where that gives no such sequence (the row is of none,
+// or some bound is wrong and the search was led astray) all are looked at, 32 at a time: 256 sequences are eight reads that do not wait for one another.
+__device__ __forceinline__ uint32_t find_seq(const int32_t *cu, uint32_t n_seqs, uint32_t t, uint32_t n) {
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t lo = 0u, n = n_seqs + 1u;           // entries lo .. lo + n - 1 are open
-    bool first = true;
-    while (n > 1u || first) {
-        const uint32_t step = (n + 31u) / 32u, i = lane * step;
-        const bool le = i < n && cu[lo + i] <= (int32_t)t;
-        const uint32_t m = __ballot_sync(0xffffffffu, le);
-        if (first && !(m & 1u)) return ~0u;
-        first = false;
-        const uint32_t at = (m ? 31u - (uint32_t)__clz((int)m) : 0u) * step;
-        n = min(step, n - at); lo += at;
+    uint32_t lo = 0u, cnt = n_seqs;              // entries lo .. lo + cnt - 1 are open
+    while (cnt > 1u) {
+        const uint32_t step = (cnt + 31u) / 32u, i = lane * step, m = __ballot_sync(0xffffffffu, i < cnt && cu[lo + i] <= (int32_t)t), at = (m ? 31u - (uint32_t)__clz((int)m) : 0u) * step;
+        cnt = min(step, cnt - at); lo += at;
     }
-    return lo;
+    auto has = [&](uint32_t b) { return seq_bounds(cu, b, n) && (int32_t)t >= cu[b] && (int32_t)t < cu[b + 1u]; };
+    if (has(lo)) return lo;
+    for (uint32_t b = 0u; b < n_seqs; b += 32u) {
+        const uint32_t m = __ballot_sync(0xffffffffu, b + lane < n_seqs && has(b + lane));
+        if (m) return b + (uint32_t)__ffs((int)m) - 1u;
+    }
+    return n_seqs;
 }
 #endif
 

@@ -275,7 +275,8 @@ typedef struct {
 
 /* Writes the K/V rows [n_kv][head_dim] (in_type; converted, rounded to nearest even) of n_tokens tokens to the cache. Rows cu_seqlens[b] up to
  * cu_seqlens[b + 1] - 1 are positions start[b], start[b] + 1, ... of sequence b; cu_seqlens NULL: one row per sequence, row b being position
- * start[b] of sequence b. A sequence with a negative start is left out, as are rows from cu_seqlens[n_seqs] on. row_stride: elements between
+ * start[b] of sequence b. A sequence with a negative start is left out, as are rows ahead of the first sequence and behind the last. Bounds that fall or leave the rows are reported
+ * and their sequence left out; a row that two sequences then claim goes to one of them. row_stride: elements between
  * the rows of two tokens, 0 = n_kv * head_dim. Where two sequences of a call write the same position of a page that both have, what it then holds is not defined. */
 int redcuda_kv_append_device(const redcuda_paged_kv *kv, const int32_t *table_dev, uint32_t table_width, uint32_t n_seqs, const int32_t *start_dev,
                              uint32_t n_tokens, const int32_t *cu_seqlens_dev, uint32_t in_type, const void *k_dev, const void *v_dev, uint64_t row_stride,
