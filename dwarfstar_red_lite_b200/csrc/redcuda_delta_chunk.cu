@@ -33,9 +33,9 @@ __host__ __device__ constexpr uint32_t dc_keys(int dig) { return (uint32_t)dig *
 
 // A call's chunks are numbered through, sequence by sequence. Bounds that cannot be count no chunk, so that the others' numbers are theirs alone whatever those are. Sequences that have no rows in common
 // have n_tokens / 64 + n_seqs chunks at most; one whose chunks lie beyond that (others claim the same rows) is left out.
-// The number of each sequence's first chunk stands in the workspace (the plan), for the kernels that take the states through: k_delta_plan writes it, or for up to DC_NEAR sequences the first block of
-// k_delta_prep, whose warps then count for themselves, a sequence a lane.
+// Up to DC_NEAR sequences every block counts for itself, a sequence a lane. Of more, k_delta_plan writes to the workspace what a block needs to know (the plan).
 constexpr uint32_t DC_NEAR = 32u;
+struct alignas(16) DcSeq { uint32_t b, first; int32_t lo, hi; };             // the sequence, the number of its first chunk, its bounds
 static uint64_t dc_slots(uint32_t n_tokens, uint32_t n_seqs) { return (uint64_t)n_tokens / DC_T + n_seqs; }
 __device__ __forceinline__ uint32_t dc_chunks(int32_t lo, int32_t hi, uint32_t n_tokens) {
     return lo < 0 || hi < lo || (uint32_t)hi > n_tokens ? 0u : ((uint32_t)(hi - lo) + DC_T - 1u) / DC_T;
@@ -46,44 +46,84 @@ __device__ __forceinline__ uint32_t dc_warp_sum_to(uint32_t x) {             // 
     for (int w = 1; w < 32; w <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, x, w); if (lane >= (uint32_t)w) x += y; }
     return x;
 }
-// the sequence that chunk number `slot` belongs to and which of its chunks that is, or false: none (for a whole warp)
-__device__ __forceinline__ bool dc_find(const DeltaArgs &A, uint32_t n_seqs, uint32_t *plan, uint32_t slot, uint32_t &b, uint32_t &chunk) {
+// The i-th longest sequence, to shared memory, for the whole block (it meets a barrier). Blocks of long sequences go first.
+__device__ __forceinline__ void dc_seq(const DeltaArgs &A, uint32_t n_seqs, const DcSeq *plan, uint32_t i, DcSeq &to) {
+    const uint32_t lane = threadIdx.x;
+    if (n_seqs > DC_NEAR) {
+        if (lane == 0u) *reinterpret_cast<uint4 *>(&to) = *reinterpret_cast<const uint4 *>(plan + i);
+    } else if (lane < 32u) {
+        int32_t lo = 0, hi = 0;
+        if (lane < n_seqs) { lo = A.cu[lane]; hi = A.cu[lane + 1u]; }
+        const uint32_t n = dc_chunks(lo, hi, A.n_tokens), first = dc_warp_sum_to(n) - n;
+        uint32_t before = 0u;                    // longer ones, and equal ones ahead of it
+        for (uint32_t j = 0; j < n_seqs; ++j) { const uint32_t other = __shfl_sync(0xffffffffu, n, (int)j); before += other > n || (other == n && j < lane); }
+        if (lane < n_seqs && before == i) to = DcSeq{lane, first, lo, hi};
+    }
+    __syncthreads();
+}
+// the plan's second part: the numbers of the sequences' first chunks, in their own order
+template <class P> __device__ __forceinline__ auto dc_firsts(P *plan, uint32_t n_seqs) { return reinterpret_cast<typename std::conditional<std::is_const<P>::value, const uint32_t, uint32_t>::type *>(plan + n_seqs); }
+// the bounds of the sequence that chunk number `slot` belongs to, and which of its chunks that is, or false: none (for a whole warp)
+__device__ __forceinline__ bool dc_find(const DeltaArgs &A, uint32_t n_seqs, const DcSeq *plan, uint32_t slot, int32_t &lo, int32_t &hi, uint32_t &chunk) {
     const uint32_t lane = threadIdx.x & 31u;
     if (n_seqs <= DC_NEAR) {
-        const uint32_t n = lane < n_seqs ? dc_chunks(A.cu[lane], A.cu[lane + 1u], A.n_tokens) : 0u, end = dc_warp_sum_to(n), m = __ballot_sync(0xffffffffu, slot < end);
-        if (slot == 0u && blockIdx.y == 0u && threadIdx.x < n_seqs) plan[threadIdx.x] = end - n;
+        lo = hi = 0;
+        if (lane < n_seqs) { lo = A.cu[lane]; hi = A.cu[lane + 1u]; }
+        const uint32_t n = dc_chunks(lo, hi, A.n_tokens), end = dc_warp_sum_to(n), m = __ballot_sync(0xffffffffu, slot < end);
         if (!m) return false;
-        b = (uint32_t)__ffs((int)m) - 1u;
-        chunk = slot - __shfl_sync(0xffffffffu, end - n, (int)b);
+        const int b = __ffs((int)m) - 1;
+        chunk = slot - __shfl_sync(0xffffffffu, end - n, b);
+        lo = __shfl_sync(0xffffffffu, lo, b); hi = __shfl_sync(0xffffffffu, hi, b);
         return true;
     }
-    uint32_t cnt = n_seqs;                       // the last sequence whose first chunk is no later: one that has chunks, unless slot is behind the last
-    b = 0u;
+    const uint32_t *const firsts = dc_firsts(plan, n_seqs);
+    uint32_t cnt = n_seqs, b = 0u;               // the last sequence whose first chunk is no later: one that has chunks, unless slot is behind the last
     while (cnt > 1u) {
-        const uint32_t step = (cnt + 31u) / 32u, i = lane * step, m = __ballot_sync(0xffffffffu, i < cnt && plan[b + i] <= slot), at = (31u - (uint32_t)__clz((int)m)) * step;
+        const uint32_t step = (cnt + 31u) / 32u, i = lane * step, m = __ballot_sync(0xffffffffu, i < cnt && firsts[b + i] <= slot), at = (31u - (uint32_t)__clz((int)m)) * step;
         cnt = min(step, cnt - at); b += at;
     }
-    chunk = slot - plan[b];
-    return chunk < dc_chunks(A.cu[b], A.cu[b + 1u], A.n_tokens);
+    chunk = slot - firsts[b];
+    lo = A.cu[b]; hi = A.cu[b + 1u];
+    return chunk < dc_chunks(lo, hi, A.n_tokens);
 }
 
-// One block: the first chunks' numbers of more than DC_NEAR sequences. A thread has a run of them; 60000 sequences take no thousandth of their call.
-__global__ void __launch_bounds__(1024) k_delta_plan(DeltaArgs A, uint32_t n_seqs, uint32_t *plan) {
+// One block: the plan of more than DC_NEAR sequences. A thread has a run of them; the order is by number of chunks, those of DC_KINDS and more alike (how they lie among themselves changes no result).
+// 1024 sequences of 64 tokens, 32 heads over 16: 3.2 ms in all; with every block of k_delta_chunk finding its sequence's place for itself 19.4, up to 256 sequences 1.07 -> 0.82.
+constexpr uint32_t DC_KINDS = 1024u;
+__global__ void __launch_bounds__(1024) k_delta_plan(DeltaArgs A, uint32_t n_seqs, DcSeq *plan) {
     pdl_prologue();
     __shared__ uint64_t s_sum[32];
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, per = (n_seqs + 1023u) / 1024u, b0 = min(n_seqs, tid * per), b1 = min(n_seqs, b0 + per);
+    __shared__ uint32_t s_kind[DC_KINDS], s_part[32];        // sequences with so many chunks; where the next of them goes
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, per = (n_seqs + 1023u) / 1024u, b0 = min(n_seqs, tid * per), b1 = min(n_seqs, b0 + per);
+    static_assert(DC_KINDS == 1024u, "one a thread");
+    s_kind[tid] = 0u;
+    __syncthreads();
     uint64_t mine = 0u;
-    for (uint32_t b = b0; b < b1; ++b) mine += dc_chunks(A.cu[b], A.cu[b + 1u], A.n_tokens);
+    for (uint32_t b = b0; b < b1; ++b) {
+        const uint32_t n = dc_chunks(A.cu[b], A.cu[b + 1u], A.n_tokens);
+        mine += n;
+        atomicAdd(&s_kind[min(n, DC_KINDS - 1u)], 1u);
+    }
     uint64_t at = mine;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) { const uint64_t y = __shfl_up_sync(0xffffffffu, at, w); if (lane >= (uint32_t)w) at += y; }
-    if (lane == 31u) s_sum[tid >> 5] = at;
+    if (lane == 31u) s_sum[warp] = at;
     __syncthreads();
-    for (uint32_t w = 0; w < tid >> 5; ++w) at += s_sum[w];
+    for (uint32_t w = 0; w < warp; ++w) at += s_sum[w];
     at -= mine;
+    const uint32_t kind = DC_KINDS - 1u - tid, many = s_kind[kind], upto = dc_warp_sum_to(many);       // thread 0 has the longest
+    if (lane == 31u) s_part[warp] = upto;
+    __syncthreads();
+    uint32_t to = upto - many;
+    for (uint32_t w = 0; w < warp; ++w) to += s_part[w];
+    s_kind[kind] = to;
+    __syncthreads();
     for (uint32_t b = b0; b < b1; ++b) {
-        plan[b] = (uint32_t)min(at, (uint64_t)0xffffffffu);
-        at += dc_chunks(A.cu[b], A.cu[b + 1u], A.n_tokens);
+        const int32_t lo = A.cu[b], hi = A.cu[b + 1u];
+        const uint32_t n = dc_chunks(lo, hi, A.n_tokens), first = (uint32_t)min(at, (uint64_t)0xffffffffu);
+        at += n;
+        dc_firsts(plan, n_seqs)[b] = first;
+        plan[atomicAdd(&s_kind[min(n, DC_KINDS - 1u)], 1u)] = DcSeq{b, first, lo, hi};
     }
 }
 
@@ -161,7 +201,7 @@ __device__ __forceinline__ void dc_block_product(float (&c)[2][4], const uint32_
 
 // WIDE: more than two value heads a key head (the products are then kept for the next two)
 template <class T, int DIG, bool WIDE>
-__global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_seqs, uint8_t *ws, uint64_t slots, uint32_t *plan) {
+__global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_seqs, uint8_t *ws, uint64_t slots, const DcSeq *plan) {
     pdl_prologue();
     extern __shared__ __align__(128) uint8_t sm[];           // the digits; then the matrices A and T of two value heads
     __shared__ float s_red[2][8], s_beta[2][DC_T], s_diag[2][4], s_amax[2][4], s_peak[2];
@@ -169,9 +209,9 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_s
     __shared__ uint32_t s_bad[2][2];             // tokens whose key or query is not finite
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, kh = blockIdx.y, width = A.rank / A.groups;
     const uint64_t slot = blockIdx.x;
-    uint32_t b, chunk;
-    if (!dc_find(A, n_seqs, plan, blockIdx.x, b, chunk)) return;
-    const int32_t lo = A.cu[b], hi = A.cu[b + 1u];
+    int32_t lo, hi;
+    uint32_t chunk;
+    if (!dc_find(A, n_seqs, plan, blockIdx.x, lo, hi, chunk)) return;
     const uint32_t t0 = (uint32_t)lo + chunk * DC_T, n = min((uint32_t)DC_T, (uint32_t)hi - t0);
     uint8_t *const keys = ws + (slot * A.groups + kh) * dc_keys(DIG), *const recs = ws + slots * A.groups * dc_keys(DIG) + slot * A.rank * DC_REC;
     const uint32_t dv = warp == 0u ? 0u : warp == 7u ? 1u : 2u;          // the value head of a pair whose decays this warp makes (2: none): the warps with the fewest products
@@ -581,34 +621,24 @@ __device__ __forceinline__ void dc_put32(const float *x, float f, uint32_t hi, u
 }
 
 template <class T, int DIG>
-__global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, const uint32_t *plan) {
+__global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, const DcSeq *plan) {
     pdl_prologue();
     constexpr uint32_t KEYS = dc_keys(DIG), VROW = DC_S * sizeof(T);
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ __align__(8) uint64_t s_bar[DB_COUNT];
     __shared__ float s_ex[4][2][DC_S];
-    __shared__ uint32_t s_from[2][DC_S], s_seq, tmem_slot;
+    __shared__ uint32_t s_from[2][DC_S], tmem_slot;
     __shared__ volatile uint32_t fail;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t h = blockIdx.x, kh = h / (A.rank / A.groups);
-    // long sequences first: the block's sequence is the blockIdx.y-th longest (of many, they are taken as they come)
-    uint32_t b = blockIdx.y + A.first_seq;
-    if (n_seqs > 1u && n_seqs <= 1024u) {
-        for (uint32_t i = tid; i < n_seqs; i += DC_THREADS) {
-            const int64_t mine = (int64_t)A.cu[i + 1u] - A.cu[i];
-            uint32_t before = 0u;
-            for (uint32_t j = 0; j < n_seqs; ++j) { const int64_t other = (int64_t)A.cu[j + 1u] - A.cu[j]; before += other > mine || (other == mine && j < i); }
-            if (before == blockIdx.y) s_seq = i;
-        }
-        __syncthreads();
-        b = s_seq;
-    }
-    const int32_t lo = A.cu[b], hi = A.cu[b + 1u];
+    __shared__ DcSeq seq;
+    dc_seq(A, n_seqs, plan, A.first_seq + blockIdx.y, seq);
+    const int32_t lo = seq.lo, hi = seq.hi;
     if (lo < 0 || hi < lo || (uint32_t)hi > A.n_tokens) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
-    const int32_t state_slot = delta_slot(A.slots, A.n_slots, b, A.status);
+    const int32_t state_slot = delta_slot(A.slots, A.n_slots, seq.b, A.status);
     if (state_slot < 0 || lo == hi) return;
     const uint32_t chunks = ((uint32_t)(hi - lo) + DC_T - 1u) / DC_T;
-    if (plan[b] + (uint64_t)chunks > slots) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
+    if (seq.first + (uint64_t)chunks > slots) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
     uint8_t *const s_kq = sm, *const s_kt = sm + DIG * DC_KQ, *const s_tt = sm + KEYS, *const s_pp = s_tt + 2u * DC_SQ, *const s_meta = s_tt + 4u * DC_SQ;
     T *const s_v = reinterpret_cast<T *>(s_meta + 2u * sizeof(DcMeta)), *const s_out = s_v + DC_T * DC_S;          // [token][row]
     auto bar = [&](uint32_t i) { return dc_smem(&s_bar[i]); };
@@ -636,7 +666,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(DC_REGS_CONTROL));
         if (warp == DC_CONTROL) {
             const uint32_t leader = tc_elect();
-            const uint64_t slot0 = plan[b];          // here: the warps of the rows have no register for it
+            const uint64_t slot0 = seq.first;
             const uint8_t *key = ws + (slot0 * A.groups + kh) * KEYS, *rec = ws + slots * A.groups * KEYS + (slot0 * A.rank + h) * DC_REC;      // the next chunk's, as each is asked for
             const uint64_t key_step = (uint64_t)A.groups * KEYS, rec_step = (uint64_t)A.rank * DC_REC;
             auto get_kq = [&](uint32_t c) { if (lane == 0u) { expect(DB_KQ, DIG * DC_KQ); copy(DB_KQ, s_kq, key + c * key_step, DIG * DC_KQ); } };
@@ -951,7 +981,7 @@ __device__ __forceinline__ float dn_most(const float (&x)[16]) {
 }
 
 template <class T, int DIG>
-__global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A, const uint8_t *ws, uint64_t slots, const uint32_t *plan) {
+__global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, const DcSeq *plan) {
     pdl_prologue();
     constexpr uint32_t KEYS = dc_keys(DIG), SPLIT = DC_S / DN_ROWS;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -960,13 +990,15 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A,
     __shared__ uint32_t s_from[4][DN_ROWS], tmem_slot;       // first tokens from which a row is no number (64: none), of a chunk in turn
     __shared__ volatile uint32_t fail;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const uint32_t h = blockIdx.x / SPLIT, n0 = blockIdx.x % SPLIT * DN_ROWS, kh = h / (A.rank / A.groups), b = blockIdx.y;
-    const int32_t lo = A.cu[b], hi = A.cu[b + 1u];
+    const uint32_t h = blockIdx.x / SPLIT, n0 = blockIdx.x % SPLIT * DN_ROWS, kh = h / (A.rank / A.groups);
+    __shared__ DcSeq seq;
+    dc_seq(A, n_seqs, plan, blockIdx.y, seq);
+    const int32_t lo = seq.lo, hi = seq.hi;
     if (lo < 0 || hi < lo || (uint32_t)hi > A.n_tokens) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
-    const int32_t state_slot = delta_slot(A.slots, A.n_slots, b, A.status);
+    const int32_t state_slot = delta_slot(A.slots, A.n_slots, seq.b, A.status);
     if (state_slot < 0 || lo == hi) return;
     const uint32_t chunks = ((uint32_t)(hi - lo) + DC_T - 1u) / DC_T;
-    const uint64_t slot0 = plan[b];
+    const uint64_t slot0 = seq.first;
     if (slot0 + chunks > slots) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
     uint8_t *const s_kq = sm, *const s_kt = sm + DIG * DC_KQ, *const s_tp = sm + KEYS, *const s_s = s_tp + 2u * DN_SQ, *const s_r = s_s + 2u * DN_STILE, *const s_d = s_r + 2u * DN_TILE, *const s_dk = s_d + 2u * DN_TILE,
                   *const s_meta = s_dk + 2u * DN_TILE;
@@ -1255,16 +1287,16 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_delta_chunk_rows(DeltaArgs A,
 
 static uint64_t dc_records(int dig, uint32_t groups, uint32_t rank, uint64_t slots) { return slots * ((uint64_t)groups * dc_keys(dig) + (uint64_t)rank * DC_REC); }
 uint64_t delta_chunk_workspace(uint32_t type, uint32_t groups, uint32_t rank, uint32_t n_tokens, uint32_t n_seqs) {
-    return dc_records(type == VT_F32 ? 2 : 1, groups, rank, dc_slots(n_tokens, n_seqs)) + n_seqs * 4ull;
+    return dc_records(type == VT_F32 ? 2 : 1, groups, rank, dc_slots(n_tokens, n_seqs)) + (n_seqs > DC_NEAR ? n_seqs * (sizeof(DcSeq) + 4ull) : 0u);
 }
 
-template <class T, int DIG> static int launch_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, const uint32_t *plan, cudaStream_t s) {
+template <class T, int DIG> static int launch_chunk(DeltaArgs A, uint32_t n_seqs, const uint8_t *ws, uint64_t slots, const DcSeq *plan, cudaStream_t s) {
     // Four blocks a state where that gives no multiprocessor two, and sequences of four chunks on the average: 32 heads, 1 sequence of 64 tokens 25.6 -> 27.5 us in F32 (21.5 -> 21.0 in BF16), of 128 30 -> 34 (24 -> 27), of 256
     // 40 -> 41 (33 -> 32), of 500 56 -> 52 (49 -> 43), of 2000 172 -> 136 (156 -> 131), of 8000 606 -> 519 (561 -> 482), each with the preparation. In two turns four blocks would take 5.5 us a chunk, one takes 4.
     if ((uint64_t)A.rank * n_seqs * (DC_S / DN_ROWS) <= sm_count() && A.n_tokens >= 256u * (uint64_t)n_seqs) {
         static std::atomic<uint64_t> set_rows{0};
         if (!raise_smem_limit(reinterpret_cast<const void *>(k_delta_chunk_rows<T, DIG>), dn_smem_bytes(DIG), set_rows)) return 0;
-        RC_LAUNCH((k_delta_chunk_rows<T, DIG>), dim3(A.rank * (DC_S / DN_ROWS), n_seqs), DN_THREADS, dn_smem_bytes(DIG), s, A, ws, slots, plan);
+        RC_LAUNCH((k_delta_chunk_rows<T, DIG>), dim3(A.rank * (DC_S / DN_ROWS), n_seqs), DN_THREADS, dn_smem_bytes(DIG), s, A, n_seqs, ws, slots, plan);
         RC_LAUNCHED();
         return 1;
     }
@@ -1281,7 +1313,7 @@ template <class T, int DIG> static int launch_chunks(const DeltaArgs &A, uint32_
     const uint64_t slots = dc_slots(A.n_tokens, n_seqs);
     constexpr size_t smem = 4u * DC_MAT > DIG * DC_KQ ? 4u * DC_MAT : DIG * DC_KQ;
     RC_REQUIRE(slots <= 0x7fffffffu && A.groups <= 65535u, "delta rule: too many chunks");
-    uint32_t *const plan = (uint32_t *)(ws + dc_records(DIG, A.groups, A.rank, slots));
+    DcSeq *const plan = (DcSeq *)(ws + dc_records(DIG, A.groups, A.rank, slots));
     prof_begin("delta_prep", s);
     if (n_seqs > DC_NEAR) {
         RC_LAUNCH(k_delta_plan, 1, 1024, 0, s, A, n_seqs, plan);

@@ -154,3 +154,26 @@ def test_more_sequences_than_a_grid_has_rows():
     rows = torch.cat([torch.arange(b * each, b * each + each) for b in some]).cuda()
     assert bool(((out[rows].double() - want[rows]).abs() <= unit / math.sqrt(S) + torch.finfo(out.dtype).eps / 2 * want[rows].abs()).all())
     assert not bool((out == 7.0).all(-1).any())           # every row is written
+
+
+def test_a_sequence_costs_the_same_among_many():
+    """The time of a call goes with its sequences: 1000 of them once took six times as long as 1100, as every block of the former looked at all of them for its own place. Twice is allowed here."""
+    def time_of(n):
+        x = _inputs(6, 64 * n, 4, 8, torch.bfloat16, n)
+        dims = rc.DeltaDims(30, 4, 8, S)
+        cu, out = torch.arange(n + 1, dtype=torch.int32, device="cuda") * 64, torch.empty_like(x["v"])
+        work = _workspace(dims, 64 * n, n)
+        torch.cuda.synchronize()
+        times = []
+        for _ in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            rc.delta_rule_device(dims, 64 * n, n, cu.data_ptr(), 0, n, *[x[y].data_ptr() for y in ("q", "k", "v", "gate", "beta")], x["state"].data_ptr(), out.data_ptr(), work.data_ptr(),
+                                 work.numel(), torch.cuda.current_stream().cuda_stream)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        rc.device_status()
+        return sorted(times[1:])[2] / n
+
+    assert time_of(1000) <= 2 * time_of(1100)
