@@ -67,19 +67,24 @@ uint32_t *status_words() {
     return g_status;
 }
 int status_failed() {
-    volatile uint32_t *st = g_status;
-    if (!st) return 0;
-    const uint32_t a = st[ST_ROUTER_NONFINITE], b = st[ST_TOKEN_RANGE], c = st[ST_EXPERT_RANGE], d = st[ST_TIMEOUT];
-    const uint32_t pg = st[ST_PAGE_RANGE], sl = st[ST_SLOT], sq = st[ST_SEQ_BOUNDS];
-    if (!(a | b | c | d | pg | sl | sq)) return 0;
-    for (uint32_t i = 0; i < ST_WORDS; ++i) st[i] = 0;
-    if (a) set_error("invalid router softmax denominator (non-finite router logits)");
-    else if (b) set_error("token id out of range on the device (non-finite logits in the argmax?)");
-    else if (c) set_error("an expert id outside this shard reached an expert kernel");
-    else if (pg) set_error("a position beyond a sequence's page table, or a page id outside the cache");
-    else if (sl) set_error("a state slot outside the states, or one that two sequences of a call share");
-    else if (sq) set_error("sequence bounds that do not ascend within the rows of the call");
-    else set_error("a kernel gave up waiting for a copy or a product (bounded wait ran out); its outputs are incomplete");
+    if (!g_status) return 0;
+    static const struct { uint32_t word; const char *text; } reports[] = {
+        {ST_ROUTER_NONFINITE, "invalid router softmax denominator (non-finite router logits)"},
+        {ST_TOKEN_RANGE, "token id out of range on the device (non-finite logits in the argmax?)"},
+        {ST_EXPERT_RANGE, "an expert id outside this shard reached an expert kernel"},
+        {ST_PAGE_RANGE, "a position beyond a sequence's page table, or a page id outside the cache"},
+        {ST_SLOT, "a state slot outside the states, or one that two sequences of a call share"},
+        {ST_SEQ_BOUNDS, "sequence bounds that do not ascend within the rows of the call"},
+        {ST_TIMEOUT, "a kernel gave up waiting for a copy or a product (bounded wait ran out); its outputs are incomplete"},
+    };
+    static_assert(sizeof(reports) / sizeof(reports[0]) == ST_WORDS, "a text for every word");
+    char text[1024];
+    int n = 0;
+    text[0] = 0;
+    for (const auto &r : reports)      // read and cleared at once: a kernel of another stream may report meanwhile
+        if (__atomic_exchange_n(&g_status[r.word], 0u, __ATOMIC_ACQ_REL) && n < (int)sizeof(text)) n += snprintf(text + n, sizeof(text) - n, "%s%s", n ? "; " : "", r.text);
+    if (!n) return 0;
+    set_error("%s", text);
     return 1;
 }
 

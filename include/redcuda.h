@@ -259,7 +259,7 @@ int redcuda_profile_report(char *buf, size_t cap);
  * refused are refused before anything is launched.
  * ---------------------------------------------------------------------------------------------------------- */
 
-/* 1 when no kernel has reported anything since the last failure that was read, else 0 with a message (and the reports are
+/* 1 when no kernel has reported anything since the last failure that was read, else 0 with a message that names every kind of report (and they are
  * cleared). The caller waits for the stream first. */
 int redcuda_device_status(void);
 
