@@ -12,6 +12,7 @@
 #include <string.h>
 #include <map>
 #include <mutex>
+#include <thread>
 #include <vector>
 
 namespace rc {
@@ -26,24 +27,28 @@ void set_error(const char *fmt, ...) {
 }
 
 // ---- per-kernel event timing ----
-struct ProfRec { const char *tag; cudaEvent_t a, b; };
+struct ProfRec { const char *tag; cudaEvent_t a, b; cudaStream_t stream; std::thread::id thread; bool open; };
 static bool g_prof_on = false;
 static std::vector<ProfRec> g_prof;
 static std::mutex g_prof_mu;
 
 void prof_begin(const char *tag, cudaStream_t s) {
     if (!g_prof_on) return;
-    ProfRec r{tag, nullptr, nullptr};
+    ProfRec r{tag, nullptr, nullptr, s, std::this_thread::get_id(), true};
     if (cudaEventCreate(&r.a) != cudaSuccess || cudaEventCreate(&r.b) != cudaSuccess) return;
     cudaEventRecord(r.a, s);
     std::lock_guard<std::mutex> lk(g_prof_mu);
     g_prof.push_back(r);
 }
 bool prof_active() { return g_prof_on; }
+// ends the innermost record that this thread has open on the stream: brackets may lie in one another, and threads launch at once
 void prof_end(cudaStream_t s) {
     if (!g_prof_on) return;
     std::lock_guard<std::mutex> lk(g_prof_mu);
-    if (!g_prof.empty()) cudaEventRecord(g_prof.back().b, s);
+    for (size_t i = g_prof.size(); i-- > 0;) {
+        ProfRec &r = g_prof[i];
+        if (r.open && r.stream == s && r.thread == std::this_thread::get_id()) { cudaEventRecord(r.b, s); r.open = false; return; }
+    }
 }
 
 int pdl_mode() {
@@ -565,7 +570,7 @@ int redcuda_profile_report(char *buf, size_t cap) {
     std::map<std::string, std::pair<uint64_t, double>> agg;
     for (auto &r : g_prof) {
         float ms = 0.f;
-        if (r.a && r.b && cudaEventElapsedTime(&ms, r.a, r.b) == cudaSuccess) { auto &e = agg[r.tag]; e.first += 1; e.second += ms; }
+        if (!r.open && r.a && r.b && cudaEventElapsedTime(&ms, r.a, r.b) == cudaSuccess) { auto &e = agg[r.tag]; e.first += 1; e.second += ms; }
     }
     cudaGetLastError();
     size_t pos = 0; int n = 0;
