@@ -808,23 +808,24 @@ int redcuda_kv_attend_device(const redcuda_paged_kv *kv, const int32_t *table_de
                "kv attend: row strides %llu and %llu (multiples of 16 bytes, at least a row)", (unsigned long long)q_stride, (unsigned long long)new_stride);
     RC_REQUIRE(aligned16(q_dev) && aligned16(k_new_dev) && aligned16(v_new_dev) && aligned16(out_dev) && aligned16(workspace_dev), "kv attend: a pointer is not 16-byte aligned");
     const uint64_t out_bytes = (uint64_t)n_seqs * qrow * qs;
+    // what the call needs of the workspace, which may begin an arena with other arrays of the call behind it; without a device, which refuses the call anyway, all that is given
+    const uint32_t sms = sm_count(), most_blocks = sms * kv_blocks(val_size(kv->type), hd);
+    const uint64_t need = attend_workspace(most_blocks, hd), ws_bytes = sms && need < workspace_bytes ? need : workspace_bytes;
     RC_REQUIRE(!overlap(out_dev, out_bytes, q_dev, span_bytes(n_seqs, q_stride, qrow, qs)) && !overlap(out_dev, out_bytes, k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) &&
                !overlap(out_dev, out_bytes, v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)), "kv attend: the output lies inside the inputs");
     RC_REQUIRE(aligned4(table_dev) && aligned4(lens_dev) && aligned4(lse_dev), "kv attend: whole numbers or lse are not 4-byte aligned");
-    RC_REQUIRE(!kv_overlap(kv, st, out_dev, out_bytes) && !kv_overlap(kv, st, q_dev, span_bytes(n_seqs, q_stride, qrow, qs)) && !kv_overlap(kv, st, workspace_dev, workspace_bytes) &&
+    RC_REQUIRE(!kv_overlap(kv, st, out_dev, out_bytes) && !kv_overlap(kv, st, q_dev, span_bytes(n_seqs, q_stride, qrow, qs)) && !kv_overlap(kv, st, workspace_dev, ws_bytes) &&
                !kv_overlap(kv, st, k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) && !kv_overlap(kv, st, v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)) &&
                !kv_overlap(kv, st, lse_dev, (uint64_t)n_seqs * n_q * 4u), "kv attend: rows, output or workspace lie inside the cache");
-    const Span written[3] = {{out_dev, out_bytes}, {lse_dev, (uint64_t)n_seqs * n_q * 4u}, {workspace_dev, workspace_bytes}};
+    const Span written[3] = {{out_dev, out_bytes}, {lse_dev, (uint64_t)n_seqs * n_q * 4u}, {workspace_dev, ws_bytes}};
     const Span read[5] = {{q_dev, span_bytes(n_seqs, q_stride, qrow, qs)}, {k_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)}, {v_new_dev, span_bytes(n_seqs, new_stride, nrow, qs)},
                           {table_dev, (uint64_t)n_seqs * table_width * 4u}, {lens_dev, (uint64_t)n_seqs * 4u}};
     RC_REQUIRE(!spans_overlap(written, read), "kv attend: output, lse or workspace overlap one another or the inputs");
     RC_REQUIRE(!kv_overlap(kv, st, table_dev, read[3].n) && !kv_overlap(kv, st, lens_dev, read[4].n), "kv attend: the page table or the lengths lie inside the cache");
     RC_REQUIRE(!(scale != scale), "kv attend: scale is not a number");
     if (!require_device()) return 0;
-    const uint32_t sms = sm_count();
     RC_REQUIRE(sms, "kv attend: the device's size is not known");
-    const uint32_t most_blocks = sms * kv_blocks(val_size(kv->type), hd);
-    RC_REQUIRE(workspace_dev && workspace_bytes >= attend_workspace(most_blocks, hd), "kv attend: a workspace of %llu bytes is needed", (unsigned long long)attend_workspace(most_blocks, hd));
+    RC_REQUIRE(workspace_dev && workspace_bytes >= need, "kv attend: a workspace of %llu bytes is needed", (unsigned long long)need);
     AttendArgs A{};
     A.k = kv->k; A.v = kv->v; A.page_stride = st[0]; A.token_stride = st[1]; A.head_stride = st[2];
     A.table = table_dev; A.table_width = table_width; A.page_size = kv->page_size; A.n_pages = kv->n_pages;
