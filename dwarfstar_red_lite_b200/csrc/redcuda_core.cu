@@ -86,8 +86,8 @@ int status_failed() {
     char text[1024];
     int n = 0;
     text[0] = 0;
-    for (const auto &r : reports)      // read and cleared at once: a kernel of another stream may report meanwhile
-        if (__atomic_exchange_n(&g_status[r.word], 0u, __ATOMIC_ACQ_REL) && n < (int)sizeof(text)) n += snprintf(text + n, sizeof(text) - n, "%s%s", n ? "; " : "", r.text);
+    for (const auto &r : reports)      // a word that is set is read and cleared at once: a kernel of another stream may report meanwhile
+        if (__atomic_load_n(&g_status[r.word], __ATOMIC_RELAXED) && __atomic_exchange_n(&g_status[r.word], 0u, __ATOMIC_ACQ_REL) && n < (int)sizeof(text)) n += snprintf(text + n, sizeof(text) - n, "%s%s", n ? "; " : "", r.text);
     if (!n) return 0;
     set_error("%s", text);
     return 1;
