@@ -199,7 +199,7 @@ __device__ __forceinline__ void dc_block_product(float (&c)[2][4], const uint32_
     }
 }
 
-// WIDE: more than two value heads a key head (the products are then kept for the next two)
+// WIDE: more than two value heads a key head (the products are then kept for the next two, which spills 136 to 168 bytes a thread)
 template <class T, int DIG, bool WIDE>
 __global__ void __launch_bounds__(256, 3) k_delta_prep(DeltaArgs A, uint32_t n_seqs, uint8_t *ws, uint64_t slots, const DcSeq *plan) {
     pdl_prologue();
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1) k_delta_chunk(DeltaArgs A, uint
     const uint32_t h = blockIdx.x, kh = h / (A.rank / A.groups);
     __shared__ DcSeq seq;
     dc_seq(A, n_seqs, plan, A.first_seq + blockIdx.y, seq);
-    const int32_t lo = seq.lo, hi = seq.hi;
+    const int32_t &lo = seq.lo, &hi = seq.hi;     // read where they are wanted: the warps of the rows have no registers for them
     if (lo < 0 || hi < lo || (uint32_t)hi > A.n_tokens) { if (A.status && tid == 0u) A.status[ST_SEQ_BOUNDS] = 1u; return; }
     const int32_t state_slot = delta_slot(A.slots, A.n_slots, seq.b, A.status);
     if (state_slot < 0 || lo == hi) return;
