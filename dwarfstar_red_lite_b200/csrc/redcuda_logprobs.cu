@@ -106,8 +106,8 @@ template <class T> __device__ __forceinline__ float lp_most(uint4 w) {
 }
 
 // What bounds it is the row's bytes for 32-bit logits (592 rows of 151936: 56 us, 6.4 TB/s) and instructions for 16-bit ones (seven a value, one of them an exponential at a
-// sixteenth of the fp32 rate: 777 rows 50 us, 4.8 TB/s). A round's loads are on their way while the last one's values are added up; four blocks an SM for 32 bits, three for 16, which spill with four
-// (777 rows 65 us).
+// sixteenth of the fp32 rate: 777 rows 50 us, 4.8 TB/s). A round's loads are on their way while the last one's values are added up; four blocks an SM for 32 bits, three for 16, which have to
+// spill more with four (777 rows 65 us); as they are, each of the three forms spills one register.
 // The alternatives cost one comparison a lane and round of LP_UNROLL pieces where there are none: a warp keeps its 32 largest keys, one a
 // lane, and looks at single values only where the largest of a lane's round reaches what is known to be among the row's n largest. That is the n-th of the warp's own,
 // or the least of the warps' ceil(n / LP_WARPS)-th largest, which every warp publishes (n values are at least that large; a stale one is a lower bound too), or in a warp's first

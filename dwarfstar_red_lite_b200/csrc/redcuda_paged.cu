@@ -131,8 +131,9 @@ __device__ __forceinline__ uint64_t kv_request(const AttendArgs &A, uint32_t b, 
 }
 
 // A warp's share of a part: every KV_WARPS-th tile of [t0, t1), up to NH query heads; (m, l, O) to shared memory. For a cache of floats the sums on CUDA cores, 32 / NH positions at a time:
-// their 32 scores are summed over the lanes together and end in a lane each. What bounds it is instructions: 4 NH of a warp for a position's products and some 20 for the rest (packed fp32), where the
-// bytes of a position of 128 leave an SM 23 cycles; hence the form for 4 heads.
+// their 32 scores are summed over the lanes together and end in a lane each. A position costs a warp 4 NH instructions for its products and some 20 for the rest (packed fp32), where the bytes of a position of 128 leave
+// an SM 23 cycles; hence the form for 4 heads. With it no pipe is the bound: 24 sequences of 500 to 1999 positions, 32 heads over 8 of 128, 45.7 us: issue slots 44 %, fp32 pipe 29 %, DRAM 61 % of nominal, and the
+// warps' first stall is on global memory (the next tile of a ring of two).
 template <class T, class QT, int HD, int NH>
 __device__ __forceinline__ void attend_part_f32(const AttendArgs &A, uint32_t b, uint32_t kvh, uint32_t h0, uint32_t nh, uint32_t len, uint32_t t0, uint32_t t1,
                                             uint8_t *ring, uint64_t *valid, float *p_sh, float *m_out, float *l_out, float *o_out) {
@@ -457,6 +458,7 @@ __device__ __forceinline__ void kv_write_new(const AttendArgs &A, uint32_t b, ui
 }
 
 // NH: heads that a group can have (4 only for a cache of floats)
+// Over 16-bit caches it takes all 255 registers, and with heads of 64 and 256 spills 36 to 56 bytes a thread; over floats with heads of 128 and eight query heads 168, and 36 bytes.
 template <class T, class QT, int HD, int NH>
 __global__ void __launch_bounds__(KV_WARPS * 32, kv_blocks(sizeof(T), HD)) k_kv_attend(AttendArgs A) {
     pdl_prologue();
@@ -576,7 +578,7 @@ __global__ void __launch_bounds__(256) k_kv_attend_join(AttendArgs A) {
 #pragma unroll
     for (uint32_t i = 0; i < AHEAD; ++i) x[i] = row + i * ROWS <= n ? part(row + i * ROWS) : make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, l = 0.f;
-    for (uint32_t p = tid; p <= n; p += 256u) {  // once, unless a device has more than 256 multiprocessors
+    for (uint32_t p = tid; p <= n; p += 256u) {  // a head can have as many parts as there are blocks: two or four an SM
         const float m = A.part_ml[slot(p) * 16u + h], lp = A.part_ml[slot(p) * 16u + 8u + h], to = fmaxf(M, m), z = to == -INFINITY ? 0.f : to;
         l = l * exp2f(M - z) + lp * exp2f(m - z);
         M = to;

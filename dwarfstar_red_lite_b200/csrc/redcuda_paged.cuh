@@ -7,7 +7,7 @@ namespace rc {
 // Warps and stages of a block, blocks of a multiprocessor: twelve stages of 16 KB an SM in every form. Six warps x two stages x one block: two documents of 131072 and some 115000 positions 86 us, 64 ragged
 // sequences 22, 238 of 147 positions 42, 205 of up to 33 36; three x two x two 89, 20, 35, 24 (one block's head begins or ends while the other's tiles flow); two x three x two 90, 21, 36, 25;
 // two x two x three 93, 21, 34, 22.
-// Caches of floats with heads of up to 128 wait for their arithmetic, not for bytes, and have the registers for twelve warps an SM: tiles of 8 KB and twice the blocks. us, 16 KB x two blocks -> 8 KB x four: heads of 128, 32 over 8, 24 sequences
+// Caches of floats with heads of up to 128 have the registers for twelve warps an SM, which wait less for one another's tiles: tiles of 8 KB and twice the blocks. us, 16 KB x two blocks -> 8 KB x four: heads of 128, 32 over 8, 24 sequences
 // of 500 to 1999 positions 48.8 -> 45.7, 64 of up to 2048 42.8 -> 32.5, 200 of up to 40 31 -> 23, 4 of 30000 to 60000 242 -> 234; 64 over 8 76 -> 60; heads of 64, 8 over 8 37.9 -> 29.5.
 // 16-bit caches with heads of 128 lose by the same what they gain: 200 of up to 40 28 -> 22, 64 of up to 2048 24.2 -> 22.6, 1 of 8000 12.8 -> 14.8, 24 of 500 to 1999 26.5 -> 28.1.
 constexpr int KV_WARPS = 3, KV_STAGES = 2, KV_BLOCKS = 2;

@@ -288,7 +288,9 @@ int redcuda_kv_append_device(const redcuda_paged_kv *kv, const int32_t *table_de
  * outside the inputs), lse_dev [n_seqs][n_q] F32 or NULL. scale 0: 1 / sqrt(head_dim). With k_new_dev / v_new_dev (both or neither; q_type, new_stride as
  * row_stride above) the sequences' new rows are first written to position lens[b] - 1, so that a decode step is one call. A sequence of no positions
  * (lens[b] <= 0) has nothing written to the cache, out = 0 and lse = -infinity. Positions whose page is not in the cache are left out.
- * Types: q_type F32 with a cache of F32 or F16, or q_type equal to the cache's type. With an F16 or BF16 cache an infinity in a row that is
+ * Types: q_type F32 with a cache of F32 or F16, or q_type equal to the cache's type. Sums are F32; over an F16 cache F32 queries and the softmax weights enter the products with 22 bits, over a BF16
+ * cache the weights with 16 (one to two outputs in a thousand are then the neighbour of the nearest BF16). Few sequences go in one launch where table_width * page_size is small (up to 1536 positions with 16-bit
+ * heads of 256, more with smaller ones, fewer with floats); a wider table costs them some 2 us. With an F16 or BF16 cache an infinity in a row that is
  * attended to gives NaN. workspace_dev: redcuda_kv_attend_workspace bytes (for n_q heads on the current device, any batch; 0 = invalid
  * arguments), 16-byte aligned; calls that overlap on the GPU need one each. */
 uint64_t redcuda_kv_attend_workspace(const redcuda_paged_kv *kv, uint32_t n_q);
@@ -318,7 +320,8 @@ int redcuda_delta_step_device(const redcuda_delta_dims *d, uint32_t n_seqs, cons
  * of sequences that then claim the same rows, outputs and states are not defined (where they claim more than the workspace has room for, sequences behind them are reported and left out too). A value that is not finite makes what depends on it NaN, from its token on. In longer calls
  * (those that need a workspace) the keys of 64 tokens share an exponent in the products, as do their queries and 32 rows of values or of the
  * state: one 2^17 smaller than the largest beside it keeps 22 bits, smaller ones fewer. Slots as above. workspace_dev:
- * redcuda_delta_rule_workspace bytes, 16-byte aligned (0: none is needed); calls that overlap on the GPU need one each. */
+ * redcuda_delta_rule_workspace bytes for these numbers, 16-byte aligned (0: none is needed; fewer sequences with as many tokens may need more); calls that overlap on the GPU need one each.
+ * A call goes one way for all of its sequences: in chunks of 64 tokens where d_state is 128 and n_tokens >= 24 n_seqs + 32, else a token at a time. A long prompt among many single tokens is better off in a call of its own. */
 uint64_t redcuda_delta_rule_workspace(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs);
 int redcuda_delta_rule_device(const redcuda_delta_dims *d, uint32_t n_tokens, uint32_t n_seqs, const int32_t *cu_seqlens_dev, const int32_t *slots_dev,
                               uint32_t n_slots, const void *q_dev, const void *k_dev, const void *v_dev, const float *gate_dev, const float *beta_dev,
