@@ -177,3 +177,40 @@ def test_a_sequence_costs_the_same_among_many():
         return sorted(times[1:])[2] / n
 
     assert time_of(1000) <= 2 * time_of(1100)
+
+
+@pytest.mark.parametrize("n", [20, 40])
+def test_replayed_with_other_bounds(n):
+    """A captured call follows its bounds: ragged, most sequences empty, one with every row, some that cannot be, none with a row, and ragged again, all over the same workspace."""
+    T = 24 * n + 200
+    x = _inputs(7, T, 2, 4, torch.float32, n)
+    dims = rc.DeltaDims(0, 2, 4, S)
+    slots = list(range(n - 1, -1, -1))
+    cu, sl = torch.zeros(n + 1, dtype=torch.int32, device="cuda"), torch.tensor(slots, dtype=torch.int32, device="cuda")
+    state, out, work = x["state"].clone(), torch.full_like(x["v"], 7.0), _workspace(dims, T, n)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        rc.delta_rule_device(dims, T, n, cu.data_ptr(), sl.data_ptr(), n, *[x[y].data_ptr() for y in ("q", "k", "v", "gate", "beta")], state.data_ptr(), out.data_ptr(), work.data_ptr(),
+                             work.numel(), stream.cuda_stream)
+    ragged = np.sort(np.random.default_rng(n).integers(0, T + 1, n + 1)).tolist()
+    bad = [24 * b for b in range(n + 1)]
+    bad[3], bad[n - 4] = T + 1, -1
+    for bounds in (ragged, [0] * (n - 2) + [70, 70, 199], [0] * 5 + [T] * (n - 4), bad, [T] * (n + 1), ragged):
+        cu.copy_(torch.tensor(bounds, dtype=torch.int32))
+        state.copy_(x["state"])
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        served = [b for b in range(n) if 0 <= bounds[b] < bounds[b + 1] <= T]
+        if bounds is bad:
+            with pytest.raises(rc.RedcudaError, match="bounds"):
+                rc.device_status()
+        else:
+            rc.device_status()
+        if served:
+            _check(x, bounds, slots, served, state, out)
+        else:
+            assert torch.equal(state, x["state"]) and bool((out == 7.0).all())
+    del graph
