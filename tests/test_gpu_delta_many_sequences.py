@@ -45,7 +45,7 @@ def _reference(x, begin, lens, slots):
 
 
 def _workspace(dims, T, n):
-    """Bytes of a workspace and its fill: another call's records, so that what is left over in it looks like records."""
+    """A workspace whose bytes are all ones: NaN as numbers, and nothing that a call may go by."""
     work = torch.full((dims.workspace(T, n),), 0xff, dtype=torch.uint8, device="cuda")
     assert work.numel()                                   # the form in chunks
     return work
